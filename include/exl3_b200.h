@@ -259,6 +259,85 @@ int exl3_ep_p2p_combine(void* window, int world, int rank, int64_t capacity, int
 int exl3_ep_window_recv(int world, int64_t capacity, int64_t hidden, int topk, int x_dtype, int partial_dtype,
                         size_t* x_off, size_t* ids_off, size_t* w_off);
 
+/* A decoder step's paged key/value cache, held in 8 bits (the reference
+ * leaves the cache to its serving engine).  Tokens of a request fill pages of
+ * `page` tokens (16, 32, 64 or 128); block_table[b][i] (int32, row stride
+ * `width`) is the page of request b's tokens [i * page, (i + 1) * page).
+ * k_cache and v_cache are codes [pages][kv_heads][page][dim], one byte each
+ * (dim 64 or 128), k_scale and v_scale fp32 [pages][kv_heads]: value =
+ * code * scale.  A scale is a power of two, the smallest that brings the
+ * block's largest magnitude within the codes' range (448 for e4m3, 127 for
+ * int8; exponents -40..40). */
+enum { EXL3_KV_E4M3 = 0, EXL3_KV_INT8 = 1 };
+#define EXL3_KV_MAX_REQUESTS 16384
+
+/* The step's bookkeeping from request lengths, in one launch: request b holds
+ * lens[b] tokens and adds new_tokens[b].  Writes kv_lens[b] = lens[b] +
+ * new_tokens[b]; cu_tokens [requests + 1], the requests' first token rows;
+ * for each token row t < n_tokens its position in its request and its slot
+ * (page * page_size + offset; -1 for rows past the last request and tokens
+ * without a page).  Pages that requests need beyond those they hold are
+ * taken from free_pages[cursor ...] in request order and entered into
+ * block_table; cursor_out is the cursor after them.  Nothing that it reads is
+ * changed, so a call can be repeated.  When the list or the table's width
+ * runs out, the tokens concerned get slot -1 (table entries -1) and status 7
+ * is recorded; so it is for negative lengths (taken as 0) and for more new
+ * tokens than n_tokens.  `status` may be NULL. */
+int exl3_kv_plan(const int32_t* lens, const int32_t* new_tokens, int requests, int32_t* block_table, int width,
+                 const int32_t* free_pages, int n_free, const int32_t* cursor, int page, int n_tokens,
+                 int32_t* kv_lens, int32_t* cu_tokens, int32_t* positions, int64_t* slots, int32_t* cursor_out,
+                 int* status, void* stream);
+
+/* Writes new rows of K and V (fp16 or bf16 [tokens][kv_heads][dim], strides in
+ * elements, rows at multiples of 8 bytes) to their slots as codes.  A page's
+ * tokens of one call follow one another in ascending order, as exl3_kv_plan
+ * gives them.  A call that writes a page's first token sets its scale from
+ * the new tokens alone; one that joins a part-filled page keeps the larger of
+ * its scale and the new tokens', rounding the older codes again when it
+ * grows.  NaN stays NaN in e4m3 and becomes 0 in int8, infinities become the
+ * largest code.  Negative slots are skipped; slots past the cache are skipped
+ * with status 7. */
+int exl3_kv_append(const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v, int64_t v_tok_stride,
+                   int64_t v_head_stride, int x_dtype, const int64_t* slots, int64_t tokens, void* k_cache,
+                   void* v_cache, float* k_scale, float* v_scale, int code, int64_t pages, int kv_heads, int page,
+                   int dim, int* status, void* stream);
+
+/* out[r][h] = softmax_j(scale * q[r][h] . k_j) v_j over the cache.  Request
+ * b's rows of q and out are [cu_tokens[b], cu_tokens[b + 1]) (cu_tokens NULL:
+ * row b alone); they are its last tokens, at positions kv_lens[b] - n + i, and
+ * row i sees the keys j <= its position, j > its position - window (window 0:
+ * no lower limit).  Query head h reads kv head h / (heads / kv_heads).
+ * max_new bounds the rows of a request (it selects kernels, it is no mask).
+ * q fp16 or bf16 [q_rows][heads][dim], strides in elements, rows at multiples
+ * of 16 bytes; out [q_rows][heads][dim] in q's type; lse (NULL, or fp32
+ * [q_rows][heads]) the log of the softmax's denominator.  A row that sees no
+ * key, and rows past the last request, are zeros with lse -inf.  Keys whose
+ * page is not in the cache are not seen, with status 7.  Results do not
+ * depend on timing: repeats are equal bit for bit. */
+/* Workspace of this entry and of exl3_token_logprobs: 256-byte aligned, all
+ * zero before its first use; it starts with the status word, and may serve
+ * both, for calls that follow one another on a stream. */
+size_t exl3_kv_attend_workspace_size(int heads, int kv_heads, int dim, int max_new, int requests, int64_t q_rows);
+int exl3_kv_attend(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int x_dtype, int64_t q_rows, int heads,
+                   const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, int code,
+                   int64_t pages, int kv_heads, int page, int dim, const int32_t* block_table, int width, int requests,
+                   const int32_t* kv_lens, const int32_t* cu_tokens, int max_new, float scale, int64_t window,
+                   void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* For each row of logits (fp32, fp16 or bf16 [rows][vocab], row stride in
+ * elements): logprob = log softmax at tokens[row] (int32 or int64), the
+ * distribution's entropy (nats), rank = 1 + the entries before the token in
+ * descending order, and the `top` (0..EXL3_LOGPROBS_MAX_TOP) first entries of
+ * that order as top_logprobs fp32 and top_ids int32 [rows][top]; equal logits
+ * go lowest index first, NaN with -inf.  A token outside [0, vocab): logprob
+ * -inf, rank 0.  A row of -inf alone: every log probability -inf, entropy 0.
+ * A row with NaN or +inf: NaN, as a softmax gives. */
+#define EXL3_LOGPROBS_MAX_TOP 32
+size_t exl3_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top, int x_dtype);
+int exl3_token_logprobs(const void* logits, int x_dtype, int64_t rows, int64_t row_stride, int64_t vocab,
+                        const void* tokens, int ids_dtype, int top, float* logprob, float* entropy, int32_t* rank,
+                        float* top_logprobs, int32_t* top_ids, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Phase timing for benchmarks (no reference counterpart; the reference times
  * its kernels with CUDA events in tools/bench_moe_decode.py:24-55).  While
  * enabled, exl3_moe_forward and exl3_linear first launch a spin of

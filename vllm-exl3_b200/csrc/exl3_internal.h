@@ -194,6 +194,89 @@ cudaError_t run_ngram(const uint16_t* rows, int64_t n, int64_t n_rows, int bits,
                       const int32_t* heads, const int64_t* head_offsets, int num_heads, const void* head_bias,
                       void* out, int out_dtype, int* status, cudaStream_t s);
 
+// --- the paged 8-bit key/value cache (kv_cache.cu, kv_attend.cu) ---
+// pages hold 1 << page_shift(page) tokens; page is 16, 32, 64 or 128
+inline int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
+
+struct KvPlanCall {
+    const int32_t *lens = nullptr, *fresh = nullptr;  // [requests] cached and new tokens
+    int requests = 0;
+    int32_t* table = nullptr;  // [requests][width]
+    int width = 0;
+    const int32_t* free_pages = nullptr;
+    int n_free = 0;
+    const int32_t* cursor = nullptr;
+    int page = 16, n_tokens = 0;
+    int32_t *kv_lens = nullptr, *cu = nullptr, *positions = nullptr;
+    int64_t* slots = nullptr;
+    int32_t* cursor_out = nullptr;
+    int* status = nullptr;
+};
+cudaError_t run_kv_plan(const KvPlanCall& c, cudaStream_t s);
+
+struct KvAppendCall {
+    const void* x[2] = {nullptr, nullptr};  // K, V [tokens][heads][dim], strides in elements
+    int64_t tok_stride[2] = {0, 0}, head_stride[2] = {0, 0};
+    int x_dtype = 1;
+    const int64_t* slots = nullptr;
+    int64_t tokens = 0;
+    void* cache[2] = {nullptr, nullptr};
+    float* scale[2] = {nullptr, nullptr};
+    int64_t pages = 0;
+    int heads = 0, page = 16, dim = 128;
+    bool e4m3 = true;
+    int* status = nullptr;
+};
+cudaError_t run_kv_append(const KvAppendCall& c, cudaStream_t s);
+
+struct KvAttendCall {
+    const void* q = nullptr;  // [q_rows][heads][dim], strides in elements
+    int64_t q_tok = 0, q_head = 0;
+    int x_dtype = 1;  // of q and out
+    int64_t q_rows = 0;
+    int heads = 0, kv_heads = 0, dim = 128;
+    const void *k = nullptr, *v = nullptr;  // codes [pages][kv_heads][page][dim]
+    const float *k_scale = nullptr, *v_scale = nullptr;
+    int64_t pages = 0;
+    int page = 16;
+    bool e4m3 = true;
+    const int32_t* table = nullptr;  // [requests][width]
+    int width = 0, requests = 0;
+    const int32_t* kv_lens = nullptr;
+    const int32_t* cu = nullptr;  // [requests + 1]; nullptr: one query row per request
+    int max_new = 1;
+    float scale = 1.f;
+    int window = 0;  // 0: none
+    void* out = nullptr;   // [q_rows][heads][dim]
+    float* lse = nullptr;  // [q_rows][heads]
+    int32_t* counters = nullptr;  // zero before and after every call
+    char* ws = nullptr;           // partial sums
+    int* status = nullptr;
+};
+size_t kv_attend_workspace(const KvAttendCall& c, int sms);
+int kv_attend_counters(int sms);
+cudaError_t run_kv_attend(const KvAttendCall& c, int sms, cudaStream_t s);
+
+// --- token log probabilities (logprobs.cu) ---
+struct LogprobsCall {
+    const void* logits = nullptr;  // [rows][vocab], row stride in elements
+    int x_dtype = 0;
+    int64_t rows = 0, stride = 0;
+    int vocab = 0;
+    const void* tokens = nullptr;
+    int ids_dtype = 4;
+    int top = 0;
+    float *logprob = nullptr, *entropy = nullptr;
+    int32_t* rank = nullptr;
+    float* top_logprobs = nullptr;
+    int32_t* top_ids = nullptr;
+    int32_t* counters = nullptr;  // zero before and after every call
+    char* ws = nullptr;           // per-split partial results
+};
+size_t logprobs_workspace(const LogprobsCall& c, int sms);
+int logprobs_counters(int sms);
+cudaError_t run_logprobs(const LogprobsCall& c, int sms, cudaStream_t s);
+
 int num_sms_current();
 // stages and dynamic smem of the GEMM for mt 128-row halves per tile; false
 // if two stages do not fit at two CTAs per SM

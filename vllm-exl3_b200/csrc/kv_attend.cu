@@ -1,0 +1,534 @@
+// kv_attend.cu -- attention over the paged 8-bit cache, few query rows per request.
+//
+//   out[r] = sum_j softmax_j(scale * q_r . k_j) v_j over the keys j that row r
+//   may see: j <= pos_r, j < len, and j > pos_r - window where there is a window.
+//
+// The scales of a (page, head) tile are constant over it, so with e = log2 of
+// the V scale the tile's weights are p_j = 2^(s_j + e - m), m the running
+// maximum of s_j + e, and
+//   out = sum_j p_j code_j / sum_j p_j 2^-e :
+// codes feed the tensor core as they are and no value is multiplied by a scale.
+//
+// Work: an item is (request, kv head, group of NC = 8 NT query columns), a
+// column being one (token, query head) that reads this kv head.  Its keys are
+// cut into units of 128 (8 warps x 16 keys); all items' units form one line
+// that the CTAs split evenly, so lengths need no balancing and the host needs
+// none of them.  An item cut by a CTA boundary is joined from fp32 partials by
+// the CTA that finishes it last, in key order (results do not depend on timing).
+//
+// Bound: every code is read once, 2 D bytes per (key, kv head): HBM.  A warp
+// holds the next 16 keys' codes in registers while it works on the present
+// ones (32 lanes x 128 bytes), which with 16 warps keeps 64 KB in flight per
+// SM and needs no shared memory or barrier inside the loop.  The products run
+// as S^T = K Q^T and O^T = V^T P^T on m16n8k16: the keys (then the dims) are
+// the 16 rows, so 8 query columns fill an MMA, and both operands come straight
+// from the loaded words.  A dim may sit at any place of the contraction, so
+// each lane's 16-byte loads already are its A fragment of K; for V, words of
+// two keys are interleaved with one byte permute.
+#include <cuda_fp16.h>
+#include <cuda_bf16.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "kv_common.cuh"
+
+namespace exl3 {
+
+constexpr int kAttWarps = 8, kAttThreads = kAttWarps * 32, kAttUnit = 16 * kAttWarps;
+constexpr int kAttCtasPerSm = 2;
+
+struct KvAttendArgs {
+    const uint16_t* q;
+    int64_t q_tok, q_head, q_rows;
+    int heads, kv_heads, group;  // group = heads / kv_heads
+    const uint8_t *k, *v;
+    const float *k_scale, *v_scale;
+    int64_t pages;
+    int shift;
+    const int32_t* table;
+    int width, requests;
+    const int32_t *kv_lens, *cu;
+    float scale_log2;  // softmax scale * log2(e)
+    int window;
+    uint16_t* out;
+    float* lse;
+    int32_t* counters;
+    float* part;
+    int* status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// two codes (bytes 0, 1 of w; int8 already offset by 128) as f16x2, exact
+template <bool E4M3>
+__device__ __forceinline__ uint32_t half2_lo(uint32_t w) {
+    if constexpr (E4M3) {
+        return e4m3x2_to_half2(w);
+    } else {
+        uint32_t h = __byte_perm(w, 0x64646464u, 0x4140);  // 1024 + u
+        const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&h), __float2half2_rn(1152.f));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+template <bool E4M3>
+__device__ __forceinline__ uint32_t half2_hi(uint32_t w) {
+    if constexpr (E4M3) {
+        return e4m3x2_to_half2(w >> 16);
+    } else {
+        uint32_t h = __byte_perm(w, 0x64646464u, 0x4342);
+        const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&h), __float2half2_rn(1152.f));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+template <bool E4M3>
+__device__ __forceinline__ uint32_t code_word(uint32_t w) {
+    return E4M3 ? w : w ^ 0x80808080u;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// what a request asks for
+struct AttReq {
+    int len, fresh, lo16, groups, units;  // keys, new rows, first key's tile, column groups, units per item
+    int64_t row0;
+};
+
+template <int NC>
+__device__ __forceinline__ AttReq att_request(const KvAttendArgs& a, int b) {
+    AttReq r;
+    r.row0 = a.cu ? a.cu[b] : b;
+    r.fresh = a.cu ? max(a.cu[b + 1] - int(r.row0), 0) : 1;
+    r.len = int(min(int64_t(max(a.kv_lens[b], 0)), int64_t(a.width) << a.shift));
+    const int first = r.len - r.fresh;  // position of the first new row
+    const int lo = a.window > 0 ? max(first + 1 - a.window, 0) : 0;
+    r.lo16 = min(lo, r.len) & ~15;
+    r.groups = (r.fresh * a.group + NC - 1) / NC;
+    r.units = max((r.len - r.lo16 + kAttUnit - 1) / kAttUnit, 1);
+    return r;
+}
+
+template <bool E4M3, bool BF16, int D, int NT>
+__global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) kv_attend_kernel(const KvAttendArgs a) {
+    constexpr int NC = 8 * NT;
+    constexpr int KS = D / 16;  // contraction steps of S, row tiles of O
+    constexpr int PART = NC * (D + 2);
+    extern __shared__ float att_smem[];
+    float* red = att_smem;                            // [warps][NC][D]
+    float* wm = red + kAttWarps * NC * D;             // [warps][NC] maxima, then factors
+    float* wl = wm + kAttWarps * NC;                  // [warps][NC] sums
+    float* fin = wl + kAttWarps * NC;                 // [2][NC] joined maximum, sum
+    __shared__ int64_t scan[kAttWarps];
+    __shared__ int64_t found_base;
+    __shared__ int found_b, last_flag;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+    const int Hk = a.kv_heads, G = a.group, P = 1 << a.shift;
+
+    // --- this CTA's share of the line of units ---
+    const int per = (a.requests + kAttThreads - 1) / kAttThreads;
+    int64_t mine = 0;
+    for (int i = 0; i < per; ++i) {
+        const int b = tid * per + i;
+        if (b < a.requests) {
+            const AttReq r = att_request<NC>(a, b);
+            mine += int64_t(r.groups) * Hk * r.units;
+        }
+    }
+    int64_t incl = mine;
+    #pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += o;
+    }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    int64_t total = 0;
+    #pragma unroll
+    for (int w = 0; w < kAttWarps; ++w) {
+        if (w == warp) incl += total;
+        total += scan[w];
+    }
+    // rows no request owns are zeros
+    if (a.cu) {
+        const int64_t live = a.cu[a.requests], n = (a.q_rows - live) * a.heads;
+        for (int64_t i = int64_t(blockIdx.x) * kAttWarps + warp; i < n; i += int64_t(gridDim.x) * kAttWarps) {
+            const int64_t row = live * a.heads + i;
+            for (int d = lane; d < D; d += 32) a.out[row * D + d] = 0;
+            if (a.lse && lane == 0) a.lse[row] = -INFINITY;
+        }
+    }
+    const int ctas = int(min(int64_t(gridDim.x), total));
+    const int cta = blockIdx.x;
+    if (cta >= ctas) return;
+    int64_t u = total * cta / ctas;
+    const int64_t u_end = total * (cta + 1) / ctas;
+    if (u >= incl - mine && u < incl) {
+        int64_t base = incl - mine;
+        int b = tid * per;
+        for (;;) {
+            const AttReq r = att_request<NC>(a, b);
+            const int64_t n = int64_t(r.groups) * Hk * r.units;
+            if (u < base + n) break;
+            base += n, ++b;
+        }
+        found_b = b, found_base = base;
+    }
+    __syncthreads();
+    int b = found_b;
+    int64_t base = found_base;
+    AttReq rq = att_request<NC>(a, b);
+
+    while (u < u_end) {
+        while (u >= base + int64_t(rq.groups) * Hk * rq.units) {  // next request with work
+            base += int64_t(rq.groups) * Hk * rq.units;
+            rq = att_request<NC>(a, ++b);
+        }
+        const int64_t item = (u - base) / rq.units;
+        const int off = int((u - base) - item * rq.units);
+        const int n_units = int(min(int64_t(rq.units - off), u_end - u));
+        const int hk = int(item % Hk), cg = int(item / Hk);
+        const int ncols = min(rq.fresh * G - cg * NC, NC);
+        const int64_t u_item = u - off;
+        u += n_units;
+
+        // --- the query columns: B fragments of Q^T, and each column's key range ---
+        uint32_t qf[NT][KS][2];
+        float cfac[NT][2];           // columns 2c, 2c + 1: softmax scale (and Q's power of two)
+        int hi[NT][2], lo[NT][2];    // keys [lo, hi)
+        #pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int n = 8 * t + g, f = cg * NC + n;
+            const int64_t row = rq.row0 + f / G;
+            const bool live = n < ncols && row < a.q_rows;
+            const uint16_t* qp = a.q + (live ? row * a.q_tok + int64_t(hk * G + f % G) * a.q_head : 0);
+            float fac = a.scale_log2;
+            float amax = 0.f;
+            #pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int dim = D == 128 ? (s >> 2) * 64 + c * 16 + (s & 3) * 4 : c * 16 + s * 4;
+                const uint2 w = live ? *reinterpret_cast<const uint2*>(qp + dim) : make_uint2(0u, 0u);
+                qf[t][s][0] = w.x, qf[t][s][1] = w.y;
+                if constexpr (BF16) {
+                    const uint32_t m = __vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
+                    amax = fmaxf(amax, fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u)));
+                }
+            }
+            if constexpr (BF16) {
+                // the tensor core takes Q in f16 like the codes: a power of two per row puts its
+                // largest magnitude in [2^14, 2^15), where f16 keeps all 8 bits of a bf16 value
+                // down to 2^-31 of that largest one
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const int e = min(max((__float_as_int(amax) >> 23) - 127, -100), 100);
+                const float mul = exp2_int(14 - e);
+                fac *= exp2_int(e - 14);
+                #pragma unroll
+                for (int s = 0; s < KS; ++s)
+                    #pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t w = qf[t][s][i];
+                        qf[t][s][i] = pack_half2(__uint_as_float(w << 16) * mul, __uint_as_float(w & 0xffff0000u) * mul);
+                    }
+            }
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int col = 2 * c + i, fc = cg * NC + 8 * t + col;
+                cfac[t][i] = __shfl_sync(0xffffffffu, fac, 4 * col);
+                const int pos = rq.len - rq.fresh + fc / G;
+                hi[t][i] = 8 * t + col < ncols ? min(pos + 1, rq.len) : 0;
+                lo[t][i] = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
+            }
+        }
+        int full_lo = 0, full_hi = 0x7fffffff;  // keys in [full_lo, full_hi) need no test
+        #pragma unroll
+        for (int t = 0; t < NT; ++t)
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const bool live = 8 * t + 2 * c + i < ncols;
+                full_lo = max(full_lo, live ? lo[t][i] : 0);
+                full_hi = min(full_hi, live ? hi[t][i] : 0x7fffffff);
+            }
+        full_lo = __reduce_max_sync(0xffffffffu, full_lo);
+        full_hi = __reduce_min_sync(0xffffffffu, full_hi);
+
+        float o[NT][KS][4], m[NT][2], l[NT][2];
+        #pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            #pragma unroll
+            for (int j = 0; j < KS; ++j)
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) o[t][j][i] = 0.f;
+            m[t][0] = m[t][1] = -INFINITY;
+            l[t][0] = l[t][1] = 0.f;
+        }
+
+        const int first = rq.lo16 + off * kAttUnit + warp * 16;
+        const int end = min(rq.len, rq.lo16 + (off + n_units) * kAttUnit);
+        const int32_t* row_table = a.table + int64_t(b) * a.width;
+        auto page_at = [&](int tok) { return tok < end ? row_table[tok >> a.shift] : 0; };
+
+        // codes of 16 keys: K rows g and g + 8, V rows 2c, 2c + 1, 2c + 8, 2c + 9
+        uint4 kr[2][D / 64];
+        uint32_t vr[4][D / 32];
+        float ks = 0.f, vs = 0.f;
+        bool got = false;  // the tile's page exists
+        auto load_k = [&](int tok, int page) {
+            got = tok < end && page >= 0 && page < a.pages;
+            if (tok < end && !got && lane == 0) set_status(a.status, DEV_BAD_INDEX);
+            const int64_t tile = int64_t(got ? page : 0) * Hk + hk;
+            ks = got ? a.k_scale[tile] : 0.f;
+            vs = got ? a.v_scale[tile] : 1.f;
+            const uint8_t* p = a.k + ((tile << a.shift) + (tok & (P - 1)) + g) * D + c * 16;
+            #pragma unroll
+            for (int i = 0; i < 2; ++i)
+                #pragma unroll
+                for (int h = 0; h < D / 64; ++h)
+                    kr[i][h] = got ? __ldg(reinterpret_cast<const uint4*>(p + i * 8 * D + h * 64)) : make_uint4(0, 0, 0, 0);
+        };
+        auto load_v = [&](int tok, int page, bool ok) {
+            const int64_t tile = int64_t(ok ? page : 0) * Hk + hk;
+            const uint8_t* p = a.v + ((tile << a.shift) + (tok & (P - 1)) + 2 * c) * D + g * (D / 8);
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint8_t* r = p + ((i & 1) + (i >> 1) * 8) * D;
+                if constexpr (D == 128) {
+                    const uint4 w = ok ? __ldg(reinterpret_cast<const uint4*>(r)) : make_uint4(0, 0, 0, 0);
+                    vr[i][0] = w.x, vr[i][1] = w.y, vr[i][2] = w.z, vr[i][3] = w.w;
+                } else {
+                    const uint2 w = ok ? __ldg(reinterpret_cast<const uint2*>(r)) : make_uint2(0, 0);
+                    vr[i][0] = w.x, vr[i][1] = w.y;
+                }
+            }
+        };
+        int page = page_at(first), page_next = page_at(first + kAttUnit);
+        load_k(first, page);
+        load_v(first, page, got);
+
+        for (int tok = first; tok < end; tok += kAttUnit) {
+            // --- S^T = K Q^T ---
+            float s[NT][4];
+            #pragma unroll
+            for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+            #pragma unroll
+            for (int st = 0; st < KS; ++st) {
+                auto word = [&](const uint4& q4) {
+                    return code_word<E4M3>((st & 3) == 0 ? q4.x : (st & 3) == 1 ? q4.y : (st & 3) == 2 ? q4.z : q4.w);
+                };
+                const uint32_t w0 = word(kr[0][D == 128 ? st >> 2 : 0]), w1 = word(kr[1][D == 128 ? st >> 2 : 0]);
+                const uint32_t af[4] = {half2_lo<E4M3>(w0), half2_lo<E4M3>(w1), half2_hi<E4M3>(w0), half2_hi<E4M3>(w1)};
+                #pragma unroll
+                for (int t = 0; t < NT; ++t) mma_16816(s[t], af, qf[t][st][0], qf[t][st][1]);
+            }
+            const bool have = got;
+            const float kscale = ks;
+            const int ve = stored_exponent(vs);
+            page = page_next;
+            page_next = page_at(tok + 2 * kAttUnit);
+            load_k(tok + kAttUnit, page);
+
+            // --- softmax over these 16 keys ---
+            const bool edge = tok < full_lo || tok + 16 > full_hi || !have;
+            const float vexp = float(ve), vinv = exp2_int(-ve);
+            uint32_t pf[NT][2];
+            #pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) s[t][i] = fmaf(s[t][i], cfac[t][i & 1] * kscale, vexp);
+                if (edge) {
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = tok + g + 8 * (i >> 1);
+                        if (!have || key >= hi[t][i & 1] || key < lo[t][i & 1]) s[t][i] = -INFINITY;
+                    }
+                }
+                float p[4];
+                #pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float mx = fmaxf(s[t][i], s[t][i + 2]);
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float mn = fmaxf(m[t][i], mx), ref = mn == -INFINITY ? 0.f : mn;
+                    const float alpha = ex2(m[t][i] - ref);  // 0 while nothing has been seen
+                    m[t][i] = mn;
+                    p[i] = ex2(s[t][i] - ref), p[i + 2] = ex2(s[t][i + 2] - ref);
+                    l[t][i] = fmaf(l[t][i], alpha, (p[i] + p[i + 2]) * vinv);
+                    if (__any_sync(0xffffffffu, alpha != 1.f)) {
+                        #pragma unroll
+                        for (int j = 0; j < KS; ++j) o[t][j][i] *= alpha, o[t][j][i + 2] *= alpha;
+                    }
+                }
+                pf[t][0] = transpose8x8(pack_half2(p[0], p[1]));
+                pf[t][1] = transpose8x8(pack_half2(p[2], p[3]));
+            }
+            if (E4M3 && tok + 16 > rq.len) {  // codes past the end may be NaN, and 0 * NaN is not 0
+                #pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (tok + 2 * c + (i & 1) + (i >> 1) * 8 >= rq.len)
+                        #pragma unroll
+                        for (int w = 0; w < D / 32; ++w) vr[i][w] = 0u;
+            }
+
+            // --- O^T += V^T P^T ---
+            #pragma unroll
+            for (int w = 0; w < D / 32; ++w) {
+                const uint32_t v0 = code_word<E4M3>(vr[0][w]), v1 = code_word<E4M3>(vr[1][w]);
+                const uint32_t v2 = code_word<E4M3>(vr[2][w]), v3 = code_word<E4M3>(vr[3][w]);
+                #pragma unroll
+                for (int h = 0; h < 2; ++h) {  // dims 4w + 2h, 4w + 2h + 1 of the lane's D / 8
+                    const uint32_t x = __byte_perm(v0, v1, h ? 0x7362 : 0x5140);
+                    const uint32_t y = __byte_perm(v2, v3, h ? 0x7362 : 0x5140);
+                    const uint32_t af[4] = {half2_lo<E4M3>(x), half2_hi<E4M3>(x), half2_lo<E4M3>(y), half2_hi<E4M3>(y)};
+                    #pragma unroll
+                    for (int t = 0; t < NT; ++t) mma_16816(o[t][2 * w + h], af, pf[t][0], pf[t][1]);
+                }
+            }
+            load_v(tok + kAttUnit, page, got);
+        }
+
+        // --- join the warps ---
+        #pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                #pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], d);
+                if (g == 0) wm[warp * NC + 8 * t + 2 * c + i] = m[t][i], wl[warp * NC + 8 * t + 2 * c + i] = l[t][i];
+                #pragma unroll
+                for (int j = 0; j < KS; ++j)
+                    *reinterpret_cast<float2*>(red + (warp * NC + 8 * t + 2 * c + i) * D + g * (D / 8) + 2 * j) =
+                        make_float2(o[t][j][i], o[t][j][i + 2]);
+            }
+        }
+        __syncthreads();
+        if (tid < NC) {
+            float mx = -INFINITY, sum = 0.f;
+            for (int w = 0; w < kAttWarps; ++w) mx = fmaxf(mx, wm[w * NC + tid]);
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            for (int w = 0; w < kAttWarps; ++w) {
+                const float f = ex2(wm[w * NC + tid] - ref);
+                wm[w * NC + tid] = f;
+                sum = fmaf(wl[w * NC + tid], f, sum);
+            }
+            fin[tid] = mx, fin[NC + tid] = sum;
+        }
+        __syncthreads();
+        auto emit = [&](int col, int d, float value, float sum, float mx) {
+            const int f = cg * NC + col;
+            const int64_t row = rq.row0 + f / G;
+            if (col >= ncols || row >= a.q_rows) return;
+            const int64_t at = row * a.heads + hk * G + f % G;
+            const float r = sum == 0.f ? 0.f : value / sum;  // a row that sees no key is zero
+            a.out[at * D + d] = BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(r)) : __half_as_ushort(__float2half_rn(r));
+            if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
+        };
+        const bool whole = n_units == rq.units;
+        // partial slots: 2 cta + 1 for the item that begins in this CTA, 2 cta for the one it carries on
+        float* part = a.part + int64_t(2 * cta + (off == 0 ? 1 : 0)) * PART;
+        for (int i = tid; i < NC * D; i += kAttThreads) {
+            const int col = i / D, d = i % D;
+            float v = 0.f;
+            #pragma unroll
+            for (int w = 0; w < kAttWarps; ++w) v = fmaf(red[(w * NC + col) * D + d], wm[w * NC + col], v);
+            if (whole) emit(col, d, v, fin[NC + col], fin[col]);
+            else __stcg(part + 2 * NC + i, v);
+        }
+        if (!whole) {
+            if (tid < 2 * NC) __stcg(part + tid, fin[tid]);
+            const int64_t T = total;
+            const int c0 = int(((u_item + 1) * ctas - 1) / T), c1 = int(((u_item + rq.units) * ctas - 1) / T);
+            const int pieces = c1 - c0 + 1;
+            __syncthreads();
+            if (tid == 0) {
+                int prev;
+                asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(prev) : "l"(a.counters + c0) : "memory");
+                last_flag = prev == pieces - 1;
+                if (prev == pieces - 1) a.counters[c0] = 0;  // ready for the next call
+            }
+            __syncthreads();
+            if (last_flag) {
+                auto piece = [&](int p) { return a.part + int64_t(2 * (c0 + p) + (p == 0 ? 1 : 0)) * PART; };
+                float* wt = red;  // [pieces][NC] weights
+                if (tid < NC) {
+                    float mx = -INFINITY, sum = 0.f;
+                    for (int p = 0; p < pieces; ++p) mx = fmaxf(mx, __ldcg(piece(p) + tid));
+                    const float ref = mx == -INFINITY ? 0.f : mx;
+                    for (int p = 0; p < pieces; ++p) {
+                        const float f = ex2(__ldcg(piece(p) + tid) - ref);
+                        wt[p * NC + tid] = f;
+                        sum = fmaf(__ldcg(piece(p) + NC + tid), f, sum);
+                    }
+                    fin[tid] = mx, fin[NC + tid] = sum;
+                }
+                __syncthreads();
+                for (int i = tid; i < NC * D; i += kAttThreads) {
+                    const int col = i / D;
+                    float v = 0.f;
+                    #pragma unroll 4
+                    for (int p = 0; p < pieces; ++p) v = fmaf(__ldcg(piece(p) + 2 * NC + i), wt[p * NC + col], v);
+                    emit(col, i % D, v, fin[NC + col], fin[col]);
+                }
+            }
+        }
+        __syncthreads();  // shared memory is the next item's
+    }
+}
+
+int kv_attend_counters(int sms) { return sms * kAttCtasPerSm; }
+
+static int att_tiles(const KvAttendCall& c) { return int64_t(c.max_new) * (c.heads / c.kv_heads) > 8 ? 2 : 1; }
+
+size_t kv_attend_workspace(const KvAttendCall& c, int sms) {
+    return size_t(sms) * kAttCtasPerSm * 2 * (8 * att_tiles(c)) * (c.dim + 2) * 4;
+}
+
+template <bool E4M3, bool BF16, int D, int NT>
+static cudaError_t launch_attend(const KvAttendArgs& a, int sms, cudaStream_t s) {
+    constexpr int NC = 8 * NT;
+    const size_t smem = size_t(kAttWarps * NC * (D + 2) + 2 * NC) * 4;
+    auto* kernel = kv_attend_kernel<E4M3, BF16, D, NT>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (e != cudaSuccess) return e;
+    kernel<<<sms * kAttCtasPerSm, kAttThreads, smem, s>>>(a);
+    return cudaGetLastError();
+}
+
+cudaError_t run_kv_attend(const KvAttendCall& c, int sms, cudaStream_t s) {
+    if (c.q_rows <= 0) return cudaSuccess;
+    KvAttendArgs a;
+    a.q = static_cast<const uint16_t*>(c.q), a.q_tok = c.q_tok, a.q_head = c.q_head, a.q_rows = c.q_rows;
+    a.heads = c.heads, a.kv_heads = c.kv_heads, a.group = c.heads / c.kv_heads;
+    a.k = static_cast<const uint8_t*>(c.k), a.v = static_cast<const uint8_t*>(c.v);
+    a.k_scale = c.k_scale, a.v_scale = c.v_scale, a.pages = c.pages, a.shift = page_shift(c.page);
+    a.table = c.table, a.width = c.width, a.requests = c.requests, a.kv_lens = c.kv_lens, a.cu = c.cu;
+    a.scale_log2 = c.scale * 1.4426950408889634f, a.window = c.window;
+    a.out = static_cast<uint16_t*>(c.out), a.lse = c.lse, a.counters = c.counters;
+    a.part = reinterpret_cast<float*>(c.ws), a.status = c.status;
+    const bool bf16 = c.x_dtype == DT_BF16, wide = att_tiles(c) == 2, d128 = c.dim == 128;
+    const auto pick = [&](auto e4, auto bf, auto dim) {
+        constexpr bool E = decltype(e4)::value, B = decltype(bf)::value;
+        constexpr int Dm = decltype(dim)::value;
+        return wide ? launch_attend<E, B, Dm, 2>(a, sms, s) : launch_attend<E, B, Dm, 1>(a, sms, s);
+    };
+    const auto by_dim = [&](auto e4, auto bf) {
+        return d128 ? pick(e4, bf, std::integral_constant<int, 128>()) : pick(e4, bf, std::integral_constant<int, 64>());
+    };
+    if (c.e4m3) return bf16 ? by_dim(std::true_type(), std::true_type()) : by_dim(std::true_type(), std::false_type());
+    return bf16 ? by_dim(std::false_type(), std::true_type()) : by_dim(std::false_type(), std::false_type());
+}
+
+}  // namespace exl3

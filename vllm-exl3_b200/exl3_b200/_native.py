@@ -7,6 +7,7 @@ torch's current stream of the tensors' device.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -73,6 +74,13 @@ SIGNATURES = {
                                   ctypes.POINTER(SZ)]),
     "exl3_ngram_dequant": (I32, [P, I64, I32, P, P, I32, P, I32, P]),
     "exl3_ngram_lookup": (I32, [P, I64, I32, P, I32, I64, P, I32, P, P, I32, P, P]),
+    "exl3_kv_plan": (I32, [P, P, I32, P, I32, P, I32, P, I32, I32, P, P, P, P, P, P, P]),
+    "exl3_kv_append": (I32, [P, I64, I64, P, I64, I64, I32, P, I64, P, P, P, P, I32, I64, I32, I32, I32, P, P]),
+    "exl3_kv_attend_workspace_size": (SZ, [I32, I32, I32, I32, I32, I64]),
+    "exl3_kv_attend": (I32, [P, I64, I64, I32, I64, I32, P, P, P, P, I32, I64, I32, I32, I32, P, I32, I32, P, P, I32,
+                             F32, I64, P, P, P, SZ, P]),
+    "exl3_token_logprobs_workspace_size": (SZ, [I64, I64, I32, I32]),
+    "exl3_token_logprobs": (I32, [P, I32, I64, I64, I64, P, I32, I32, P, P, P, P, P, P, SZ, P]),
     "exl3_profile_enable": (I32, [I32, ctypes.c_longlong]),
     "exl3_profile_read": (I32, [ctypes.POINTER(F32), I32, ctypes.POINTER(I32)]),
 }
@@ -128,6 +136,19 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def raw_stream(device: torch.device) -> int:
+    """torch's current stream of ``device`` as a raw handle."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A guard that makes ``device`` current; free of cost where it is already."""
+    return _NO_SWITCH if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
 def require_cuda(*tensors: torch.Tensor | None, who: str) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
@@ -179,6 +200,23 @@ def workspace(device: torch.device, nbytes: int, stream: torch.cuda.Stream | Non
         with torch.cuda.stream(stream):
             buf = torch.empty(size, dtype=torch.uint8, device=device)
             buf[:256].zero_()  # the device status word starts clean
+        _ws_cache[key] = buf
+    return buf
+
+
+def zeroed_workspace(device: torch.device, nbytes: int, stream: int) -> torch.Tensor:
+    """The workspace of the cache and log-probability entries for the raw
+    ``stream`` of ``device``: kept apart from :func:`workspace` because those
+    entries need its counters zero and leave them zero.  Grows and is retained
+    in the same way."""
+    key = (device.type, device.index, stream, "zeroed")
+    buf = _ws_cache.get(key)
+    if buf is None or buf.numel() < nbytes:
+        size = max(int(nbytes), 1 << 20)
+        if buf is not None:
+            size = max(size, 2 * buf.numel())
+            _ws_retired.append(buf)
+        buf = torch.zeros(size, dtype=torch.uint8, device=device)
         _ws_cache[key] = buf
     return buf
 
