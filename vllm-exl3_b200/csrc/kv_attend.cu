@@ -31,75 +31,16 @@
 
 #include <type_traits>
 
-#include "kv_common.cuh"
+#include "kv_attend.cuh"
 
 namespace exl3 {
 
 constexpr int kAttWarps = 8, kAttThreads = kAttWarps * 32, kAttUnit = 16 * kAttWarps;
 constexpr int kAttCtasPerSm = 2;
 
-struct KvAttendArgs {
-    const uint16_t* q;
-    int64_t q_tok, q_head, q_rows;
-    int heads, kv_heads, group;  // group = heads / kv_heads
-    const uint8_t *k, *v;
-    const float *k_scale, *v_scale;
-    int64_t pages;
-    int shift;
-    const int32_t* table;
-    int width, requests;
-    const int32_t *kv_lens, *cu;
-    float scale_log2;  // softmax scale * log2(e)
-    int window;
-    uint16_t* out;
-    float* lse;
-    int32_t* counters;
-    float* part;
-    int* status;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// two codes (bytes 0, 1 of w; int8 already offset by 128) as f16x2, exact
-template <bool E4M3>
-__device__ __forceinline__ uint32_t half2_lo(uint32_t w) {
-    if constexpr (E4M3) {
-        return e4m3x2_to_half2(w);
-    } else {
-        uint32_t h = __byte_perm(w, 0x64646464u, 0x4140);  // 1024 + u
-        const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&h), __float2half2_rn(1152.f));
-        return *reinterpret_cast<const uint32_t*>(&r);
-    }
-}
-template <bool E4M3>
-__device__ __forceinline__ uint32_t half2_hi(uint32_t w) {
-    if constexpr (E4M3) {
-        return e4m3x2_to_half2(w >> 16);
-    } else {
-        uint32_t h = __byte_perm(w, 0x64646464u, 0x4342);
-        const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&h), __float2half2_rn(1152.f));
-        return *reinterpret_cast<const uint32_t*>(&r);
-    }
-}
-template <bool E4M3>
-__device__ __forceinline__ uint32_t code_word(uint32_t w) {
-    return E4M3 ? w : w ^ 0x80808080u;
-}
-
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
-    uint32_t r;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-    return r;
-}
+// Requests of more query columns (rows x heads per kv head) than this go to
+// the prompt kernel when the call has such requests at all.
+constexpr int kAttFew = 16;
 
 // what a request asks for
 struct AttReq {
@@ -116,7 +57,7 @@ __device__ __forceinline__ AttReq att_request(const KvAttendArgs& a, int b) {
     const int first = r.len - r.fresh;  // position of the first new row
     const int lo = a.window > 0 ? max(first + 1 - a.window, 0) : 0;
     r.lo16 = min(lo, r.len) & ~15;
-    r.groups = (r.fresh * a.group + NC - 1) / NC;
+    r.groups = int64_t(r.fresh) * a.group > a.few ? 0 : (r.fresh * a.group + NC - 1) / NC;
     r.units = max((r.len - r.lo16 + kAttUnit - 1) / kAttUnit, 1);
     return r;
 }
@@ -488,12 +429,17 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) kv_attend_kernel(c
     }
 }
 
-int kv_attend_counters(int sms) { return sms * kAttCtasPerSm; }
+// counters: one per CTA of the kernel here, one per item of a split prompt (fewer than SMs)
+int kv_attend_counters(int sms) { return sms * (kAttCtasPerSm + 1); }
 
-static int att_tiles(const KvAttendCall& c) { return int64_t(c.max_new) * (c.heads / c.kv_heads) > 8 ? 2 : 1; }
+static int64_t att_columns(const KvAttendCall& c) { return int64_t(c.max_new) * (c.heads / c.kv_heads); }
+static int att_tiles(const KvAttendCall& c) { return att_columns(c) > 8 ? 2 : 1; }
+static size_t att_bytes(const KvAttendCall& c, int sms) {
+    return size_t(sms) * kAttCtasPerSm * 2 * (8 * att_tiles(c)) * (c.dim + 2) * 4;
+}
 
 size_t kv_attend_workspace(const KvAttendCall& c, int sms) {
-    return size_t(sms) * kAttCtasPerSm * 2 * (8 * att_tiles(c)) * (c.dim + 2) * 4;
+    return att_bytes(c, sms) + (att_columns(c) > kAttFew ? kv_prompt_plan(c, sms).bytes : 0);
 }
 
 template <bool E4M3, bool BF16, int D, int NT>
@@ -518,6 +464,15 @@ cudaError_t run_kv_attend(const KvAttendCall& c, int sms, cudaStream_t s) {
     a.scale_log2 = c.scale * 1.4426950408889634f, a.window = c.window;
     a.out = static_cast<uint16_t*>(c.out), a.lse = c.lse, a.counters = c.counters;
     a.part = reinterpret_cast<float*>(c.ws), a.status = c.status;
+    a.few = INT32_MAX;
+    if (att_columns(c) > kAttFew) {
+        a.few = kAttFew;
+        KvAttendArgs p = a;
+        p.counters = c.counters + sms * kAttCtasPerSm;
+        p.part = reinterpret_cast<float*>(c.ws + att_bytes(c, sms));
+        const cudaError_t e = run_kv_prompt(c, p, kv_prompt_plan(c, sms), s);
+        if (e != cudaSuccess) return e;
+    }
     const bool bf16 = c.x_dtype == DT_BF16, wide = att_tiles(c) == 2, d128 = c.dim == 128;
     const auto pick = [&](auto e4, auto bf, auto dim) {
         constexpr bool E = decltype(e4)::value, B = decltype(bf)::value;

@@ -1,0 +1,82 @@
+// kv_attend.cuh -- what the two attention kernels over the paged 8-bit cache
+// share: their arguments and the conversion of codes to tensor-core operands.
+#pragma once
+
+#include "kv_common.cuh"
+
+namespace exl3 {
+
+struct KvAttendArgs {
+    const uint16_t* q;
+    int64_t q_tok, q_head, q_rows;
+    int heads, kv_heads, group;  // group = heads / kv_heads
+    const uint8_t *k, *v;
+    const float *k_scale, *v_scale;
+    int64_t pages;
+    int shift;
+    const int32_t* table;
+    int width, requests;
+    const int32_t *kv_lens, *cu;
+    float scale_log2;  // softmax scale * log2(e)
+    int window;
+    int few;  // requests of more query columns (rows x group) than this are the prompt kernel's
+    uint16_t* out;
+    float* lse;
+    int32_t* counters;
+    float* part;
+    int* status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// two codes (bytes 0, 1 of w; int8 already offset by 128) as f16x2, exact
+template <bool E4M3>
+__device__ __forceinline__ uint32_t half2_lo(uint32_t w) {
+    if constexpr (E4M3) {
+        return e4m3x2_to_half2(w);
+    } else {
+        uint32_t h = __byte_perm(w, 0x64646464u, 0x4140);  // 1024 + u
+        const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&h), __float2half2_rn(1152.f));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+template <bool E4M3>
+__device__ __forceinline__ uint32_t half2_hi(uint32_t w) {
+    if constexpr (E4M3) {
+        return e4m3x2_to_half2(w >> 16);
+    } else {
+        uint32_t h = __byte_perm(w, 0x64646464u, 0x4342);
+        const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&h), __float2half2_rn(1152.f));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+template <bool E4M3>
+__device__ __forceinline__ uint32_t code_word(uint32_t w) {
+    return E4M3 ? w : w ^ 0x80808080u;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// kv_prompt.cu: requests with more than `few` query columns
+struct KvPromptPlan {
+    int64_t tiles;  // at most: 256-column tiles of all requests
+    int splits;     // at most: parts of a tile's keys
+    size_t bytes;   // workspace for partial results
+};
+KvPromptPlan kv_prompt_plan(const KvAttendCall& c, int sms);
+cudaError_t run_kv_prompt(const KvAttendCall& c, const KvAttendArgs& a, const KvPromptPlan& p, cudaStream_t s);
+
+}  // namespace exl3

@@ -18,8 +18,8 @@ CSRC = os.path.join(ROOT, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libexl3_b200.so")
 
 SOURCES = ["capi.cu", "moe.cu", "reconstruct.cu", "noalloc.cu", "tc_gemm.cu", "ep.cu", "ngram.cu",
-           "kv_cache.cu", "kv_attend.cu", "logprobs.cu"]
-HEADERS = ["exl3_common.cuh", "exl3_internal.h", "tc_common.cuh", "tc_gemm.h", "kv_common.cuh"]
+           "kv_cache.cu", "kv_attend.cu", "kv_prompt.cu", "logprobs.cu"]
+HEADERS = ["exl3_common.cuh", "exl3_internal.h", "tc_common.cuh", "tc_gemm.h", "kv_common.cuh", "kv_attend.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
