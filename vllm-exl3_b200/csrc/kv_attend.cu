@@ -40,7 +40,7 @@ constexpr int kAttCtasPerSm = 2;
 
 // Requests of more query columns (rows x heads per kv head) than this go to
 // the prompt kernel when the call has such requests at all.
-constexpr int kAttFew = 16;
+constexpr int kAttFew = 32;
 
 // what a request asks for
 struct AttReq {
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) kv_attend_kernel(c
         const int64_t item = (u - base) / rq.units;
         const int off = int((u - base) - item * rq.units);
         const int n_units = int(min(int64_t(rq.units - off), u_end - u));
-        const int hk = int(item % Hk), cg = int(item / Hk);
+        const int hk = int(item / rq.groups), cg = int(item % rq.groups);
         const int ncols = min(rq.fresh * G - cg * NC, NC);
         const int64_t u_item = u - off;
         u += n_units;

@@ -37,7 +37,7 @@ __device__ __forceinline__ float ex2(float x) {
 template <bool E4M3>
 __device__ __forceinline__ uint32_t half2_lo(uint32_t w) {
     if constexpr (E4M3) {
-        return e4m3x2_to_half2(w);
+        return e4m3x2_lo(w);
     } else {
         uint32_t h = __byte_perm(w, 0x64646464u, 0x4140);  // 1024 + u
         const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&h), __float2half2_rn(1152.f));
@@ -47,7 +47,7 @@ __device__ __forceinline__ uint32_t half2_lo(uint32_t w) {
 template <bool E4M3>
 __device__ __forceinline__ uint32_t half2_hi(uint32_t w) {
     if constexpr (E4M3) {
-        return e4m3x2_to_half2(w >> 16);
+        return e4m3x2_hi(w);
     } else {
         uint32_t h = __byte_perm(w, 0x64646464u, 0x4342);
         const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&h), __float2half2_rn(1152.f));

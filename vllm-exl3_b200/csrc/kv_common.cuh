@@ -51,17 +51,22 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
     }
 }
 
-// two e4m3 codes (the low 16 bits) as f16x2, exact
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t v) {
+// two e4m3 codes (the low, the high 16 bits) as f16x2, exact
+__device__ __forceinline__ uint32_t e4m3x2_lo(uint32_t v) {
     uint32_t r;
-    asm("{\n .reg .b16 lo;\n cvt.u16.u32 lo, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(r) : "r"(v));
+    asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_hi(uint32_t v) {
+    uint32_t r;
+    asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, hi;\n}\n" : "=r"(r) : "r"(v));
     return r;
 }
 
 template <bool E4M3>
 __device__ __forceinline__ void decode4(uint32_t w, float (&v)[4]) {
     if constexpr (E4M3) {
-        const uint32_t lo = e4m3x2_to_half2(w & 0xffffu), hi = e4m3x2_to_half2(w >> 16);
+        const uint32_t lo = e4m3x2_lo(w), hi = e4m3x2_hi(w);
         const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
         const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
         v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;

@@ -8,11 +8,13 @@
 // and, with D = 128, 1024 of the other).
 //
 // Two 128-row tiles per CTA, so that one's products run while the other's
-// weights are computed.  13 warps:
+// weights are computed.  16 warps:
 //   0-3, 4-7  one row per thread: running maximum, weights, sums (tiles 0 and 1)
 //   8-11      codes of 128 keys from global memory to f16 in shared memory
 //             (128-byte swizzle; K is a K-major operand, V an MN-major one: the same bytes)
-//   12        one thread issues S = Q K^T and O += P V (tcgen05, fp32 in TMEM)
+//   12        an elected lane issues S = Q K^T and O += P V (tcgen05, fp32 in TMEM)
+//   13-15     leave at once: they make up the warpgroup whose registers the first eight warps take
+//             (184 a thread: a row's 128 scores are read from TMEM once and stay in registers)
 // TMEM: S0 S1 (128 columns each; the weights, f16, take the place of the
 // scores that they came from and are the A operand of P V), O0 O1.
 // The order of the issue S0 S1 | PV0 S0' PV1 S1' | ... keeps one tile's
@@ -33,10 +35,11 @@
 
 namespace exl3 {
 
-constexpr int kPrThreads = 13 * 32;
+constexpr int kPrThreads = 16 * 32;
 constexpr int kPrKeys = 128;        // keys per step
 constexpr int kPrRows = 256;        // query rows per CTA
 constexpr int kPrScaleSlots = 4;
+constexpr int kPrMaxSplits = 64;    // weights of the parts fit shared memory
 constexpr float kPrSlack = 8.f;     // log2: growth of the maximum that is let pass
 constexpr uint32_t kPrTmem = 512;
 
@@ -44,7 +47,7 @@ struct PrSmem {
     uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], sc_full[kPrScaleSlots];
     uint32_t tmem;
     int abort_flag, last;
-    int64_t scan[13];
+    int64_t scan[kPrThreads / 32];
     int found_b;
     int64_t found_base;
     float4 sc[kPrScaleSlots][8];  // of 16 keys: K scale, log2 V scale, 1 / V scale, 1 if the page exists
@@ -75,13 +78,24 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint3
     return d;
 }
 
-// D[tmem] (+)= A[tmem] B[smem]
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// D[tmem] (+)= A B by one elected lane of a converged warp; A in shared memory or in TMEM
+__device__ __forceinline__ void elect_umma_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
+        "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void elect_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void elect_commit(uint64_t* bar) {
+    asm volatile(
+        "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+        : "memory");
 }
 
 __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -123,6 +137,32 @@ __device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
+// two fp32 values in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+        " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}\n"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+        " add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// 8 bytes, or zeros.  Volatile: the load stays where it is written, ahead of the waits it is to overlap.
+__device__ __forceinline__ uint2 load_early(const uint8_t* p, bool get) {
+    uint2 v;
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %3, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n"
+        " @p ld.global.nc.v2.u32 {%0, %1}, [%2];\n}\n"
+        : "=r"(v.x), "=r"(v.y) : "l"(p), "r"(int(get)));
+    return v;
+}
+
 struct PrArgs {
     KvAttendArgs a;
     int splits;  // parts of a tile's keys (at most; no more than its steps)
@@ -141,7 +181,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
     PrSmem& sm = *reinterpret_cast<PrSmem*>(qs + 2 * kTile);
     volatile int* abort_flag = &sm.abort_flag;
 
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // warp: uniform
     const int Hk = a.kv_heads, G = a.group, P = 1 << a.shift;
 
     // --- which tile ---
@@ -221,9 +261,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tm = sm.tmem;
-    // columns: S0 0, S1 128, O0 256, O1 384
+    const uint32_t tm = __shfl_sync(0xffffffffu, sm.tmem, 0);
+    // columns: S0 0, S1 128, O0 256, O1 384.  Registers: 512 x 128 at launch = 256 x 184 + 128 x 96 + 128 x 48
     if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;\n");
         const int t = warp >> 2;
         if (t < nt) {
             // --- this thread's row ---
@@ -274,6 +315,84 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
             const int lo = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
             float ref = -INFINITY, l = 0.f;
             bool ok = true;
+            // of scores: above 0 whatever the scales, so that -inf stays -inf
+            auto factor = [&](float kscale) { return fmaxf(cfac * kscale, 1e-37f); };
+            // Scores of 128 keys to weights.  `edge`: some row of the warp does not see all of them.
+            auto weigh = [&](bool edge, int base, int j, const float4* sc) {
+                uint32_t v[4][32];
+                #pragma unroll
+                for (int h = 0; h < 4; ++h) tmem_load32(ts + 32 * h, v[h]);
+                #pragma unroll
+                for (int h = 0; h < 4; ++h) tmem_load_wait(v[h]);
+                if (edge) {
+                    #pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        // bit i: key base + 16 g + i is seen
+                        const int from = min(max(lo - base - 16 * g, 0), 16), to = min(max(hi - base - 16 * g, 0), 16);
+                        uint32_t bits = ((1u << to) - 1u) & ~((1u << from) - 1u);
+                        if (sc[g].w == 0.f) bits = 0u;
+                        #pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (!(bits >> i & 1u)) v[g >> 1][16 * (g & 1) + i] = 0xff800000u;  // -inf
+                    }
+                }
+                // the row's largest
+                float mx = -INFINITY;
+                #pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    const float4 s4 = sc[g];
+                    float x[16];
+                    #pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(v[g >> 1][16 * (g & 1) + i]);
+                    #pragma unroll
+                    for (int n = 8; n; n >>= 1)
+                        #pragma unroll
+                        for (int i = 0; i < n; ++i) x[i] = fmaxf(x[i], x[i + n]);
+                    mx = fmaxf(mx, fmaf(x[0], factor(s4.x), s4.y));
+                }
+                if (__any_sync(0xffffffffu, mx > ref + kPrSlack || (ref == -INFINITY && mx > ref))) {
+                    const float nref = fmaxf(ref, mx);
+                    const float alpha = ref == nref ? 1.f : ex2(ref - nref);  // 0 where nothing has been seen
+                    l *= alpha;
+                    ref = nref;
+                    if (j > 0) {
+                        if (!__all_sync(0xffffffffu, pr_wait(&sm.o_full[t], (j - 1) & 1, a.status, abort_flag))) return false;
+                        tc_fence_after();
+                        #pragma unroll 1
+                        for (int h = 0; h < D / 32; ++h) {
+                            uint32_t o[32];
+                            tmem_load32(to + 32 * h, o);
+                            tmem_load_wait(o);
+                            #pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_store32(to + 32 * h, o);
+                        }
+                    }
+                }
+                const float off = ref == -INFINITY ? 0.f : ref;
+                #pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    uint32_t p[16];
+                    #pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const float4 s4 = sc[2 * h + g];
+                        const float f = factor(s4.x);
+                        const float2 mul = make_float2(f, f), add = make_float2(s4.y - off, s4.y - off);
+                        float2 sum = make_float2(0.f, 0.f);
+                        #pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            const float2 raw = make_float2(__uint_as_float(v[h][16 * g + i]), __uint_as_float(v[h][16 * g + i + 1]));
+                            float2 x = fma2(raw, mul, add);
+                            x = make_float2(ex2(x.x), ex2(x.y));
+                            sum = add2(sum, x);
+                            p[8 * g + i / 2] = pack_half2(x.x, x.y);
+                        }
+                        l = fmaf(sum.x + sum.y, s4.z, l);
+                    }
+                    tmem_store16(ts + 16 * h, p);
+                }
+                return true;
+            };
             for (int j = 0; j < steps; ++j) {
                 const int base = key0 + j * kPrKeys;
                 ok = pr_wait(&sm.sc_full[j & 3], (j >> 2) & 1, a.status, abort_flag) &&
@@ -287,80 +406,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
                 for (int g = 0; g < 8; ++g) dead |= sc[g].w == 0.f;
                 const bool edge = __any_sync(0xffffffffu, dead);
 
-                // largest score of the row
-                float mx = -INFINITY;
-                #pragma unroll 1
-                for (int h = 0; h < 4; ++h) {
-                    uint32_t v[32];
-                    tmem_load32(ts + 32 * h, v);
-                    tmem_load_wait(v);
-                    #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const float4 s4 = sc[2 * h + g];
-                        const int kb = base + 32 * h + 16 * g;
-                        float gm = -INFINITY;
-                        if (!edge) {
-                            #pragma unroll
-                            for (int i = 0; i < 16; ++i) gm = fmaxf(gm, __uint_as_float(v[16 * g + i]));
-                        } else {
-                            #pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (kb + i < hi && kb + i >= lo) gm = fmaxf(gm, __uint_as_float(v[16 * g + i]));
-                            if (s4.w == 0.f) gm = -INFINITY;
-                        }
-                        mx = fmaxf(mx, fmaf(gm, cfac * s4.x, s4.y));
-                    }
-                }
-                if (__any_sync(0xffffffffu, mx > ref + kPrSlack || (ref == -INFINITY && mx > ref))) {
-                    const float nref = fmaxf(ref, mx);
-                    const float alpha = ref == -INFINITY ? 0.f : ex2(ref - nref);
-                    l = ref == nref ? l : l * alpha;
-                    const float scale = ref == nref ? 1.f : alpha;
-                    ref = nref;
-                    if (j > 0) {
-                        ok = __all_sync(0xffffffffu, pr_wait(&sm.o_full[t], (j - 1) & 1, a.status, abort_flag));
-                        if (!ok) break;
-                        tc_fence_after();
-                        #pragma unroll 1
-                        for (int h = 0; h < D / 32; ++h) {
-                            uint32_t o[32];
-                            tmem_load32(to + 32 * h, o);
-                            tmem_load_wait(o);
-                            #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * scale);
-                            tmem_store32(to + 32 * h, o);
-                        }
-                    }
-                }
-                const float off = ref == -INFINITY ? 0.f : ref;
-                // weights
-                #pragma unroll 1
-                for (int h = 0; h < 4; ++h) {
-                    uint32_t v[32], p[16];
-                    tmem_load32(ts + 32 * h, v);
-                    tmem_load_wait(v);
-                    #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const float4 s4 = sc[2 * h + g];
-                        const int kb = base + 32 * h + 16 * g;
-                        const float mul = cfac * s4.x, add = s4.y - off;
-                        float sum = 0.f;
-                        #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            float x = fmaf(__uint_as_float(v[16 * g + i]), mul, add);
-                            float y = fmaf(__uint_as_float(v[16 * g + i + 1]), mul, add);
-                            if (edge) {
-                                if (kb + i >= hi || kb + i < lo || s4.w == 0.f) x = -INFINITY;
-                                if (kb + i + 1 >= hi || kb + i + 1 < lo || s4.w == 0.f) y = -INFINITY;
-                            }
-                            x = ex2(x), y = ex2(y);
-                            sum += x + y;
-                            p[8 * g + i / 2] = pack_half2(x, y);
-                        }
-                        l = fmaf(sum, s4.z, l);
-                    }
-                    tmem_store16(ts + 16 * h, p);
-                }
+                ok = weigh(edge, base, j, sc);
+                if (!ok) break;
                 tmem_store_wait();
                 tc_fence_before();
                 mbar_arrive(&sm.p_full[t]);
@@ -419,199 +466,212 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
             }
             tc_fence_before();
         }
+        named_bar_arrive(1, 288);
+        if (ns == 1) return;
+
+        // --- join the parts of the keys: the CTA that ends last, in key order ---
+        named_bar_sync(2, 256);
+        if (tid == 0) {
+            int prev;
+            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(prev) : "l"(a.counters + item) : "memory");
+            sm.last = prev == ns - 1;
+            if (prev == ns - 1) a.counters[item] = 0;  // ready for the next call
+        }
+        named_bar_sync(2, 256);
+        if (!sm.last) return;
+        const float* parts = a.part + item * args.splits * int64_t(kPrRows) * (D + 2);
+        const int64_t pitch = int64_t(kPrRows) * (D + 2);
+        float* wt = reinterpret_cast<float*>(smem);  // [ns][rows]
+        for (int f = tid; f < rows; f += 256) {
+            float mx = -INFINITY, sum = 0.f;
+            for (int p = 0; p < ns; ++p) mx = fmaxf(mx, __ldcg(parts + p * pitch + f));
+            for (int p = 0; p < ns; ++p) {
+                const float w = mx == -INFINITY ? 0.f : ex2(__ldcg(parts + p * pitch + f) - mx);
+                wt[p * kPrRows + f] = w;
+                sum = fmaf(__ldcg(parts + p * pitch + kPrRows + f), w, sum);
+            }
+            sm.wt[f] = sum;
+            const int64_t row = row0 + (col0 + f) / G;
+            if (a.lse && row < a.q_rows)
+                a.lse[row * a.heads + hk * G + (col0 + f) % G] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
+        }
+        named_bar_sync(2, 256);
+        for (int i = tid; i < rows * (D / 4); i += 256) {
+            const int f = i / (D / 4), d = 4 * (i % (D / 4));
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            #pragma unroll 4
+            for (int p = 0; p < ns; ++p) {
+                const float4 o = __ldcg(reinterpret_cast<const float4*>(parts + p * pitch + 2 * kPrRows + f * D + d));
+                const float w = wt[p * kPrRows + f];
+                v.x = fmaf(o.x, w, v.x), v.y = fmaf(o.y, w, v.y), v.z = fmaf(o.z, w, v.z), v.w = fmaf(o.w, w, v.w);
+            }
+            const float sum = sm.wt[f], inv = sum == 0.f ? 0.f : 1.f / sum;
+            const int64_t row = row0 + (col0 + f) / G;
+            if (row >= a.q_rows) continue;
+            uint2 w;
+            if constexpr (BF16) {
+                const __nv_bfloat162 x = __floats2bfloat162_rn(v.x * inv, v.y * inv), y = __floats2bfloat162_rn(v.z * inv, v.w * inv);
+                w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+            } else {
+                w = make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
+            }
+            if (sum == 0.f) w = make_uint2(0u, 0u);
+            *reinterpret_cast<uint2*>(a.out + (row * a.heads + hk * G + (col0 + f) % G) * D + d) = w;
+        }
     } else if (warp < 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
         // --- codes to f16 ---
-        constexpr int CH = D / 16;           // 16-byte loads per key
-        constexpr int RPP = 128 / CH;        // keys per pass
-        constexpr int NP = kPrKeys / RPP;
-        const int ct = tid - 256, kr = ct / CH, ch = ct % CH;
+        // a thread takes 8 dims of each 64-dim block of a key: 8 lanes' 16-byte stores of one block
+        // fall on 8 different places of a swizzled 128-byte row
+        constexpr int NB = D / 64;
+        constexpr int NP = 4;                // passes of 16 keys (of one page) to half a step
+        const int ct = tid - 256, kr = ct >> 3, ch = ct & 7;
         const int32_t* row_table = a.table + int64_t(b) * a.width;
-        auto page_of = [&](int key) {  // of a key below len
-            const int p = row_table[key >> a.shift];
-            if (p >= 0 && p < a.pages) return p;
-            set_status(a.status, DEV_BAD_INDEX);
-            return -1;
+        // Of the 16 keys (lane & 7) of a step: whether the tile sees any, and their page as the
+        // table has it.  It is looked at one step later, when its load has long arrived.
+        auto key_of = [&](int j) { return key0 + j * kPrKeys + 16 * (lane & 7); };
+        auto some = [&](int j) { return j < steps && key_of(j) + 16 > lo_all && key_of(j) < hi_all; };
+        auto raw_page = [&](int j) { return some(j) ? __ldg(row_table + (key_of(j) >> a.shift)) : -1; };
+        auto page_of = [&](int j, int raw) {
+            const bool in = raw >= 0 && raw < a.pages;
+            if (some(j) && !in) set_status(a.status, DEV_BAD_INDEX);
+            return in ? raw : -1;
         };
-        auto pages = [&](int j, int (&pg)[NP]) {
+        const int64_t page_bytes = (int64_t(Hk) * D) << a.shift;
+        const int64_t mine = (int64_t(hk) * D << a.shift) + kr * D + ch * 8;
+        auto load = [&](const uint8_t* codes, int j, int half, int pg, uint2 (&w)[NP][NB]) {
             #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                const int key = key0 + j * kPrKeys + i * RPP + kr;
+                const int key = key0 + j * kPrKeys + (half * NP + i) * 16, pi = __shfl_sync(0xffffffffu, pg, half * NP + i);
+                const uint8_t* p = codes + pi * page_bytes + mine + (key & (P - 1)) * D;
                 // keys that no row sees are zeros: their codes may be NaN, and 0 * NaN is not 0
-                pg[i] = j < steps && key >= lo_all && key < hi_all ? page_of(key) : -1;
-            }
-        };
-        auto load = [&](const uint8_t* codes, int j, const int (&pg)[NP], uint4 (&w)[NP]) {
-            #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int key = key0 + j * kPrKeys + i * RPP + kr;
-                const uint8_t* p = codes + (((int64_t(max(pg[i], 0)) * Hk + hk) << a.shift) + (key & (P - 1))) * D + ch * 16;
-                w[i] = pg[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
-            }
-        };
-        auto put = [&](char* dst, const uint4 (&w)[NP], const int (&pg)[NP]) {
-            #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int key = i * RPP + kr;
-                const uint32_t in[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-                uint32_t o[8];
+                const bool get = pi >= 0 && key + kr >= lo_all && key + kr < hi_all;
                 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const uint32_t c = code_word<E4M3>(in[q]);
-                    o[2 * q] = half2_lo<E4M3>(c), o[2 * q + 1] = half2_hi<E4M3>(c);
-                    if (!E4M3 && pg[i] < 0) o[2 * q] = o[2 * q + 1] = 0u;
-                }
-                // lanes of dims 64 and up store their halves in the other order: 8 lanes, 8 banks of 16 bytes
-                char* rowp = dst + (ch >> 2) * kBlk + key * 128;
-                const int c0 = 2 * (ch & 3), sw = key & 7;
-                const bool flip = ch >= 4;
-                const uint4 x = make_uint4(o[0], o[1], o[2], o[3]), y = make_uint4(o[4], o[5], o[6], o[7]);
-                *reinterpret_cast<uint4*>(rowp + (((c0 + (flip ? 1 : 0)) ^ sw) << 4)) = flip ? y : x;
-                *reinterpret_cast<uint4*>(rowp + (((c0 + (flip ? 0 : 1)) ^ sw) << 4)) = flip ? x : y;
+                for (int n = 0; n < NB; ++n) w[i][n] = load_early(p + 64 * n, get);
             }
+        };
+        const uint32_t place = uint32_t(kr * 128 + ((ch ^ (kr & 7)) << 4));
+        auto put = [&](char* dst, int half, const uint2 (&w)[NP][NB]) {
+            #pragma unroll
+            for (int i = 0; i < NP; ++i)
+                #pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    const uint32_t x = code_word<E4M3>(w[i][n].x), y = code_word<E4M3>(w[i][n].y);
+                    *reinterpret_cast<uint4*>(dst + n * kBlk + (half * NP + i) * (16 * 128) + place) =
+                        make_uint4(half2_lo<E4M3>(x), half2_hi<E4M3>(x), half2_lo<E4M3>(y), half2_hi<E4M3>(y));
+                }
+        };
+        auto handed = [&](uint64_t* bar) {
             fence_async_smem();
             __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
         };
-        auto scales = [&](int j) {  // of 16 keys, by the first 8 threads
-            const int key = key0 + j * kPrKeys + 16 * ct;
-            if (ct >= 8 || j >= steps || key + 16 <= lo_all || key >= hi_all) return make_float4(0.f, 0.f, 1.f, 1.f);
-            const int pg = page_of(key);
-            if (pg < 0) return make_float4(0.f, 0.f, 1.f, 0.f);
-            const int64_t at = int64_t(pg) * Hk + hk;
-            const int ve = stored_exponent(__ldg(a.v_scale + at));
-            return make_float4(__ldg(a.k_scale + at), float(ve), exp2_int(-ve), 1.f);
+        float ks = 0.f, vs = 1.f;  // of lanes 0-7 of warp 8: their 16 keys' scales
+        auto scales = [&](int pg) {
+            if (warp != 8 || pg < 0) return;
+            ks = __ldg(a.k_scale + int64_t(pg) * Hk + hk);
+            vs = __ldg(a.v_scale + int64_t(pg) * Hk + hk);
         };
-        int pg[NP], pn[NP];
-        uint4 kw[NP], vw[NP];
-        pages(0, pg);
-        load(a.k, 0, pg, kw);
-        float4 sc = scales(0);
-        bool ok = true;
+        // two halves are on their way while a third is written
+        uint2 k0[NP][NB], k1[NP][NB], v0[NP][NB], v1[NP][NB];
+        int pg = page_of(0, raw_page(0)), raw = raw_page(1);
+        load(a.k, 0, 0, pg, k0);
+        load(a.k, 0, 1, pg, k1);
+        scales(pg);
         for (int j = 0; j < steps; ++j) {
             const int s = j & 1;
-            load(a.v, j, pg, vw);
-            pages(j + 1, pn);
-            if (j >= 2) ok = pr_wait(&sm.k_empty[s], ((j >> 1) - 1) & 1, a.status, abort_flag);
+            bool ok = j < 2 || pr_wait(&sm.k_empty[s], ((j >> 1) - 1) & 1, a.status, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) break;
-            put(kst + s * kTile, kw, pg);
+            put(kst + s * kTile, 0, k0);
+            load(a.v, j, 0, pg, v0);
+            put(kst + s * kTile, 1, k1);
+            load(a.v, j, 1, pg, v1);
             if (warp == 8) {
-                if (ct < 8) sm.sc[j & 3][ct] = sc;
+                const int ve = stored_exponent(vs);
+                if (lane < 8)
+                    sm.sc[j & 3][lane] = pg < 0 ? make_float4(0.f, 0.f, 1.f, some(j) ? 0.f : 1.f)
+                                                : make_float4(ks, float(ve), exp2_int(-ve), 1.f);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.sc_full[j & 3]);
             }
-            if (lane == 0) mbar_arrive(&sm.k_full[s]);
-            if (warp == 8) sc = scales(j + 1);
-            load(a.k, j + 1, pn, kw);
-            if (j >= 2) ok = pr_wait(&sm.v_empty[s], ((j >> 1) - 1) & 1, a.status, abort_flag);
+            handed(&sm.k_full[s]);
+            pg = page_of(j + 1, raw);
+            raw = raw_page(j + 2);
+            scales(pg);
+            ok = j < 2 || pr_wait(&sm.v_empty[s], ((j >> 1) - 1) & 1, a.status, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) break;
-            put(vst + s * kTile, vw, pg);
-            if (lane == 0) mbar_arrive(&sm.v_full[s]);
-            #pragma unroll
-            for (int i = 0; i < NP; ++i) pg[i] = pn[i];
+            put(vst + s * kTile, 0, v0);
+            load(a.k, j + 1, 0, pg, k0);
+            put(vst + s * kTile, 1, v1);
+            load(a.k, j + 1, 1, pg, k1);
+            handed(&sm.v_full[s]);
         }
-    } else if (lane == 0 && steps > 0) {
-        // --- the products; a stage is handed back only where it will be filled again, so the last
-        // arrival that is on its way is one that somebody waits for ---
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
+      if (warp > 12) return;
+      if (steps > 0) {
+        // --- the products.  The whole warp runs this, so that addresses stay in uniform registers; an
+        // elected lane issues.  A stage is handed back only where it will be filled again, so the last
+        // arrival on its way is one that somebody waits for ---
         constexpr uint32_t idesc_s = umma_idesc_f16_f32(128, kPrKeys);
         constexpr uint32_t idesc_o = umma_idesc_f16_f32(128, D) | (1u << 16);  // V: MN-major
-        const uint32_t q0 = smem_u32(qs), k0 = smem_u32(kst), v0 = smem_u32(vst);
+        constexpr uint32_t kStep = kTile >> 4;
+        const uint64_t q0 = umma_desc_k_sw128(smem_u32(qs)), k0 = umma_desc_k_sw128(smem_u32(kst));
+        const uint64_t v0 = umma_desc_mn_sw128(smem_u32(vst), kBlk);
         auto scores = [&](int t, int s) {
+            const uint64_t qd = q0 + uint32_t(t) * kStep, kd = k0 + uint32_t(s) * kStep;
             #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-                const uint32_t at = uint32_t((i >> 2) * kBlk + (i & 3) * 32);
-                umma_f16(tm + 128 * t, umma_desc_k_sw128(q0 + t * kTile + at), umma_desc_k_sw128(k0 + s * kTile + at),
-                         idesc_s, i > 0);
+                const uint32_t at = uint32_t((i >> 2) * kBlk + (i & 3) * 32) >> 4;
+                elect_umma_ss(tm + 128 * t, qd + at, kd + at, idesc_s, i > 0);
             }
-            umma_commit(&sm.s_full[t]);
+            elect_commit(&sm.s_full[t]);
         };
-        bool ok = pr_wait(&sm.q_full, 0, a.status, abort_flag) && pr_wait(&sm.k_full[0], 0, a.status, abort_flag);
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            return __all_sync(0xffffffffu, pr_wait(bar, parity, a.status, abort_flag)) != 0;
+        };
+        bool ok = wait(&sm.q_full, 0) && wait(&sm.k_full[0], 0);
         tc_fence_after();
         if (ok) {
             for (int t = 0; t < nt; ++t) scores(t, 0);
-            if (steps > 2) umma_commit(&sm.k_empty[0]);
+            if (steps > 2) elect_commit(&sm.k_empty[0]);
         }
         for (int j = 0; ok && j < steps; ++j) {
             const int s = j & 1, sn = (j + 1) & 1;
             const bool more = j + 1 < steps;
-            if (more) ok = pr_wait(&sm.k_full[sn], ((j + 1) >> 1) & 1, a.status, abort_flag);
-            ok = ok && pr_wait(&sm.v_full[s], (j >> 1) & 1, a.status, abort_flag);
+            if (more) ok = wait(&sm.k_full[sn], ((j + 1) >> 1) & 1);
+            ok = ok && wait(&sm.v_full[s], (j >> 1) & 1);
             for (int t = 0; ok && t < nt; ++t) {
-                ok = pr_wait(&sm.p_full[t], j & 1, a.status, abort_flag);
+                ok = wait(&sm.p_full[t], j & 1);
                 if (!ok) break;
                 tc_fence_after();
+                const uint64_t vd = v0 + uint32_t(s) * kStep;
                 #pragma unroll
                 for (int i = 0; i < kPrKeys / 16; ++i)
-                    umma_f16_ts(tm + 256 + 128 * t, tm + 128 * t + 8 * i,
-                                umma_desc_mn_sw128(v0 + s * kTile + 2048 * i, kBlk), idesc_o, j > 0 || i > 0);
-                umma_commit(&sm.o_full[t]);
+                    elect_umma_ts(tm + 256 + 128 * t, tm + 128 * t + 8 * i, vd + uint32_t(2048 * i >> 4), idesc_o,
+                                  i > 0 ? 1u : uint32_t(j > 0));
+                elect_commit(&sm.o_full[t]);
                 if (more) scores(t, sn);
             }
             if (!ok) break;
-            if (j + 2 < steps) umma_commit(&sm.v_empty[s]);
-            if (j + 3 < steps) umma_commit(&sm.k_empty[sn]);
+            if (j + 2 < steps) elect_commit(&sm.v_empty[s]);
+            if (j + 3 < steps) elect_commit(&sm.k_empty[sn]);
         }
         // after a wait that ran out: the products in flight still use TMEM and shared memory
         if (!ok) {
-            mbar_init(&sm.q_full, 1);
-            mbar_fence_init();
-            umma_commit(&sm.q_full);
+            if (lane == 0) {
+                mbar_init(&sm.q_full, 1);
+                mbar_fence_init();
+            }
+            __syncwarp();
+            elect_commit(&sm.q_full);
             mbar_wait(&sm.q_full, 0, a.status);
         }
-    }
-    __syncwarp();
-    __syncthreads();
-    if (warp == 12) {
-        tc_fence_after();
-        tmem_dealloc(tm, kPrTmem);
-    }
-    if (ns == 1) return;
-
-    // --- join the parts of the keys: the CTA that ends last, in key order ---
-    if (tid == 0) {
-        int prev;
-        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(prev) : "l"(a.counters + item) : "memory");
-        sm.last = prev == ns - 1;
-        if (prev == ns - 1) a.counters[item] = 0;  // ready for the next call
-    }
-    __syncthreads();
-    if (!sm.last) return;
-    const float* parts = a.part + item * args.splits * int64_t(kPrRows) * (D + 2);
-    const int64_t pitch = int64_t(kPrRows) * (D + 2);
-    float* wt = reinterpret_cast<float*>(qs);  // [ns][rows]
-    for (int f = tid; f < rows; f += kPrThreads) {
-        float mx = -INFINITY, sum = 0.f;
-        for (int p = 0; p < ns; ++p) mx = fmaxf(mx, __ldcg(parts + p * pitch + f));
-        for (int p = 0; p < ns; ++p) {
-            const float w = mx == -INFINITY ? 0.f : ex2(__ldcg(parts + p * pitch + f) - mx);
-            wt[p * kPrRows + f] = w;
-            sum = fmaf(__ldcg(parts + p * pitch + kPrRows + f), w, sum);
-        }
-        sm.wt[f] = sum;
-        const int64_t row = row0 + (col0 + f) / G;
-        if (a.lse && row < a.q_rows)
-            a.lse[row * a.heads + hk * G + (col0 + f) % G] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
-    }
-    __syncthreads();
-    for (int i = tid; i < rows * (D / 4); i += kPrThreads) {
-        const int f = i / (D / 4), d = 4 * (i % (D / 4));
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        #pragma unroll 4
-        for (int p = 0; p < ns; ++p) {
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(parts + p * pitch + 2 * kPrRows + f * D + d));
-            const float w = wt[p * kPrRows + f];
-            v.x = fmaf(o.x, w, v.x), v.y = fmaf(o.y, w, v.y), v.z = fmaf(o.z, w, v.z), v.w = fmaf(o.w, w, v.w);
-        }
-        const float sum = sm.wt[f], inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int64_t row = row0 + (col0 + f) / G;
-        if (row >= a.q_rows) continue;
-        uint2 w;
-        if constexpr (BF16) {
-            const __nv_bfloat162 x = __floats2bfloat162_rn(v.x * inv, v.y * inv), y = __floats2bfloat162_rn(v.z * inv, v.w * inv);
-            w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-        } else {
-            w = make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
-        }
-        if (sum == 0.f) w = make_uint2(0u, 0u);
-        *reinterpret_cast<uint2*>(a.out + (row * a.heads + hk * G + (col0 + f) % G) * D + d) = w;
+      }
+      __syncwarp();
+      named_bar_sync(1, 288);  // the rows are read
+      tc_fence_after();
+      tmem_dealloc(tm, kPrTmem);
     }
 }
 
@@ -622,7 +682,7 @@ KvPromptPlan kv_prompt_plan(const KvAttendCall& c, int sms) {
     KvPromptPlan p;
     p.tiles = c.q_rows * group / kPrRows + c.requests;
     const int64_t items = p.tiles * c.kv_heads;
-    p.splits = items > 0 && items * 2 <= sms ? int(sms / items) : 1;
+    p.splits = items > 0 && items * 2 <= sms ? int(sms / items < kPrMaxSplits ? sms / items : kPrMaxSplits) : 1;
     p.bytes = p.splits > 1 ? size_t(items) * p.splits * kPrRows * (c.dim + 2) * 4 : 0;
     return p;
 }
@@ -630,7 +690,7 @@ KvPromptPlan kv_prompt_plan(const KvAttendCall& c, int sms) {
 template <bool E4M3, bool BF16, int D>
 static cudaError_t launch_prompt(const PrArgs& a, unsigned grid, cudaStream_t s) {
     constexpr size_t smem = pr_smem_bytes<D>();
-    static_assert(smem <= 227 * 1024, "shared memory");
+    static_assert(smem <= 227 * 1024 && kPrMaxSplits * kPrRows * 4 + sizeof(PrSmem) + 1024 <= smem, "shared memory");
     auto* kernel = kv_prompt_kernel<E4M3, BF16, D>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (e != cudaSuccess) return e;
