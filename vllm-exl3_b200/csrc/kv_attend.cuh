@@ -27,12 +27,6 @@ struct KvAttendArgs {
     int* status;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // two codes (bytes 0, 1 of w; int8 already offset by 128) as f16x2, exact
 template <bool E4M3>
 __device__ __forceinline__ uint32_t half2_lo(uint32_t w) {

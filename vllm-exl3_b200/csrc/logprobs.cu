@@ -35,7 +35,8 @@ namespace exl3 {
 constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
 constexpr int kLpCap = 2048;     // candidate keys a CTA holds
 constexpr int kLpMaxTop = 32;    // one group maximum each
-constexpr int kLpMaxSplit = 64;  // splits * top <= kLpCap
+constexpr int kLpMaxSplit = 64;
+static_assert(kLpMaxSplit * kLpMaxTop <= kLpCap, "the parts' lists are joined in one buffer");
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct LpArgs {
@@ -60,12 +61,6 @@ struct LpStats {
     int above;
 };
 
-__device__ __forceinline__ float lp_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -76,7 +71,7 @@ __device__ __forceinline__ void lp_join(LpStats& a, const LpStats& b) {
     const float m = fmaxf(a.m, b.m);
     auto bring = [m](const LpStats& p, float& s, float& w) {
         const float d = p.m == m ? 0.f : p.m - m;
-        const float f = lp_ex2(d * kLog2e);
+        const float f = ex2(d * kLog2e);
         s = p.s * f;
         w = f == 0.f ? 0.f : (p.w + p.s * d) * f;
     };
@@ -84,6 +79,13 @@ __device__ __forceinline__ void lp_join(LpStats& a, const LpStats& b) {
     bring(a, sa, wa);
     bring(b, sb, wb);
     a.m = m, a.s = sa + sb, a.w = wa + wb, a.above += b.above;
+}
+
+__device__ __forceinline__ void lp_join_warp(LpStats& st) {
+    #pragma unroll
+    for (int d = 16; d; d >>= 1)
+        lp_join(st, LpStats{__shfl_xor_sync(0xffffffffu, st.m, d), __shfl_xor_sync(0xffffffffu, st.s, d),
+                            __shfl_xor_sync(0xffffffffu, st.w, d), __shfl_xor_sync(0xffffffffu, st.above, d)});
 }
 
 __device__ __forceinline__ uint32_t sortable(float x) {  // ascending; NaN as -inf, -0 as 0
@@ -122,18 +124,66 @@ struct LpType {
             return (i & 1) ? __high2float(h) : __low2float(h);
         }
     }
+    static __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
+        return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+    }
+    static __device__ __forceinline__ __half2 h2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+    static __device__ __forceinline__ __nv_bfloat162 b2(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
     static __device__ __forceinline__ float largest(const uint4& v) {  // NaN left out unless all are
         if constexpr (DT == DT_F32) {
             return fmaxf(fmaxf(get(v, 0), get(v, 1)), fmaxf(get(v, 2), get(v, 3)));
         } else if constexpr (DT == DT_BF16) {
-            auto b = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
-            const __nv_bfloat162 m = __hmax2(__hmax2(b(v.x), b(v.y)), __hmax2(b(v.z), b(v.w)));
+            const __nv_bfloat162 m = __hmax2(__hmax2(b2(v.x), b2(v.y)), __hmax2(b2(v.z), b2(v.w)));
             return fmaxf(__low2float(m), __high2float(m));
         } else {
-            auto b = [](uint32_t w) { return *reinterpret_cast<const __half2*>(&w); };
-            const __half2 m = __hmax2(__hmax2(b(v.x), b(v.y)), __hmax2(b(v.z), b(v.w)));
+            const __half2 m = __hmax2(__hmax2(h2(v.x), h2(v.y)), __hmax2(h2(v.z), h2(v.w)));
             return fmaxf(__low2float(m), __high2float(m));
         }
+    }
+    // A reference this near 0 is far above the lowest number: their difference has weight 0 and is finite.
+    static constexpr float kNear = DT == DT_F16 ? 3e4f : 1e35f;
+    // entries 2 i and 2 i + 1, -inf as the lowest number
+    static __device__ __forceinline__ float2 pair(const uint4& v, int i) {
+        if constexpr (DT == DT_F32) {
+            return make_float2(max_nan(get(v, 2 * i), -3.3e38f), max_nan(get(v, 2 * i + 1), -3.3e38f));
+        } else if constexpr (DT == DT_BF16) {
+            const __nv_bfloat162 x = __hmax2_nan(b2(word(v, i)), b2(0xff7fff7fu));
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(&x);
+            return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+        } else {
+            return __half22float2(__hmax2_nan(h2(word(v, i)), h2(0xfbfffbffu)));
+        }
+    }
+    // Counts: of 16-bit types two at a time, as sums of ones (at most 32 a half before total())
+    using Count = std::conditional_t<DT == DT_F32, int, std::conditional_t<DT == DT_F16, __half2, __nv_bfloat162>>;
+    static __device__ __forceinline__ Count zero() {
+        if constexpr (DT == DT_F32) return 0;
+        else if constexpr (DT == DT_F16) return h2(0u);
+        else return b2(0u);
+    }
+    template <bool GE>
+    static __device__ __forceinline__ void count(Count& n, const uint4& v, float xt) {
+        if constexpr (DT == DT_F32) {
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) n += GE ? get(v, i) >= xt : get(v, i) > xt;
+        } else {
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (DT == DT_F16) {
+                    const __half2 t = __float2half2_rn(xt);  // exact: an entry of the row, or +inf
+                    n = __hadd2(n, GE ? __hge2(h2(word(v, i)), t) : __hgt2(h2(word(v, i)), t));
+                } else {
+                    const __nv_bfloat162 t = __float2bfloat162_rn(xt);
+                    n = __hadd2(n, GE ? __hge2(b2(word(v, i)), t) : __hgt2(b2(word(v, i)), t));
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ void count_ge(Count& n, const uint4& v, float xt) { count<true>(n, v, xt); }
+    static __device__ __forceinline__ void count_gt(Count& n, const uint4& v, float xt) { count<false>(n, v, xt); }
+    static __device__ __forceinline__ int total(Count n) {
+        if constexpr (DT == DT_F32) return n;
+        else return int(__low2float(n)) + int(__high2float(n));
     }
 };
 
@@ -143,7 +193,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
     constexpr int VEC = T::kVec;
     extern __shared__ uint64_t lp_smem[];
     uint64_t* cand = lp_smem;            // [kLpCap]
-    uint64_t* best = lp_smem + kLpCap;   // [kLpMaxTop]
+    uint64_t* best = lp_smem + kLpCap;   // [kLpMaxSplit], at least kLpMaxTop
     __shared__ uint32_t group_max[32];
     __shared__ float wr[kLpWarps], ws[kLpWarps], ww[kLpWarps];
     __shared__ int wc[kLpWarps];
@@ -202,25 +252,47 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
         // --- sums ---
         LpStats part{mx, 0.f, 0.f, 0};
         const float ref = mx == -INFINITY ? 0.f : mx;
+        if (fabsf(ref) < T::kNear) {
+            // two at a time.  -inf stands as the type's lowest number: its weight is 0 against such
+            // a reference, and 0 times the difference stays 0
+            const float2 neg = make_float2(-ref, -ref), l2 = make_float2(kLog2e, kLog2e);
+            float2 s2 = make_float2(0.f, 0.f), w2 = make_float2(0.f, 0.f);
+            #pragma unroll
+            for (int u = 0; u < U; ++u)
+                #pragma unroll
+                for (int i = 0; i < VEC / 2; ++i) {
+                    const float2 d = add2(T::pair(v[u], i), neg);
+                    const float2 t = mul2(d, l2);
+                    const float2 e = make_float2(ex2(t.x), ex2(t.y));
+                    s2 = add2(s2, e);
+                    w2 = fma2(e, d, w2);
+                }
+            part.s = s2.x + s2.y, part.w = w2.x + w2.y;
+        } else {
+            #pragma unroll 1
+            for (int u = 0; u < U; ++u) {
+                const int64_t j = j0 + u * kLpThreads;
+                const uint4 again = load(j, j * VEC - shift);
+                #pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float d = max_nan(T::get(again, i) - ref, -300.f);
+                    const float e = ex2(d * kLog2e);
+                    part.s += e;
+                    part.w = fmaf(e, d, part.w);
+                }
+            }
+        }
+        // --- rank: entries above the token, and before it as high ---
+        typename T::Count before_n = T::zero(), after_n = T::zero();
         #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t e0 = (j0 + u * kLpThreads) * VEC - shift;
-            #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                // -inf takes -300: its weight is 0, and 0 * -300 is 0
-                const float d = max_nan(T::get(v[u], i) - ref, -300.f);
-                const float e = lp_ex2(d * kLog2e);
-                part.s += e;
-                part.w = fmaf(e, d, part.w);
-            }
             if (e0 + VEC <= tok) {
-                #pragma unroll
-                for (int i = 0; i < VEC; ++i) part.above += T::get(v[u], i) >= xt;
+                T::count_ge(before_n, v[u], xt);
                 // entries before the row's first one are no part of it
                 if (e0 < 0 && xt == -INFINITY) part.above += int(e0);
             } else if (e0 > tok) {
-                #pragma unroll
-                for (int i = 0; i < VEC; ++i) part.above += T::get(v[u], i) > xt;
+                T::count_gt(after_n, v[u], xt);
             } else {
                 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
@@ -229,6 +301,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
                 }
             }
         }
+        part.above += T::total(before_n) + T::total(after_n);
         lp_join(st, part);
 
         // --- alternatives ---
@@ -287,12 +360,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
     }
 
     // --- join the threads ---
-    #pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        LpStats o{__shfl_xor_sync(0xffffffffu, st.m, d), __shfl_xor_sync(0xffffffffu, st.s, d),
-                  __shfl_xor_sync(0xffffffffu, st.w, d), __shfl_xor_sync(0xffffffffu, st.above, d)};
-        lp_join(st, o);
-    }
+    lp_join_warp(st);
     if (lane == 0) wr[warp] = st.m, ws[warp] = st.s, ww[warp] = st.w, wc[warp] = st.above;
     __syncthreads();
     st = LpStats{wr[0], ws[0], ww[0], wc[0]};
@@ -312,18 +380,32 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
         }
         __syncthreads();
         if (!last_flag) return;
-        for (int i = 0; i < a.splits; ++i) {
+        // lane i takes parts i and i + 32, then the lanes join: the same order every time
+        st = LpStats{-INFINITY, 0.f, 0.f, 0};
+        for (int i = lane; i < a.splits; i += 32) {
             const float4 o = __ldcg(a.stats + row * a.splits + i);
-            const LpStats p{o.x, o.y, o.z, __float_as_int(o.w)};
-            if (i == 0) st = p;
-            else lp_join(st, p);
+            lp_join(st, LpStats{o.x, o.y, o.z, __float_as_int(o.w)});
         }
-        if (a.top) {
-            if (tid == 0) count = 0;
+        lp_join_warp(st);
+        if constexpr (TOP) {
+            // The lists are in order.  With c + 1 the keys of a list that are surely enough from m
+            // lists, c = ceil(top / splits) - 1, m = ceil(top / (c + 1)): the m-th largest of the
+            // lists' c-th keys bounds the answer from below, and little more than `top` keys pass it.
+            const int c = (a.top - 1) / a.splits, m = (a.top + c) / (c + 1);
+            const uint64_t* keys = a.keys + row * a.splits * a.top;
+            if (tid < a.splits) best[tid] = __ldcg(keys + tid * a.top + c);
+            if (tid == 0) count = 0, bound = 0;
             __syncthreads();
+            if (tid < a.splits) {
+                int n = 0;
+                for (int i = 0; i < a.splits; ++i) n += best[i] > best[tid] || (best[i] == best[tid] && i < tid);
+                if (n == m - 1) bound = best[tid];
+            }
+            __syncthreads();
+            const uint64_t least = max(bound, uint64_t(1));  // 0: no key
             for (int i = tid; i < a.splits * a.top; i += kLpThreads) {
-                const uint64_t k = __ldcg(a.keys + row * a.splits * a.top + i);
-                if (k) cand[atomicAdd(&count, 1)] = k;  // no entry's key is 0
+                const uint64_t k = __ldcg(keys + i);
+                if (k >= least) cand[atomicAdd(&count, 1)] = k;
             }
             __syncthreads();
             lp_reduce(cand, best, count, a.top);
@@ -345,7 +427,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
 
 // A row's chunks of 256 threads x U vectors (one vector more than the row's
 // own where its start is not aligned), and over how many CTAs it is split:
-// enough for two CTAs per SM.
+// what runs at once (4 CTAs per SM).
 struct LpPlan {
     int U, chunks, splits;
 };
@@ -355,13 +437,13 @@ static LpPlan lp_plan(const LogprobsCall& c, int sms) {
     // few rows: chunks of 2 vectors, so that a row spreads over four times the CTAs
     const int U = c.rows * chunks(8) < sms ? 2 : 8;
     LpPlan p{U, chunks(U), 1};
-    const int64_t want = (2 * int64_t(sms) + c.rows - 1) / c.rows;
-    p.splits = int(want < p.chunks ? want : p.chunks);
+    const int64_t want = 4 * int64_t(sms) / c.rows;
+    p.splits = int(want < 1 ? 1 : want < p.chunks ? want : p.chunks);
     if (p.splits > kLpMaxSplit) p.splits = kLpMaxSplit;
     return p;
 }
 
-// a row is split only where there are fewer than two rows per SM
+// a row is split only where there are at most two rows per SM
 int logprobs_counters(int sms) { return 2 * sms; }
 
 size_t logprobs_workspace(const LogprobsCall& c, int sms) {
@@ -380,7 +462,7 @@ cudaError_t run_logprobs(const LogprobsCall& c, int sms, cudaStream_t s) {
     a.top_logprobs = c.top_logprobs, a.top_ids = c.top_ids, a.counters = c.counters;
     a.stats = reinterpret_cast<float4*>(c.ws);
     a.keys = reinterpret_cast<uint64_t*>(c.ws + size_t(c.rows) * p.splits * 16);
-    const size_t smem = c.top ? size_t(kLpCap + kLpMaxTop) * 8 : 0;
+    const size_t smem = c.top ? size_t(kLpCap + kLpMaxSplit) * 8 : 0;
     const unsigned grid = unsigned(c.rows * p.splits);
     const auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
