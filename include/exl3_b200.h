@@ -271,6 +271,9 @@ int exl3_ep_window_recv(int world, int64_t capacity, int64_t hidden, int topk, i
 enum { EXL3_KV_E4M3 = 0, EXL3_KV_INT8 = 1 };
 #define EXL3_KV_MAX_REQUESTS 16384
 
+/* The entries below take their arguments as one struct of 8-byte fields (a
+ * call of a few microseconds should not spend them on argument lists). */
+
 /* The step's bookkeeping from request lengths, in one launch: request b holds
  * lens[b] tokens and adds new_tokens[b].  Writes kv_lens[b] = lens[b] +
  * new_tokens[b]; cu_tokens [requests + 1], the requests' first token rows;
@@ -283,24 +286,50 @@ enum { EXL3_KV_E4M3 = 0, EXL3_KV_INT8 = 1 };
  * runs out, the tokens concerned get slot -1 (table entries -1) and status 7
  * is recorded; so it is for negative lengths (taken as 0) and for more new
  * tokens than n_tokens.  `status` may be NULL. */
-int exl3_kv_plan(const int32_t* lens, const int32_t* new_tokens, int requests, int32_t* block_table, int width,
-                 const int32_t* free_pages, int n_free, const int32_t* cursor, int page, int n_tokens,
-                 int32_t* kv_lens, int32_t* cu_tokens, int32_t* positions, int64_t* slots, int32_t* cursor_out,
-                 int* status, void* stream);
+typedef struct exl3_kv_plan_args {
+    const int32_t* lens;        /* [requests] */
+    const int32_t* new_tokens;  /* [requests] */
+    int64_t requests;           /* at most EXL3_KV_MAX_REQUESTS */
+    int32_t* block_table;       /* [requests][width] */
+    int64_t width;
+    const int32_t* free_pages;  /* [n_free] */
+    int64_t n_free;
+    const int32_t* cursor;      /* [1] */
+    int64_t page, n_tokens;
+    int32_t* kv_lens;           /* out [requests] */
+    int32_t* cu_tokens;         /* out [requests + 1] */
+    int32_t* positions;         /* out [n_tokens] */
+    int64_t* slots;             /* out [n_tokens] */
+    int32_t* cursor_out;        /* out [1] */
+    int* status;
+} exl3_kv_plan_args;
+int exl3_kv_plan(const exl3_kv_plan_args* args, void* stream);
 
 /* Writes new rows of K and V (fp16 or bf16 [tokens][kv_heads][dim], strides in
- * elements, rows at multiples of 8 bytes) to their slots as codes.  A page's
+ * elements, rows at multiples of 16 bytes) to their slots as codes.  A page's
  * tokens of one call follow one another in ascending order, as exl3_kv_plan
  * gives them.  A call that writes a page's first token sets its scale from
  * the new tokens alone; one that joins a part-filled page keeps the larger of
  * its scale and the new tokens', rounding the older codes again when it
- * grows.  NaN stays NaN in e4m3 and becomes 0 in int8, infinities become the
- * largest code.  Negative slots are skipped; slots past the cache are skipped
+ * grows.  Infinities become the largest code.  int8 has no NaN: they become 0.
+ * In e4m3 a NaN of K stays NaN; one of V becomes 0 and makes the token's whole
+ * key of that head NaN, so that the rows that see the token, and no others,
+ * come out NaN.  Negative slots are skipped; slots past the cache are skipped
  * with status 7. */
-int exl3_kv_append(const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v, int64_t v_tok_stride,
-                   int64_t v_head_stride, int x_dtype, const int64_t* slots, int64_t tokens, void* k_cache,
-                   void* v_cache, float* k_scale, float* v_scale, int code, int64_t pages, int kv_heads, int page,
-                   int dim, int* status, void* stream);
+typedef struct exl3_kv_append_args {
+    const void* k;
+    int64_t k_tok_stride, k_head_stride;
+    const void* v;
+    int64_t v_tok_stride, v_head_stride;
+    int64_t x_dtype;            /* of k and v */
+    const int64_t* slots;       /* [tokens] */
+    int64_t tokens;
+    void *k_cache, *v_cache;
+    float *k_scale, *v_scale;
+    int64_t code, pages, kv_heads, page, dim;
+    int* status;
+} exl3_kv_append_args;
+int exl3_kv_append(const exl3_kv_append_args* args, void* stream);
 
 /* out[r][h] = softmax_j(scale * q[r][h] . k_j) v_j over the cache.  Request
  * b's rows of q and out are [cu_tokens[b], cu_tokens[b + 1]) (cu_tokens NULL:
@@ -318,11 +347,27 @@ int exl3_kv_append(const void* k, int64_t k_tok_stride, int64_t k_head_stride, c
  * zero before its first use; it starts with the status word, and may serve
  * both, for calls that follow one another on a stream. */
 size_t exl3_kv_attend_workspace_size(int heads, int kv_heads, int dim, int max_new, int requests, int64_t q_rows);
-int exl3_kv_attend(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int x_dtype, int64_t q_rows, int heads,
-                   const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, int code,
-                   int64_t pages, int kv_heads, int page, int dim, const int32_t* block_table, int width, int requests,
-                   const int32_t* kv_lens, const int32_t* cu_tokens, int max_new, float scale, int64_t window,
-                   void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+typedef struct exl3_kv_attend_args {
+    const void* q;
+    int64_t q_tok_stride, q_head_stride;
+    int64_t x_dtype;            /* of q and out */
+    int64_t q_rows, heads;
+    const void *k_cache, *v_cache;
+    const float *k_scale, *v_scale;
+    int64_t code, pages, kv_heads, page, dim;
+    const int32_t* block_table; /* [requests][width] */
+    int64_t width, requests;
+    const int32_t* kv_lens;     /* [requests] */
+    const int32_t* cu_tokens;   /* [requests + 1] or NULL */
+    int64_t max_new;
+    double scale;
+    int64_t window;
+    void* out;
+    float* lse;                 /* or NULL */
+    void* workspace;
+    int64_t workspace_bytes;
+} exl3_kv_attend_args;
+int exl3_kv_attend(const exl3_kv_attend_args* args, void* stream);
 
 /* For each row of logits (fp32, fp16 or bf16 [rows][vocab], row stride in
  * elements): logprob = log softmax at tokens[row] (int32 or int64), the
@@ -334,9 +379,19 @@ int exl3_kv_attend(const void* q, int64_t q_tok_stride, int64_t q_head_stride, i
  * A row with NaN or +inf: NaN, as a softmax gives. */
 #define EXL3_LOGPROBS_MAX_TOP 32
 size_t exl3_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top, int x_dtype);
-int exl3_token_logprobs(const void* logits, int x_dtype, int64_t rows, int64_t row_stride, int64_t vocab,
-                        const void* tokens, int ids_dtype, int top, float* logprob, float* entropy, int32_t* rank,
-                        float* top_logprobs, int32_t* top_ids, void* workspace, size_t workspace_bytes, void* stream);
+typedef struct exl3_token_logprobs_args {
+    const void* logits;
+    int64_t x_dtype, rows, row_stride, vocab;
+    const void* tokens;         /* [rows] */
+    int64_t ids_dtype, top;
+    float *logprob, *entropy;   /* out [rows] */
+    int32_t* rank;              /* out [rows] */
+    float* top_logprobs;        /* out [rows][top] */
+    int32_t* top_ids;           /* out [rows][top] */
+    void* workspace;
+    int64_t workspace_bytes;
+} exl3_token_logprobs_args;
+int exl3_token_logprobs(const exl3_token_logprobs_args* args, void* stream);
 
 /* Phase timing for benchmarks (no reference counterpart; the reference times
  * its kernels with CUDA events in tools/bench_moe_decode.py:24-55).  While

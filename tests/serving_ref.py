@@ -47,8 +47,9 @@ def round_code(y, code):
     return np.where(np.isnan(y), np.nan, np.sign(y) * np.minimum(np.rint(mag / step) * step, 448.0))
 
 
-def append(x, slots, codes, scale, code):
-    """One of K and V: x [T, heads, dim], codes [pages, heads, page, dim] as numbers, scale [pages, heads]."""
+def append(x, slots, codes, scale, code, v=None):
+    """One of K and V: x [T, heads, dim], codes [pages, heads, page, dim] as numbers, scale [pages, heads].
+    For K in e4m3, `v` is V: a token's NaN there makes its whole key NaN; for V it is not given, and NaN becomes 0."""
     codes, scale = codes.astype(np.float64).copy(), scale.astype(np.float64).copy()
     P = codes.shape[2]
     t = 0
@@ -71,7 +72,12 @@ def append(x, slots, codes, scale, code):
                     codes[pg, h, :off] = round_code(codes[pg, h, :off] * 2.0 ** (was - e), code)
             scale[pg, h] = 2.0 ** e
             for i in range(n):
-                codes[pg, h, slots[t + i] % P] = round_code(rows[i] * 2.0 ** -e, code)
+                got = round_code(rows[i] * 2.0 ** -e, code)
+                if v is None:
+                    got = np.nan_to_num(got)
+                elif code == "e4m3" and np.isnan(v[t + i, h]).any():
+                    got = np.full_like(got, np.nan)
+                codes[pg, h, slots[t + i] % P] = got
         t += n
     return codes, scale
 

@@ -97,8 +97,8 @@ def _check_append(cuda, k, v, slots, dim, page, heads, code, pages=40):
     import torch
     kc, ks = _cache(cuda, pages, heads, page, dim, code, 1)
     vc, vs = _cache(cuda, pages, heads, page, dim, code, 2)
-    want = [ref.append(x.float().cpu().numpy(), slots, c.float().cpu().numpy(), s.cpu().numpy(), code)
-            for x, c, s in ((k, kc, ks), (v, vc, vs))]
+    want = [ref.append(x.float().cpu().numpy(), slots, c.float().cpu().numpy(), s.cpu().numpy(), code, other)
+            for x, c, s, other in ((k, kc, ks, v.float().cpu().numpy()), (v, vc, vs, None))]
     _kv().kv_append(k, v, torch.tensor(slots, device=cuda), kc, vc, ks, vs)
     for (wc, ws), c, s in zip(want, (kc, vc), (ks, vs)):
         assert np.array_equal(s.cpu().numpy(), ws)
@@ -149,6 +149,7 @@ def test_append_values(native, cuda, code):
     rows[11] = float("nan")
     slots = np.arange(12) * 16          # each the first of its page
     _check_append(cuda, rows, -rows, slots, 64, 16, 2, code)
+    _check_append(cuda, rows, rows.flip(0), slots, 64, 16, 2, code)  # K and V have their NaN in other tokens
     _check_append(cuda, rows, -rows, slots + 5, 64, 16, 2, code)  # each joins a page
     _check_append(cuda, rows, -rows, np.arange(12) + 32, 64, 16, 2, code)  # all of one page
 
@@ -323,6 +324,25 @@ def test_attend_ignores_what_it_may_not_see(native, cuda):
         p["table"][0, 2:] = 1 << 30
         again, _ = _attend(cuda, p)
         assert torch.equal(clean, again)
+
+
+def test_attend_nan_stays_with_its_token(native, cuda):
+    """A NaN in a token's K or V reaches the rows that see the token and no others (e4m3; int8 has none)."""
+    import torch
+    for new, dim in ((40, 64), (3, 128), (200, 128)):
+        cache = _kv().Exl3KvCache(1, 20, 2, dim, requests=1, max_len=320, page_size=16, device=cuda)
+        k, v, q = (torch.randn(new, n, dim, device=cuda).bfloat16() for n in (2, 2, 6))
+        bad = new // 2
+        plan = cache.plan(torch.tensor([new], dtype=torch.int32, device=cuda), new)
+        cache.append(0, k, v, plan)
+        clean = cache.attend(0, q, plan, new)
+        k[bad, 0, 5] = float("nan")
+        v[bad, 1, 7] = float("nan")
+        cache.append(0, k, v, plan)
+        out = cache.attend(0, q, plan, new)
+        assert torch.equal(out[:bad], clean[:bad]) and bool(out[bad:].isnan().all())
+        windowed = cache.attend(0, q, plan, new, window=2)
+        assert not windowed[bad + 2:].isnan().any() and bool(windowed[bad:bad + 2].isnan().all())
 
 
 def test_attend_bad_page(native, cuda):

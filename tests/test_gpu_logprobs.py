@@ -140,7 +140,7 @@ def test_refusals(native, cuda):
     x, t = torch.zeros(2, 50, device=cuda), torch.zeros(2, dtype=torch.int64, device=cuda)
     for args, kw, exc, match in (
             ((x.cpu(), t), {}, RuntimeError, "CUDA"), ((x[0], t), {}, ValueError, "rows, vocab"),
-            ((x.int(), t), {}, ValueError, "fp32"), ((x.double(), t), {}, RuntimeError, "dtype"),
+            ((x.int(), t), {}, ValueError, "fp32"), ((x.double(), t), {}, ValueError, "fp32"),
             ((x, t[:1]), {}, ValueError, "tokens"), ((x, t.float()), {}, ValueError, "tokens"),
             ((x, t), {"top": 33}, ValueError, "top"), ((x, t), {"top": -1}, ValueError, "top"),
             ((x[:, :3], t), {"top": 4}, ValueError, "top")):

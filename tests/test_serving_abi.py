@@ -11,13 +11,18 @@ def _lib():
     return _native.load(), _native.last_error
 
 
+def _pack(name, a):
+    from exl3_b200 import _native
+    return getattr(_native, name)(*[0 if v is None else v for k, v in a.items() if k != "stream"])
+
+
 def _attend(**kw):
     a = dict(q=A, qt=512, qh=128, xd=2, rows=1, heads=4, k=A, v=A, ks=A, vs=A, code=0, pages=8, hk=2, page=16, dim=128,
              table=A, width=4, req=1, lens=A, cu=None, max_new=1, scale=1.0, window=0, out=A, lse=None, ws=A,
              wsb=1 << 30, stream=None)
     a.update(kw)
     lib, err = _lib()
-    return lib.exl3_kv_attend(*a.values()), err()
+    return lib.exl3_kv_attend(_pack("PACK_KV_ATTEND", a), a["stream"]), err()
 
 
 @pytest.mark.parametrize("kw,match", [
@@ -44,14 +49,14 @@ def test_attend_workspace_refused():
 
 
 @pytest.mark.parametrize("kw,match", [
-    (dict(k=None), "null"), (dict(xd=0), "fp16 or bf16"), (dict(kt=130), "8 bytes"), (dict(v=A + 4), "8 bytes"),
+    (dict(k=None), "null"), (dict(xd=0), "fp16 or bf16"), (dict(kt=132), "16 bytes"), (dict(v=A + 8), "16 bytes"),
     (dict(tokens=-1), "tokens"), (dict(slots=None), "null"), (dict(page=8), "page"), (dict(kc=None), "null")])
 def test_append_refuses(kw, match):
     a = dict(k=A, kt=512, kh=128, v=A, vt=512, vh=128, xd=1, slots=A, tokens=4, kc=A, vc=A, ks=A, vs=A, code=0, pages=8,
              hk=2, page=16, dim=128, status=None, stream=None)
     a.update(kw)
     lib, err = _lib()
-    assert lib.exl3_kv_append(*a.values()) == ARG and match in err()
+    assert lib.exl3_kv_append(_pack("PACK_KV_APPEND", a), None) == ARG and match in err()
 
 
 @pytest.mark.parametrize("kw,match", [
@@ -62,7 +67,7 @@ def test_plan_refuses(kw, match):
              cur=A, status=None, stream=None)
     a.update(kw)
     lib, err = _lib()
-    assert lib.exl3_kv_plan(*a.values()) == ARG and match in err()
+    assert lib.exl3_kv_plan(_pack("PACK_KV_PLAN", a), None) == ARG and match in err()
 
 
 @pytest.mark.parametrize("kw,rc,match", [
@@ -75,7 +80,33 @@ def test_logprobs_refuses(kw, rc, match):
              wsb=1 << 30, stream=None)
     a.update(kw)
     lib, err = _lib()
-    assert lib.exl3_token_logprobs(*a.values()) == rc and (rc == OK or match in err())
+    assert lib.exl3_token_logprobs(_pack("PACK_TOKEN_LOGPROBS", a), None) == rc and (rc == OK or match in err())
+
+
+def test_packed_structs_match_the_header():
+    """Every struct of the header has one 8-byte field per packed value, the double where it is packed."""
+    import os
+    import re
+    from conftest import ROOT
+    from exl3_b200 import _native
+    with open(os.path.join(ROOT, "include", "exl3_b200.h")) as f:
+        text = re.sub(r"/\*.*?\*/", "", f.read(), flags=re.S)
+    found = re.findall(r"typedef struct \w+ \{(.*?)\} exl3_(\w+)_args;", text, flags=re.S)
+    assert {n for _, n in found} == {"kv_plan", "kv_append", "kv_attend", "token_logprobs"}
+    for body, name in found:
+        kinds = []
+        for decl in filter(None, (d.strip() for d in body.split(";"))):
+            assert re.match(r"(const )?(void|int|float|int32_t|int64_t|double)\b", decl)
+            for field in decl.split(","):
+                assert "*" in field or "int64_t" in decl or "double" in decl, decl
+                kinds.append("d" if "double" in decl else "q")
+        pack = getattr(_native, "PACK_" + name.upper())
+        fmt = pack.__self__.format
+        want = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([qd])", fmt))
+        assert "".join(kinds) == want, name
+    lib, err = _lib()
+    for name in ("kv_plan", "kv_append", "kv_attend", "token_logprobs"):
+        assert getattr(lib, "exl3_" + name)(None, None) == ARG and "null" in err()
 
 
 def test_cpu_tensors_fail_loudly():

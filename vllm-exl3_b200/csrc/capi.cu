@@ -597,14 +597,14 @@ int exl3_ngram_lookup(const void* table, int64_t n_rows, int bits, const void* i
 
 // --- the paged 8-bit key/value cache ---
 
-static int check_cache(const char* who, const void* k, const void* v, const float* ks, const float* vs, int code,
-                       int64_t pages, int kv_heads, int page, int dim) {
+static int check_cache(const char* who, const void* k, const void* v, const float* ks, const float* vs, int64_t code,
+                       int64_t pages, int64_t kv_heads, int64_t page, int64_t dim) {
     if (!k || !v || !ks || !vs) return fail(EXL3_ERR_ARG, "%s: null cache or scale pointer", who);
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(EXL3_ERR_ARG, "%s: the caches must be 16-byte aligned", who);
     if (code != EXL3_KV_E4M3 && code != EXL3_KV_INT8) return fail(EXL3_ERR_ARG, "%s: code must be 0 (e4m3) or 1 (int8)", who);
     if (page != 16 && page != 32 && page != 64 && page != 128)
-        return fail(EXL3_ERR_ARG, "%s: page must be 16, 32, 64 or 128 tokens (got %d)", who, page);
-    if (dim != 64 && dim != 128) return fail(EXL3_ERR_ARG, "%s: head dim must be 64 or 128 (got %d)", who, dim);
+        return fail(EXL3_ERR_ARG, "%s: page must be 16, 32, 64 or 128 tokens (got %lld)", who, (long long)page);
+    if (dim != 64 && dim != 128) return fail(EXL3_ERR_ARG, "%s: head dim must be 64 or 128 (got %lld)", who, (long long)dim);
     if (kv_heads < 1 || kv_heads > 65535) return fail(EXL3_ERR_ARG, "%s: kv_heads must be in 1..65535", who);
     if (pages < 1 || pages > INT32_MAX) return fail(EXL3_ERR_ARG, "%s: pages must be in 1..2^31-1", who);
     return EXL3_OK;
@@ -614,47 +614,49 @@ static int check_cache(const char* who, const void* k, const void* v, const floa
 static constexpr size_t kServeCounters = 256;
 static size_t serve_partials(int n_counters) { return (kServeCounters + size_t(n_counters) * 4 + 255) & ~size_t(255); }
 
-int exl3_kv_plan(const int32_t* lens, const int32_t* new_tokens, int requests, int32_t* block_table, int width,
-                 const int32_t* free_pages, int n_free, const int32_t* cursor, int page, int n_tokens,
-                 int32_t* kv_lens, int32_t* cu_tokens, int32_t* positions, int64_t* slots, int32_t* cursor_out,
-                 int* status, void* stream) {
+int exl3_kv_plan(const exl3_kv_plan_args* a, void* stream) {
     const char* who = "exl3_kv_plan";
-    if (requests < 0 || requests > EXL3_KV_MAX_REQUESTS)
-        return fail(EXL3_ERR_ARG, "%s: requests must be in 0..%d (got %d)", who, EXL3_KV_MAX_REQUESTS, requests);
-    if (width < 0 || n_free < 0 || n_tokens < 0) return fail(EXL3_ERR_ARG, "%s: sizes must be >= 0", who);
-    if (page != 16 && page != 32 && page != 64 && page != 128)
-        return fail(EXL3_ERR_ARG, "%s: page must be 16, 32, 64 or 128 tokens (got %d)", who, page);
-    if (!cursor || !cu_tokens || !cursor_out || (requests && (!lens || !new_tokens || !kv_lens)) ||
-        (requests && width && !block_table) || (n_free && !free_pages) || (n_tokens && (!positions || !slots)))
+    if (!a) return fail(EXL3_ERR_ARG, "%s: null arguments", who);
+    if (a->requests < 0 || a->requests > EXL3_KV_MAX_REQUESTS)
+        return fail(EXL3_ERR_ARG, "%s: requests must be in 0..%d (got %lld)", who, EXL3_KV_MAX_REQUESTS, (long long)a->requests);
+    if (a->width < 0 || a->n_free < 0 || a->n_tokens < 0 || a->width > INT32_MAX || a->n_free > INT32_MAX ||
+        a->n_tokens > INT32_MAX)
+        return fail(EXL3_ERR_ARG, "%s: sizes must be in 0..2^31-1", who);
+    if (a->page != 16 && a->page != 32 && a->page != 64 && a->page != 128)
+        return fail(EXL3_ERR_ARG, "%s: page must be 16, 32, 64 or 128 tokens (got %lld)", who, (long long)a->page);
+    if (!a->cursor || !a->cu_tokens || !a->cursor_out || (a->requests && (!a->lens || !a->new_tokens || !a->kv_lens)) ||
+        (a->requests && a->width && !a->block_table) || (a->n_free && !a->free_pages) ||
+        (a->n_tokens && (!a->positions || !a->slots)))
         return fail(EXL3_ERR_ARG, "%s: null pointer", who);
     exl3::KvPlanCall c;
-    c.lens = lens, c.fresh = new_tokens, c.requests = requests, c.table = block_table, c.width = width;
-    c.free_pages = free_pages, c.n_free = n_free, c.cursor = cursor, c.page = page, c.n_tokens = n_tokens;
-    c.kv_lens = kv_lens, c.cu = cu_tokens, c.positions = positions, c.slots = slots, c.cursor_out = cursor_out;
-    c.status = status;
+    c.lens = a->lens, c.fresh = a->new_tokens, c.requests = int(a->requests), c.table = a->block_table;
+    c.width = int(a->width), c.free_pages = a->free_pages, c.n_free = int(a->n_free), c.cursor = a->cursor;
+    c.page = int(a->page), c.n_tokens = int(a->n_tokens), c.kv_lens = a->kv_lens, c.cu = a->cu_tokens;
+    c.positions = a->positions, c.slots = a->slots, c.cursor_out = a->cursor_out, c.status = a->status;
     const cudaError_t e = exl3::run_kv_plan(c, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? EXL3_OK : cuda_fail(e, who);
 }
 
-int exl3_kv_append(const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v, int64_t v_tok_stride,
-                   int64_t v_head_stride, int x_dtype, const int64_t* slots, int64_t tokens, void* k_cache,
-                   void* v_cache, float* k_scale, float* v_scale, int code, int64_t pages, int kv_heads, int page,
-                   int dim, int* status, void* stream) {
+int exl3_kv_append(const exl3_kv_append_args* a, void* stream) {
     const char* who = "exl3_kv_append";
-    if (int rc = check_cache(who, k_cache, v_cache, k_scale, v_scale, code, pages, kv_heads, page, dim)) return rc;
-    if (x_dtype != EXL3_DT_F16 && x_dtype != EXL3_DT_BF16) return fail(EXL3_ERR_ARG, "%s: k and v must be fp16 or bf16", who);
-    if (tokens < 0 || tokens > INT32_MAX) return fail(EXL3_ERR_ARG, "%s: tokens must be in 0..2^31-1", who);
-    if (tokens == 0) return EXL3_OK;
-    if (!k || !v || !slots) return fail(EXL3_ERR_ARG, "%s: null pointer", who);
-    if (!aligned(k, 8) || !aligned(v, 8) || ((k_tok_stride | k_head_stride | v_tok_stride | v_head_stride) & 3))
-        return fail(EXL3_ERR_ARG, "%s: rows of k and v must start at multiples of 8 bytes", who);
+    if (!a) return fail(EXL3_ERR_ARG, "%s: null arguments", who);
+    if (int rc = check_cache(who, a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->code, a->pages, a->kv_heads, a->page, a->dim))
+        return rc;
+    if (a->x_dtype != EXL3_DT_F16 && a->x_dtype != EXL3_DT_BF16)
+        return fail(EXL3_ERR_ARG, "%s: k and v must be fp16 or bf16", who);
+    if (a->tokens < 0 || a->tokens > INT32_MAX) return fail(EXL3_ERR_ARG, "%s: tokens must be in 0..2^31-1", who);
+    if (a->tokens == 0) return EXL3_OK;
+    if (!a->k || !a->v || !a->slots) return fail(EXL3_ERR_ARG, "%s: null pointer", who);
+    if (!aligned(a->k, 16) || !aligned(a->v, 16) ||
+        ((a->k_tok_stride | a->k_head_stride | a->v_tok_stride | a->v_head_stride) & 7))
+        return fail(EXL3_ERR_ARG, "%s: rows of k and v must start at multiples of 16 bytes", who);
     exl3::KvAppendCall c;
-    c.x[0] = k, c.x[1] = v, c.tok_stride[0] = k_tok_stride, c.tok_stride[1] = v_tok_stride;
-    c.head_stride[0] = k_head_stride, c.head_stride[1] = v_head_stride, c.x_dtype = x_dtype;
-    c.slots = slots, c.tokens = tokens, c.cache[0] = k_cache, c.cache[1] = v_cache;
-    c.scale[0] = k_scale, c.scale[1] = v_scale, c.pages = pages, c.heads = kv_heads, c.page = page, c.dim = dim;
-    c.e4m3 = code == EXL3_KV_E4M3, c.status = status;
-    const cudaError_t e = exl3::run_kv_append(c, static_cast<cudaStream_t>(stream));
+    c.x[0] = a->k, c.x[1] = a->v, c.tok_stride[0] = a->k_tok_stride, c.tok_stride[1] = a->v_tok_stride;
+    c.head_stride[0] = a->k_head_stride, c.head_stride[1] = a->v_head_stride, c.x_dtype = int(a->x_dtype);
+    c.slots = a->slots, c.tokens = a->tokens, c.cache[0] = a->k_cache, c.cache[1] = a->v_cache;
+    c.scale[0] = a->k_scale, c.scale[1] = a->v_scale, c.pages = a->pages, c.heads = int(a->kv_heads);
+    c.page = int(a->page), c.dim = int(a->dim), c.e4m3 = a->code == EXL3_KV_E4M3, c.status = a->status;
+    const cudaError_t e = exl3::run_kv_append(c, exl3::num_sms_cached(), static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? EXL3_OK : cuda_fail(e, who);
 }
 
@@ -664,48 +666,48 @@ size_t exl3_kv_attend_workspace_size(int heads, int kv_heads, int dim, int max_n
         return 0;
     exl3::KvAttendCall c;
     c.heads = heads, c.kv_heads = kv_heads, c.dim = dim, c.max_new = max_new, c.requests = requests, c.q_rows = q_rows;
-    const int sms = exl3::num_sms_current();
+    const int sms = exl3::num_sms_cached();
     return serve_partials(exl3::kv_attend_counters(sms)) + exl3::kv_attend_workspace(c, sms);
 }
 
-int exl3_kv_attend(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int x_dtype, int64_t q_rows, int heads,
-                   const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, int code,
-                   int64_t pages, int kv_heads, int page, int dim, const int32_t* block_table, int width, int requests,
-                   const int32_t* kv_lens, const int32_t* cu_tokens, int max_new, float scale, int64_t window,
-                   void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+int exl3_kv_attend(const exl3_kv_attend_args* a, void* stream) {
     const char* who = "exl3_kv_attend";
-    if (int rc = check_cache(who, k_cache, v_cache, k_scale, v_scale, code, pages, kv_heads, page, dim)) return rc;
-    if (x_dtype != EXL3_DT_F16 && x_dtype != EXL3_DT_BF16) return fail(EXL3_ERR_ARG, "%s: q must be fp16 or bf16", who);
-    if (heads < 1 || heads % kv_heads) return fail(EXL3_ERR_ARG, "%s: heads (%d) must be a multiple of kv_heads (%d)", who, heads, kv_heads);
-    if (heads > 65535) return fail(EXL3_ERR_ARG, "%s: heads must be at most 65535", who);
-    if (q_rows < 0 || q_rows > INT32_MAX / heads) return fail(EXL3_ERR_ARG, "%s: q rows x heads must be in 0..2^31-1", who);
-    if (requests < 0 || width < 0) return fail(EXL3_ERR_ARG, "%s: requests and table width must be >= 0", who);
-    if (int64_t(width) * page > INT32_MAX) return fail(EXL3_ERR_ARG, "%s: the table holds more than 2^31-1 tokens", who);
-    if (max_new < 1) return fail(EXL3_ERR_ARG, "%s: max_new must be >= 1", who);
-    if (!cu_tokens && (max_new != 1 || q_rows != requests))
+    if (!a) return fail(EXL3_ERR_ARG, "%s: null arguments", who);
+    if (int rc = check_cache(who, a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->code, a->pages, a->kv_heads, a->page, a->dim))
+        return rc;
+    if (a->x_dtype != EXL3_DT_F16 && a->x_dtype != EXL3_DT_BF16) return fail(EXL3_ERR_ARG, "%s: q must be fp16 or bf16", who);
+    if (a->heads < 1 || a->heads % a->kv_heads)
+        return fail(EXL3_ERR_ARG, "%s: heads (%lld) must be a multiple of kv_heads (%lld)", who, (long long)a->heads, (long long)a->kv_heads);
+    if (a->heads > 65535) return fail(EXL3_ERR_ARG, "%s: heads must be at most 65535", who);
+    if (a->q_rows < 0 || a->q_rows > INT32_MAX / a->heads) return fail(EXL3_ERR_ARG, "%s: q rows x heads must be in 0..2^31-1", who);
+    if (a->requests < 0 || a->requests > INT32_MAX || a->width < 0)
+        return fail(EXL3_ERR_ARG, "%s: requests and table width must be >= 0", who);
+    if (a->width > INT32_MAX / a->page) return fail(EXL3_ERR_ARG, "%s: the table holds more than 2^31-1 tokens", who);
+    if (a->max_new < 1 || a->max_new > INT32_MAX) return fail(EXL3_ERR_ARG, "%s: max_new must be >= 1", who);
+    if (!a->cu_tokens && (a->max_new != 1 || a->q_rows != a->requests))
         return fail(EXL3_ERR_ARG, "%s: without cu_tokens every request has one row of q", who);
-    if (window < 0) return fail(EXL3_ERR_ARG, "%s: window must be >= 0 (0: none)", who);
-    if (!(std::fabs(scale) <= 3.0e38f)) return fail(EXL3_ERR_ARG, "%s: scale must be finite", who);
-    if (q_rows == 0) return EXL3_OK;
-    if (!q || !out || (requests && (!kv_lens || (width && !block_table)))) return fail(EXL3_ERR_ARG, "%s: null pointer", who);
-    if (!aligned(q, 16) || ((q_tok_stride | q_head_stride) & 7))
+    if (a->window < 0) return fail(EXL3_ERR_ARG, "%s: window must be >= 0 (0: none)", who);
+    if (!(std::fabs(a->scale) <= 3.0e37)) return fail(EXL3_ERR_ARG, "%s: scale must be finite", who);
+    if (a->q_rows == 0) return EXL3_OK;
+    if (!a->q || !a->out || (a->requests && (!a->kv_lens || (a->width && !a->block_table))))
+        return fail(EXL3_ERR_ARG, "%s: null pointer", who);
+    if (!aligned(a->q, 16) || ((a->q_tok_stride | a->q_head_stride) & 7))
         return fail(EXL3_ERR_ARG, "%s: rows of q must start at multiples of 16 bytes", who);
-    if (!aligned(out, 16)) return fail(EXL3_ERR_ARG, "%s: out must be 16-byte aligned", who);
-    const size_t need = exl3_kv_attend_workspace_size(heads, kv_heads, dim, max_new, requests, q_rows);
-    if (!workspace || workspace_bytes < need)
-        return fail(EXL3_ERR_WORKSPACE, "%s: workspace of %zu bytes required (got %zu)", who, need, workspace_bytes);
-    if (!aligned(workspace, 256)) return fail(EXL3_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
-    const int sms = exl3::num_sms_current();
+    if (!aligned(a->out, 16)) return fail(EXL3_ERR_ARG, "%s: out must be 16-byte aligned", who);
     exl3::KvAttendCall c;
-    c.q = q, c.q_tok = q_tok_stride, c.q_head = q_head_stride, c.x_dtype = x_dtype, c.q_rows = q_rows;
-    c.heads = heads, c.kv_heads = kv_heads, c.dim = dim, c.k = k_cache, c.v = v_cache;
-    c.k_scale = k_scale, c.v_scale = v_scale, c.pages = pages, c.page = page, c.e4m3 = code == EXL3_KV_E4M3;
-    c.table = block_table, c.width = width, c.requests = requests, c.kv_lens = kv_lens, c.cu = cu_tokens;
-    c.max_new = max_new, c.scale = scale, c.window = window > INT32_MAX / 2 ? 0 : int(window);
-    c.out = out, c.lse = lse, c.status = static_cast<int*>(workspace);
-    char* ws = static_cast<char*>(workspace);
-    c.counters = reinterpret_cast<int32_t*>(ws + kServeCounters);
-    c.ws = ws + serve_partials(exl3::kv_attend_counters(sms));
+    c.q = a->q, c.q_tok = a->q_tok_stride, c.q_head = a->q_head_stride, c.x_dtype = int(a->x_dtype), c.q_rows = a->q_rows;
+    c.heads = int(a->heads), c.kv_heads = int(a->kv_heads), c.dim = int(a->dim), c.k = a->k_cache, c.v = a->v_cache;
+    c.k_scale = a->k_scale, c.v_scale = a->v_scale, c.pages = a->pages, c.page = int(a->page);
+    c.e4m3 = a->code == EXL3_KV_E4M3, c.table = a->block_table, c.width = int(a->width), c.requests = int(a->requests);
+    c.kv_lens = a->kv_lens, c.cu = a->cu_tokens, c.max_new = int(a->max_new), c.scale = float(a->scale);
+    c.window = a->window > INT32_MAX / 2 ? 0 : int(a->window), c.out = a->out, c.lse = a->lse;
+    const int sms = exl3::num_sms_cached();
+    const size_t partials = serve_partials(exl3::kv_attend_counters(sms)), need = partials + exl3::kv_attend_workspace(c, sms);
+    if (!a->workspace || a->workspace_bytes < 0 || size_t(a->workspace_bytes) < need)
+        return fail(EXL3_ERR_WORKSPACE, "%s: workspace of %zu bytes required (got %lld)", who, need, (long long)a->workspace_bytes);
+    if (!aligned(a->workspace, 256)) return fail(EXL3_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
+    char* ws = static_cast<char*>(a->workspace);
+    c.status = reinterpret_cast<int*>(ws), c.counters = reinterpret_cast<int32_t*>(ws + kServeCounters), c.ws = ws + partials;
     const cudaError_t e = exl3::run_kv_attend(c, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? EXL3_OK : cuda_fail(e, who);
 }
@@ -714,37 +716,36 @@ size_t exl3_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top, 
     if (rows < 0 || vocab < 1 || vocab > INT32_MAX || top < 0 || top > EXL3_LOGPROBS_MAX_TOP || !float_dtype(x_dtype)) return 0;
     exl3::LogprobsCall c;
     c.rows = rows, c.vocab = int(vocab), c.top = top, c.x_dtype = x_dtype;
-    const int sms = exl3::num_sms_current();
+    const int sms = exl3::num_sms_cached();
     return serve_partials(exl3::logprobs_counters(sms)) + (rows ? exl3::logprobs_workspace(c, sms) : 0);
 }
 
-int exl3_token_logprobs(const void* logits, int x_dtype, int64_t rows, int64_t row_stride, int64_t vocab,
-                        const void* tokens, int ids_dtype, int top, float* logprob, float* entropy, int32_t* rank,
-                        float* top_logprobs, int32_t* top_ids, void* workspace, size_t workspace_bytes, void* stream) {
+int exl3_token_logprobs(const exl3_token_logprobs_args* a, void* stream) {
     const char* who = "exl3_token_logprobs";
-    if (!float_dtype(x_dtype)) return fail(EXL3_ERR_ARG, "%s: logits must be fp32, fp16 or bf16", who);
-    if (ids_dtype != EXL3_DT_I32 && ids_dtype != EXL3_DT_I64) return fail(EXL3_ERR_ARG, "%s: tokens must be int32 or int64", who);
-    if (vocab < 1 || vocab > INT32_MAX - 65536) return fail(EXL3_ERR_ARG, "%s: vocab out of range", who);
-    if (top < 0 || top > EXL3_LOGPROBS_MAX_TOP || top > vocab)
-        return fail(EXL3_ERR_ARG, "%s: top must be in 0..min(%d, vocab) (got %d)", who, EXL3_LOGPROBS_MAX_TOP, top);
-    if (rows < 0 || rows > INT32_MAX / 2) return fail(EXL3_ERR_ARG, "%s: rows must be in 0..2^30", who);
-    if (rows == 0) return EXL3_OK;
-    if (row_stride < vocab && rows > 1) return fail(EXL3_ERR_ARG, "%s: rows of logits overlap", who);
-    if (!logits || !tokens || !logprob || !entropy || !rank || (top && (!top_logprobs || !top_ids)))
+    if (!a) return fail(EXL3_ERR_ARG, "%s: null arguments", who);
+    if (!float_dtype(int(a->x_dtype))) return fail(EXL3_ERR_ARG, "%s: logits must be fp32, fp16 or bf16", who);
+    if (a->ids_dtype != EXL3_DT_I32 && a->ids_dtype != EXL3_DT_I64)
+        return fail(EXL3_ERR_ARG, "%s: tokens must be int32 or int64", who);
+    if (a->vocab < 1 || a->vocab > INT32_MAX - 65536) return fail(EXL3_ERR_ARG, "%s: vocab out of range", who);
+    if (a->top < 0 || a->top > EXL3_LOGPROBS_MAX_TOP || a->top > a->vocab)
+        return fail(EXL3_ERR_ARG, "%s: top must be in 0..min(%d, vocab) (got %lld)", who, EXL3_LOGPROBS_MAX_TOP, (long long)a->top);
+    if (a->rows < 0 || a->rows > INT32_MAX / 4) return fail(EXL3_ERR_ARG, "%s: rows must be in 0..2^29", who);
+    if (a->rows == 0) return EXL3_OK;
+    if (a->row_stride < a->vocab && a->rows > 1) return fail(EXL3_ERR_ARG, "%s: rows of logits overlap", who);
+    if (!a->logits || !a->tokens || !a->logprob || !a->entropy || !a->rank || (a->top && (!a->top_logprobs || !a->top_ids)))
         return fail(EXL3_ERR_ARG, "%s: null pointer", who);
-    if (!aligned(logits, x_dtype == EXL3_DT_F32 ? 4 : 2)) return fail(EXL3_ERR_ARG, "%s: misaligned logits", who);
-    const size_t need = exl3_token_logprobs_workspace_size(rows, vocab, top, x_dtype);
-    if (!workspace || workspace_bytes < need)
-        return fail(EXL3_ERR_WORKSPACE, "%s: workspace of %zu bytes required (got %zu)", who, need, workspace_bytes);
-    if (!aligned(workspace, 256)) return fail(EXL3_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
-    const int sms = exl3::num_sms_current();
+    if (!aligned(a->logits, a->x_dtype == EXL3_DT_F32 ? 4 : 2)) return fail(EXL3_ERR_ARG, "%s: misaligned logits", who);
     exl3::LogprobsCall c;
-    c.logits = logits, c.x_dtype = x_dtype, c.rows = rows, c.stride = row_stride, c.vocab = int(vocab);
-    c.tokens = tokens, c.ids_dtype = ids_dtype, c.top = top, c.logprob = logprob, c.entropy = entropy, c.rank = rank;
-    c.top_logprobs = top_logprobs, c.top_ids = top_ids;
-    char* ws = static_cast<char*>(workspace);
-    c.counters = reinterpret_cast<int32_t*>(ws + kServeCounters);
-    c.ws = ws + serve_partials(exl3::logprobs_counters(sms));
+    c.logits = a->logits, c.x_dtype = int(a->x_dtype), c.rows = a->rows, c.stride = a->row_stride, c.vocab = int(a->vocab);
+    c.tokens = a->tokens, c.ids_dtype = int(a->ids_dtype), c.top = int(a->top), c.logprob = a->logprob;
+    c.entropy = a->entropy, c.rank = a->rank, c.top_logprobs = a->top_logprobs, c.top_ids = a->top_ids;
+    const int sms = exl3::num_sms_cached();
+    const size_t partials = serve_partials(exl3::logprobs_counters(sms)), need = partials + exl3::logprobs_workspace(c, sms);
+    if (!a->workspace || a->workspace_bytes < 0 || size_t(a->workspace_bytes) < need)
+        return fail(EXL3_ERR_WORKSPACE, "%s: workspace of %zu bytes required (got %lld)", who, need, (long long)a->workspace_bytes);
+    if (!aligned(a->workspace, 256)) return fail(EXL3_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
+    char* ws = static_cast<char*>(a->workspace);
+    c.counters = reinterpret_cast<int32_t*>(ws + kServeCounters), c.ws = ws + partials;
     const cudaError_t e = exl3::run_logprobs(c, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? EXL3_OK : cuda_fail(e, who);
 }

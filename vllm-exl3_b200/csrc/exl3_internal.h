@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace exl3 {
 
 constexpr int kRowsPerSlot = 16;  // token rows one expert work slot carries (two m16n8 mma columns)
@@ -227,7 +229,7 @@ struct KvAppendCall {
     bool e4m3 = true;
     int* status = nullptr;
 };
-cudaError_t run_kv_append(const KvAppendCall& c, cudaStream_t s);
+cudaError_t run_kv_append(const KvAppendCall& c, int sms, cudaStream_t s);
 
 struct KvAttendCall {
     const void* q = nullptr;  // [q_rows][heads][dim], strides in elements
@@ -278,6 +280,22 @@ int logprobs_counters(int sms);
 cudaError_t run_logprobs(const LogprobsCall& c, int sms, cudaStream_t s);
 
 int num_sms_current();
+// num_sms_current() looked up once per device
+int num_sms_cached();
+
+// Raises a kernel's dynamic shared memory limit, once per device: `done` is a
+// bit per device (devices from 64 on are set at every call).
+template <class Kernel>
+cudaError_t raise_smem(Kernel* kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
 // stages and dynamic smem of the GEMM for mt 128-row halves per tile; false
 // if two stages do not fit at two CTAs per SM
 bool tc_pick_stages(int kmax, int mt, int& stages, size_t& smem);

@@ -447,7 +447,8 @@ static cudaError_t launch_attend(const KvAttendArgs& a, int sms, cudaStream_t s)
     constexpr int NC = 8 * NT;
     const size_t smem = size_t(kAttWarps * NC * (D + 2) + 2 * NC) * 4;
     auto* kernel = kv_attend_kernel<E4M3, BF16, D, NT>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = raise_smem(kernel, smem, done);
     if (e != cudaSuccess) return e;
     kernel<<<sms * kAttCtasPerSm, kAttThreads, smem, s>>>(a);
     return cudaGetLastError();

@@ -11,20 +11,25 @@
 // memory.  New pages are read from the free list, not from the table, so the
 // table's writers and readers need no order.
 //
-// kv_append: one CTA per (window of P tokens, kv head, K or V); it owns the
-// runs (consecutive tokens of one page) that START in its window, so every
-// tile has one writer and its scale can be settled in shared memory: rows are
-// read once from HBM for the run's largest magnitude and once more, from L1,
-// to be coded.
+// kv_append: a run is the consecutive tokens of one page.  A CTA takes the
+// runs that START in its window of tokens, for one kv head, K and V: every tile
+// has one writer, and its scale is settled without a second pass over memory.
+// Rows are read once, 16 bytes a lane, and stay in registers between the
+// maximum and the coding: runs of up to 8 iterations of one warp are a warp's
+// alone (no barrier), longer ones the CTA's.  Bound: HBM, 2 bytes read and 1
+// written per value.
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "kv_common.cuh"
 
 namespace exl3 {
 
 constexpr int kPlanThreads = 512;
+constexpr int kKvMaxRequests = 16384;  // EXL3_KV_MAX_REQUESTS: their sums fit shared memory
 
 struct KvPlanArgs {
     const int32_t *lens, *fresh;  // [B]
@@ -131,6 +136,15 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const KvPlanArgs 
     if (bad) set_status(a.status, DEV_BAD_INDEX);
 }
 
+int num_sms_cached() {
+    static std::atomic<int> sms[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return num_sms_current();
+    int n = sms[dev].load(std::memory_order_relaxed);
+    if (n == 0) sms[dev].store(n = num_sms_current(), std::memory_order_relaxed);
+    return n;
+}
+
 cudaError_t run_kv_plan(const KvPlanCall& c, cudaStream_t s) {
     KvPlanArgs a;
     a.lens = c.lens, a.fresh = c.fresh, a.B = c.requests;
@@ -143,7 +157,8 @@ cudaError_t run_kv_plan(const KvPlanCall& c, cudaStream_t s) {
     int grid = (work + 2 * kPlanThreads - 1) / (2 * kPlanThreads);
     grid = grid < 1 ? 1 : grid > 148 ? 148 : grid;
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        static std::atomic<uint64_t> done{0};
+        const cudaError_t e = raise_smem(kv_plan_kernel, size_t(kKvMaxRequests + 1) * 8, done);
         if (e != cudaSuccess) return e;
     }
     kv_plan_kernel<<<grid, kPlanThreads, smem, s>>>(a);
@@ -152,18 +167,19 @@ cudaError_t run_kv_plan(const KvPlanCall& c, cudaStream_t s) {
 
 // ---------------------------------------------------------------------------
 
-constexpr int kAppendThreads = 256;
 constexpr int kMaxPage = 128;
+constexpr int kAppendHold = 8;  // 16-byte loads of a lane between maximum and coding
 
 struct KvAppendArgs {
-    const void* x[2];       // K and V rows [T][heads][dim] with strides
+    const uint16_t* x[2];   // K and V rows [T][heads][dim] with strides
     int64_t tok_stride[2], head_stride[2];
     const int64_t* slots;   // [T]
     int64_t T;
     uint8_t* cache[2];      // [pages][heads][page][dim]
     float* scale[2];        // [pages][heads]
     int64_t pages;
-    int heads, shift;  // pages of 1 << shift tokens
+    int heads, shift;       // pages of 1 << shift tokens
+    int window;             // tokens whose runs a CTA takes: at most a page
     int* status;
 };
 
@@ -173,134 +189,196 @@ __device__ __forceinline__ float2 pair_to_float(uint32_t v) {
     else return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
-template <bool E4M3, bool BF16, int D>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvAppendArgs a) {
-    // indices into the window's arrays: 0 is the token before the window
-    __shared__ int64_t slot[2 * kMaxPage + 1];
-    __shared__ uint32_t starts[(2 * kMaxPage) / 32];  // bit i: token w0 + i begins a run
-    __shared__ int amax[kMaxPage];                    // of the run that begins at token w0 + i (bits of a float >= 0)
-    __shared__ int exps[kMaxPage], olds[kMaxPage];
-    const int sh = a.shift, P = 1 << sh, W = 2 * P;
-    const int h = blockIdx.y, which = blockIdx.z;
-    const int64_t w0 = int64_t(blockIdx.x) * P;
+template <bool E4M3, bool BF16, int D, int THREADS>
+__global__ void __launch_bounds__(THREADS, 768 / THREADS) kv_append_kernel(const KvAppendArgs a) {
+    constexpr int LPR = D / 8;              // lanes per row (8 values each)
+    constexpr int RPW = 32 / LPR;           // rows per warp and iteration; even rows are K's, odd ones V's
+    constexpr int kWarps = THREADS / 32;
+    constexpr int kAlone = kAppendHold * RPW / 2;  // tokens of a run that one warp holds
+    __shared__ int64_t slot[2 * kMaxPage + 1];     // 0: the token before the window
+    __shared__ uint32_t starts[(2 * kMaxPage) / 32];
+    __shared__ int16_t begins[kMaxPage + 1];       // the window's runs: first token
+    __shared__ int n_runs;
+    __shared__ int amax[2];
+    const int sh = a.shift, P = 1 << sh, W = a.window, span = (W + P + 31) & ~31;
+    const int h = blockIdx.y;
+    const int64_t w0 = int64_t(blockIdx.x) * W;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int kWarps = kAppendThreads / 32;
 
-    for (int i = tid; i <= W; i += kAppendThreads) {
+    for (int i = tid; i <= span; i += THREADS) {
         const int64_t t = w0 - 1 + i;
         int64_t v = t >= 0 && t < a.T ? a.slots[t] : -1;
         if (v >= (a.pages << sh)) {
-            if (h == 0 && which == 0 && i > 0) set_status(a.status, DEV_BAD_INDEX);
+            if (h == 0 && i > 0) set_status(a.status, DEV_BAD_INDEX);
             v = -1;
         }
         slot[i] = v < 0 ? -1 : v;
     }
-    if (tid < P) amax[tid] = 0;
+    if (tid == 0) n_runs = 0;
     __syncthreads();
-    for (int i = tid; i < W; i += kAppendThreads) {
+    for (int i = tid; i < span; i += THREADS) {
         const int64_t v = slot[i + 1], u = slot[i];
-        const bool start = v >= 0 ? u < 0 || (u >> sh) != (v >> sh) : u >= 0;  // a run of skipped tokens counts as one
-        const uint32_t m = __ballot_sync(0xffffffffu, start || (i == 0 && v < 0));
+        // skipped tokens count as a run of their own, so that they end the one before
+        const bool start = v >= 0 ? u < 0 || (u >> sh) != (v >> sh) : u >= 0;
+        const uint32_t m = __ballot_sync(0xffffffffu, start);
         if (lane == 0) starts[i >> 5] = m;
+        if (start && v >= 0 && i < W) begins[atomicAdd(&n_runs, 1)] = int16_t(i);  // in any order
     }
     __syncthreads();
-    // first token of token i's run, -1 if it lies before the window or the token is skipped
-    auto run_of = [&](int i) {
-        if (slot[i + 1] < 0) return -1;
-        int w = i >> 5;
-        uint32_t m = starts[w] & (0xffffffffu >> (31 - (i & 31)));
-        while (m == 0 && w > 0) m = starts[--w];
-        return m ? (w << 5) + 31 - __clz(m) : -1;
+    const int last = int(min(int64_t(span), a.T - w0));
+    auto run_end = [&](int i) {  // first token after the run that begins at i
+        int w = (i + 1) >> 5;
+        if (i + 1 >= span) return last;
+        uint32_t m = starts[w] & (0xffffffffu << ((i + 1) & 31));
+        while (m == 0 && ++w < (span >> 5)) m = starts[w];
+        return min(min(m ? (w << 5) + __ffs(m) - 1 : span, last), i + P);
     };
-    const uint16_t* x = static_cast<const uint16_t*>(a.x[which]) + h * a.head_stride[which];
-    const int64_t ts = a.tok_stride[which];
-    const int last = int(min(int64_t(W), a.T - w0));
-    constexpr int V = D / 32;  // values per lane: 4 or 2
 
-    auto row = [&](int i, float (&v)[V]) {
-        const uint16_t* p = x + (w0 + i) * ts + lane * V;
-        if constexpr (V == 4) {
-            const uint2 r = *reinterpret_cast<const uint2*>(p);
-            const float2 lo = pair_to_float<BF16>(r.x), hi = pair_to_float<BF16>(r.y);
-            v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;
-        } else {
-            const float2 lo = pair_to_float<BF16>(*reinterpret_cast<const uint32_t*>(p));
-            v[0] = lo.x, v[1] = lo.y;
+    const int sub = lane / LPR, which = sub & 1, col = (lane % LPR) * 8;
+    const uint16_t* x = (which ? a.x[1] + h * a.head_stride[1] : a.x[0] + h * a.head_stride[0]) + col;
+    const int64_t ts = which ? a.tok_stride[1] : a.tok_stride[0];
+    uint8_t* cache = (which ? a.cache[1] : a.cache[0]) + col;
+    float* scales = which ? a.scale[1] : a.scale[0];
+    // Rows of tokens first + row / 2 (K where even): this lane's are row0, row0 + step, ...
+    uint4 v[kAppendHold];
+    auto load = [&](int first, int n, int row0, int step) {  // and their largest magnitude
+        float m = 0.f;
+        #pragma unroll
+        for (int i = 0; i < kAppendHold; ++i) {
+            const int t = (row0 + i * step) >> 1;
+            v[i] = t < n ? __ldg(reinterpret_cast<const uint4*>(x + (w0 + first + t) * ts)) : make_uint4(0, 0, 0, 0);
+        }
+        #pragma unroll
+        for (int i = 0; i < kAppendHold; ++i) {
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            #pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float2 f = pair_to_float<BF16>(w[q]);
+                m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));  // fmaxf leaves NaN out
+            }
+        }
+        #pragma unroll
+        for (int d = 1; d < LPR; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        if (RPW == 4) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2 * LPR));
+        return m;
+    };
+    auto code = [&](int first, int n, int row0, int step, int e) {
+        const float inv = exp2_int(-e);
+        const int64_t s = slot[first + 1];
+        const int64_t base = (((s >> sh) * a.heads + h) << sh) + (s & (P - 1));
+        #pragma unroll
+        for (int i = 0; i < kAppendHold; ++i) {
+            const int t = (row0 + i * step) >> 1;
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            float f[8];
+            bool nan = false;
+            #pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float2 p = pair_to_float<BF16>(w[q]);
+                nan |= p.x != p.x || p.y != p.y;
+                f[2 * q] = p.x * inv, f[2 * q + 1] = p.y * inv;
+            }
+            uint2 c;
+            if constexpr (E4M3) {
+                // A NaN of V goes into the token's key instead: every row that sees the token becomes
+                // NaN, and no other (0 * NaN would reach those that do not).
+                uint32_t bad = __ballot_sync(0xffffffffu, nan && which);
+                bad = (bad >> ((sub | 1) * LPR)) & ((1u << LPR) - 1u);
+                if (bad) {
+                    #pragma unroll
+                    for (int q = 0; q < 8; ++q) f[q] = which ? (f[q] == f[q] ? f[q] : 0.f) : NAN;
+                }
+            }
+            c.x = encode4<E4M3>(f[0], f[1], f[2], f[3]), c.y = encode4<E4M3>(f[4], f[5], f[6], f[7]);
+            if (t < n) *reinterpret_cast<uint2*>(cache + (base + t) * D) = c;
         }
     };
-    for (int i = warp; i < last; i += kWarps) {
-        const int r = run_of(i);
-        if (r >= P) break;   // this run and what follows belong to later windows
-        if (r < 0) continue;
-        float v[V], m = 0.f;
-        row(i, v);
-        #pragma unroll
-        for (int j = 0; j < V; ++j) m = fmaxf(m, fabsf(v[j]));  // fmaxf leaves NaN out
-        const int mi = __reduce_max_sync(0xffffffffu, __float_as_int(m));
-        if (lane == 0) atomicMax(&amax[r], mi);
-    }
-    __syncthreads();
-    if (tid < P && tid < last && run_of(tid) == tid) {
-        const int64_t v = slot[tid + 1], page = v >> sh;
-        float* sc = a.scale[which] + page * a.heads + h;
-        int e = scale_exponent<E4M3>(__int_as_float(amax[tid])), old = e;
-        if (v & (P - 1)) {  // joins a page that holds tokens already
+    // the scale of the run's tile, and the one it had
+    auto settle = [&](int first, float m, int& old) {
+        const int64_t s = slot[first + 1];
+        const float* sc = scales + (s >> sh) * a.heads + h;
+        int e = scale_exponent<E4M3>(m);
+        old = e;
+        if (s & (P - 1)) {  // joins a page that holds tokens already
             old = stored_exponent(*sc);
             e = max(e, old);
         }
-        exps[tid] = e, olds[tid] = old;
-        *sc = exp2_int(e);
-    }
-    __syncthreads();
-    auto store = [&](int64_t at, const float (&v)[V]) {
-        uint8_t* p = a.cache[which] + at * D + lane * V;
-        if constexpr (V == 4) *reinterpret_cast<uint32_t*>(p) = encode4<E4M3>(v[0], v[1], v[2], v[3]);
-        else *reinterpret_cast<uint16_t*>(p) = uint16_t(encode4<E4M3>(v[0], v[1], 0.f, 0.f));
+        return e;
     };
-    for (int i = warp; i < last; i += kWarps) {
-        const int r = run_of(i);
-        if (r >= P) break;
-        if (r < 0) continue;
-        float v[V];
-        row(i, v);
-        const float inv = exp2_int(-exps[r]);
-        #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] *= inv;
-        const int64_t s = slot[i + 1];
-        const int64_t tile = (((s >> sh) * a.heads + h) << sh);
+    auto publish = [&](int first, int e) {
+        const int64_t s = slot[first + 1];
+        scales[(s >> sh) * a.heads + h] = exp2_int(e);
+    };
+    // the scale grew: the tile's older codes (rows row0, row0 + step, ... of its first tokens) move to it
+    auto again = [&](int first, int row0, int step, int old, int e) {
+        const int64_t s = slot[first + 1], base = ((s >> sh) * a.heads + h) << sh;
         const int off = int(s & (P - 1));
-        store(tile + off, v);
-        if (r != i || olds[r] >= exps[r]) continue;
-        // the scale grew: the tile's older codes move to it
-        const float f = exp2_int(max(olds[r] - exps[r], -126));
-        for (int o = 0; o < off; ++o) {
-            const uint8_t* p = a.cache[which] + (tile + o) * D + lane * V;
-            const uint32_t w = V == 4 ? *reinterpret_cast<const uint32_t*>(p) : *reinterpret_cast<const uint16_t*>(p);
-            float c[4], u[V];
-            decode4<E4M3>(w, c);
-            #pragma unroll
-            for (int j = 0; j < V; ++j) u[j] = c[j] * f;
-            store(tile + o, u);
+        const float f = exp2_int(max(old - e, -126));
+        for (int r = row0; (r >> 1) < off; r += step) {
+            uint2* p = reinterpret_cast<uint2*>(cache + (base + (r >> 1)) * D);
+            const uint2 c = *p;
+            float u[4], w[4];
+            decode4<E4M3>(c.x, u);
+            decode4<E4M3>(c.y, w);
+            *p = make_uint2(encode4<E4M3>(u[0] * f, u[1] * f, u[2] * f, u[3] * f),
+                            encode4<E4M3>(w[0] * f, w[1] * f, w[2] * f, w[3] * f));
         }
+    };
+
+    bool longs = false;
+    for (int k = warp; k < n_runs; k += kWarps) {
+        const int first = begins[k], n = run_end(first) - first;
+        if (n > kAlone) {
+            longs = true;
+            continue;
+        }
+        const float m = load(first, n, sub, RPW);
+        int old;
+        const int e = settle(first, m, old);
+        __syncwarp();
+        if (lane % LPR == 0 && sub < 2) publish(first, e);
+        code(first, n, sub, RPW, e);
+        if (old < e) again(first, sub, RPW, old, e);
+    }
+    if (!__syncthreads_or(longs)) return;
+    for (int k = 0; k < n_runs; ++k) {
+        const int first = begins[k], n = run_end(first) - first;
+        if (n <= kAlone) continue;
+        if (tid < 2) amax[tid] = 0;
+        __syncthreads();
+        const float m = load(first, n, warp * RPW + sub, kWarps * RPW);
+        if (lane % LPR == 0 && sub < 2) atomicMax(&amax[which], __float_as_int(m));  // of floats >= 0
+        __syncthreads();
+        int old;
+        const int e = settle(first, __int_as_float(amax[which]), old);
+        __syncthreads();  // all have read the old scale
+        if (warp == 0 && lane % LPR == 0 && sub < 2) publish(first, e);
+        code(first, n, warp * RPW + sub, kWarps * RPW, e);
+        if (old < e) again(first, warp * RPW + sub, kWarps * RPW, old, e);
     }
 }
 
-cudaError_t run_kv_append(const KvAppendCall& c, cudaStream_t s) {
+template <bool E4M3, bool BF16, int D>
+static void launch_append(const KvAppendArgs& a, dim3 grid, cudaStream_t s) {
+    // a page's rows of K and V fit the CTA's registers: 2 P D / 8 lanes' worth in kAppendHold iterations
+    if (a.shift == 7) kv_append_kernel<E4M3, BF16, D, 512><<<grid, 512, 0, s>>>(a);
+    else kv_append_kernel<E4M3, BF16, D, 256><<<grid, 256, 0, s>>>(a);
+}
+
+cudaError_t run_kv_append(const KvAppendCall& c, int sms, cudaStream_t s) {
     if (c.tokens <= 0) return cudaSuccess;
     KvAppendArgs a;
     for (int i = 0; i < 2; ++i) {
-        a.x[i] = c.x[i], a.tok_stride[i] = c.tok_stride[i], a.head_stride[i] = c.head_stride[i];
+        a.x[i] = static_cast<const uint16_t*>(c.x[i]), a.tok_stride[i] = c.tok_stride[i], a.head_stride[i] = c.head_stride[i];
         a.cache[i] = static_cast<uint8_t*>(c.cache[i]), a.scale[i] = c.scale[i];
     }
     a.slots = c.slots, a.T = c.tokens, a.pages = c.pages, a.heads = c.heads, a.shift = page_shift(c.page), a.status = c.status;
-    const dim3 grid(unsigned((c.tokens + c.page - 1) / c.page), unsigned(c.heads), 2);
-    const auto go = [&](auto e4m3, auto bf16, auto dim) {
-        kv_append_kernel<decltype(e4m3)::value, decltype(bf16)::value, decltype(dim)::value>
-            <<<grid, kAppendThreads, 0, s>>>(a);
-    };
-    const auto by_dim = [&](auto e4m3, auto bf16) {
-        if (c.dim == 128) go(e4m3, bf16, std::integral_constant<int, 128>());
-        else go(e4m3, bf16, std::integral_constant<int, 64>());
+    // windows of a page where that gives every SM a CTA, else of 16 tokens (64 single tokens: two runs a warp)
+    a.window = (c.tokens / c.page) * c.heads >= sms ? c.page : 16;
+    const dim3 grid(unsigned((c.tokens + a.window - 1) / a.window), unsigned(c.heads), 1);
+    const auto by_dim = [&](auto e4, auto bf) {
+        constexpr bool E = decltype(e4)::value, B = decltype(bf)::value;
+        c.dim == 128 ? launch_append<E, B, 128>(a, grid, s) : launch_append<E, B, 64>(a, grid, s);
     };
     const bool bf16 = c.x_dtype == DT_BF16;
     if (c.e4m3) bf16 ? by_dim(std::true_type(), std::true_type()) : by_dim(std::true_type(), std::false_type());

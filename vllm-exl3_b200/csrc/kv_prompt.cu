@@ -676,7 +676,8 @@ static cudaError_t launch_prompt(const PrArgs& a, unsigned grid, cudaStream_t s)
     constexpr size_t smem = pr_smem_bytes<D>();
     static_assert(smem <= 227 * 1024 && kPrMaxSplits * kPrRows * 4 + sizeof(PrSmem) + 1024 <= smem, "shared memory");
     auto* kernel = kv_prompt_kernel<E4M3, BF16, D>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = raise_smem(kernel, smem, done);
     if (e != cudaSuccess) return e;
     kernel<<<grid, kPrThreads, smem, s>>>(a);
     return cudaGetLastError();

@@ -9,19 +9,18 @@
 //
 // Bound: every logit is read once: HBM (bf16: about 12 logits per clock and SM
 // at the measured copy rate, near the 16 per clock of the exponential unit).
-// A CTA takes a slice of one row, in chunks that its threads hold in
-// registers (16-byte loads, U of them in flight per thread), so a chunk's
-// maximum is known before its exponentials are taken.  Few rows: a row
-// is split over CTAs and joined by the one that ends last, in slice order.
+// A CTA streams a slice of one row, each thread 4 16-byte vectors at a time
+// with the next 4 on their way.  A thread's reference m follows its maximum
+// only when that has grown by more than 16: sums of exp(d <= 16) are as exact,
+// and the loop has no dependent rescaling.  Few rows: a row is split over CTAs
+// and joined by the one that ends last, always in the same order.
 //
 // Alternatives: entries are ordered by a 64-bit key (value, then lowest index
-// first).  The `top`-th largest of 32 group maxima of a chunk bounds the
-// answer from below, so a chunk yields some `top` candidates, not thousands;
-// they are collected in shared memory and reduced by counting, for each, the
-// larger ones.  Where more tie or pass the bound than the buffer holds, the
-// buffer is reduced, the bound rises, and the chunk is looked through again.
-// The few threads whose maximum passes the bound read their entries again
-// (from L1 or L2) rather than keep them in registers.
+// first).  The `top`-th largest of 32 thread groups' maxima bounds the answer
+// from below, so only the few threads whose maximum passes it have candidates;
+// all warps then read those threads' entries again (from L2) and collect what
+// passes, some `top` entries.  The buffer holds whatever one such round can
+// yield; before it could overflow (many ties) it is reduced, which raises the bound.
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -33,9 +32,13 @@
 namespace exl3 {
 
 constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
-constexpr int kLpCap = 2048;     // candidate keys a CTA holds
+constexpr int kLpUnroll = 4;     // vectors of a thread in flight, and in work
 constexpr int kLpMaxTop = 32;    // one group maximum each
+constexpr int kLpRound = kLpThreads * 8;               // most entries that one round of candidates looks at
+constexpr int kLpCap = kLpRound + 2 * kLpMaxTop;       // candidate keys a CTA holds
+constexpr float kLpSlack = 16.f;                       // growth of the maximum that the reference lets pass
 constexpr int kLpMaxSplit = 64;
+constexpr int kLpSplitRows = 32;  // rows per SM up to which rows are split
 static_assert(kLpMaxSplit * kLpMaxTop <= kLpCap, "the parts' lists are joined in one buffer");
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -46,7 +49,7 @@ struct LpArgs {
     int vocab;
     const void* tokens;
     int ids_dtype;
-    int top, splits, chunks;  // chunks per row
+    int top, splits;
     float *logprob, *entropy;
     int32_t* rank;
     float* top_logprobs;
@@ -154,104 +157,126 @@ struct LpType {
             return __half22float2(__hmax2_nan(h2(word(v, i)), h2(0xfbfffbffu)));
         }
     }
-    // Counts: of 16-bit types two at a time, as sums of ones (at most 32 a half before total())
+    // Entries above a threshold: of 16-bit types counted two at a time, as sums of ones
     using Count = std::conditional_t<DT == DT_F32, int, std::conditional_t<DT == DT_F16, __half2, __nv_bfloat162>>;
+    using Level = std::conditional_t<DT == DT_F32, float, uint32_t>;
     static __device__ __forceinline__ Count zero() {
         if constexpr (DT == DT_F32) return 0;
         else if constexpr (DT == DT_F16) return h2(0u);
         else return b2(0u);
     }
-    template <bool GE>
-    static __device__ __forceinline__ void count(Count& n, const uint4& v, float xt) {
+    static __device__ __forceinline__ Level level(float x) {  // exact: x is an entry, or infinite
         if constexpr (DT == DT_F32) {
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) n += GE ? get(v, i) >= xt : get(v, i) > xt;
+            return x;
+        } else if constexpr (DT == DT_F16) {
+            const __half2 t = __float2half2_rn(x);
+            return *reinterpret_cast<const uint32_t*>(&t);
         } else {
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (DT == DT_F16) {
-                    const __half2 t = __float2half2_rn(xt);  // exact: an entry of the row, or +inf
-                    n = __hadd2(n, GE ? __hge2(h2(word(v, i)), t) : __hgt2(h2(word(v, i)), t));
-                } else {
-                    const __nv_bfloat162 t = __float2bfloat162_rn(xt);
-                    n = __hadd2(n, GE ? __hge2(b2(word(v, i)), t) : __hgt2(b2(word(v, i)), t));
-                }
-            }
+            const __nv_bfloat162 t = __float2bfloat162_rn(x);
+            return *reinterpret_cast<const uint32_t*>(&t);
         }
     }
-    static __device__ __forceinline__ void count_ge(Count& n, const uint4& v, float xt) { count<true>(n, v, xt); }
-    static __device__ __forceinline__ void count_gt(Count& n, const uint4& v, float xt) { count<false>(n, v, xt); }
+    // the next lower number of the type, so that x >= t is x > below(t); t > -inf
+    static __device__ __forceinline__ Level below(Level t) {
+        if constexpr (DT == DT_F32) {
+            const uint32_t b = __float_as_uint(t);
+            return __uint_as_float((b & 0x7fffffffu) == 0u ? 0x80000001u : b >> 31 ? b + 1 : b - 1);
+        } else {
+            uint32_t b = t & 0xffffu;
+            b = (b & 0x7fffu) == 0u ? 0x8001u : b >> 15 ? b + 1 : b - 1;
+            return b | (b << 16);
+        }
+    }
+    static __device__ __forceinline__ void count(Count& n, const uint4& v, Level t) {
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == DT_F32) n += get(v, i) > t;
+            else if constexpr (DT == DT_F16) n = __hadd2(n, __hgt2(h2(word(v, i)), h2(t)));
+            else n = __hadd2(n, __hgt2(b2(word(v, i)), b2(t)));
+        }
+    }
     static __device__ __forceinline__ int total(Count n) {
         if constexpr (DT == DT_F32) return n;
         else return int(__low2float(n)) + int(__high2float(n));
     }
+    static __device__ __forceinline__ float at(const char* x, int64_t i) { return load_as_float(x, i, DT); }
+    static constexpr uint32_t kNone = DT == DT_F32 ? 0xff800000u : DT == DT_F16 ? 0xfc00fc00u : 0xff80ff80u;  // -inf
 };
 
-template <int DT, int U, bool TOP>
+template <int DT, bool TOP>
 __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a) {
     using T = LpType<DT>;
-    constexpr int VEC = T::kVec;
+    constexpr int VEC = T::kVec, U = kLpUnroll;
     extern __shared__ uint64_t lp_smem[];
     uint64_t* cand = lp_smem;            // [kLpCap]
     uint64_t* best = lp_smem + kLpCap;   // [kLpMaxSplit], at least kLpMaxTop
     __shared__ uint32_t group_max[32];
+    __shared__ uint16_t flagged[kLpThreads];
     __shared__ float wr[kLpWarps], ws[kLpWarps], ww[kLpWarps];
     __shared__ int wc[kLpWarps];
-    __shared__ int count, last_flag;
+    __shared__ int count, n_flagged, last_flag;
     __shared__ uint64_t bound;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x / a.splits;
     const int split = int(blockIdx.x % a.splits);
     const char* x = a.x + row * a.stride;
-    const int shift = int((reinterpret_cast<uintptr_t>(x) & 15) / T::kSize);  // entries of vector 0 before the row
-    const char* base = x - shift * T::kSize;
     const int64_t tok = load_id(a.tokens, row, a.ids_dtype);
     const bool asked = tok >= 0 && tok < a.vocab;
-    float xt = INFINITY;  // nothing ranks above it
-    if (asked) xt = load_as_float(x, tok, DT);
-    const int c0 = int(int64_t(a.chunks) * split / a.splits), c1 = int(int64_t(a.chunks) * (split + 1) / a.splits);
+    const float xt = asked ? T::at(x, tok) : INFINITY;  // nothing ranks above +inf
+
+    // The row: `head` entries up to the first 16-byte boundary, n_vec whole vectors, the rest.  This
+    // CTA's vectors are [v0, v1); the first part has the head too, the last one the rest.
+    const int head = min(int((-reinterpret_cast<uintptr_t>(x) & 15) / T::kSize), a.vocab);
+    const int n_vec = (a.vocab - head) / VEC, rest = (a.vocab - head) % VEC;
+    const uint4* vecs = reinterpret_cast<const uint4*>(x + head * T::kSize);
+    const int v0 = int(int64_t(n_vec) * split / a.splits), v1 = int(int64_t(n_vec) * (split + 1) / a.splits);
+    // index of this thread's single entry, one of the at most 2 (VEC - 1) at the ends, or -1
+    int single = -1;
+    if (split == 0 && tid < head) single = tid;
+    if (split == a.splits - 1 && tid >= 32 && tid < 32 + rest) single = a.vocab - rest + tid - 32;
+
+    // rank: entries before the token count when as high, the others when higher; entries of the
+    // token's own vector, and single ones, are looked at one by one
+    const bool lowest = xt == -INFINITY;  // every entry before it counts, seen or not
+    const auto above_t = T::level(xt), from_t = lowest ? T::level(INFINITY) : T::below(above_t);
+    const int tok_vec = !asked ? -1 : tok < head ? -1 : int((tok - head) / VEC);
 
     LpStats st{-INFINITY, 0.f, 0.f, 0};
-    if (tid == 0) count = 0, bound = 0;
-    __syncthreads();
+    float mx_all = -INFINITY;
+    if (single >= 0) {
+        const float v = T::at(x, single);
+        const bool fine = v < INFINITY;  // NaN and +inf make the row NaN
+        st.m = fine ? v : 0.f, st.s = fine ? (v == -INFINITY ? 0.f : 1.f) : NAN, st.w = fine ? 0.f : NAN;
+        if (asked && !(lowest && single < tok)) st.above += v > xt || (v == xt && single < tok);
+        mx_all = v == v ? v : -INFINITY;
+    }
+    if (asked && split == 0 && tid == 0 && lowest) st.above += int(tok);
+    if (asked && tok_vec >= v0 && tok_vec < v1 && tid >= 64 && tid < 64 + VEC) {
+        const int i = head + tok_vec * VEC + tid - 64;  // before it, in its vector, whose entries above it the loop counts
+        const float v = T::at(x, i);
+        if (i < tok) st.above += lowest ? -int(v > xt) : int(v == xt);
+    }
 
-    // 16-byte vector j of the row, whose first entry has index e0
-    auto load = [&](int64_t j, int64_t e0) {
-        if (e0 >= 0 && e0 + VEC <= a.vocab) return __ldg(reinterpret_cast<const uint4*>(base) + j);
-        uint32_t w[4];  // a row's ends: entry by entry, -inf outside
+    auto fetch = [&](uint4 (&v)[U], int j) {
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (DT == DT_F32) {
-                const int64_t e = e0 + i;
-                w[i] = e >= 0 && e < a.vocab ? reinterpret_cast<const uint32_t*>(x)[e] : 0xff800000u;
-            } else {
-                const uint32_t ninf = DT == DT_F16 ? 0xfc00u : 0xff80u;
-                const int64_t e = e0 + 2 * i;
-                const uint16_t* p = reinterpret_cast<const uint16_t*>(x);
-                const uint32_t lo = e >= 0 && e < a.vocab ? p[e] : ninf;
-                const uint32_t hi = e + 1 >= 0 && e + 1 < a.vocab ? p[e + 1] : ninf;
-                w[i] = lo | (hi << 16);
-            }
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
+        for (int u = 0; u < U; ++u)
+            v[u] = j + u * kLpThreads < v1 ? __ldg(vecs + j + u * kLpThreads) : make_uint4(T::kNone, T::kNone, T::kNone, T::kNone);
     };
-
-    for (int c = c0; c < c1; ++c) {
+    uint4 next[U];
+    fetch(next, v0 + tid);
+    #pragma unroll 1
+    for (int j0 = v0; j0 < v1; j0 += U * kLpThreads) {
         uint4 v[U];
-        const int64_t j0 = int64_t(c) * U * kLpThreads + tid;
-        float mx = -INFINITY;
         #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t j = j0 + u * kLpThreads;
-            v[u] = load(j, j * VEC - shift);
-        }
+        for (int u = 0; u < U; ++u) v[u] = next[u];
+        fetch(next, j0 + U * kLpThreads + tid);
+        float mx = T::largest(v[0]);
         #pragma unroll
-        for (int u = 0; u < U; ++u) mx = fmaxf(mx, T::largest(v[u]));
-
-        // --- sums ---
-        LpStats part{mx, 0.f, 0.f, 0};
-        const float ref = mx == -INFINITY ? 0.f : mx;
+        for (int u = 1; u < U; ++u) mx = fmaxf(mx, T::largest(v[u]));
+        mx_all = fmaxf(mx_all, mx);
+        if (mx > st.m + kLpSlack || (st.m == -INFINITY && mx > st.m)) lp_join(st, LpStats{mx, 0.f, 0.f, 0});
+        const float ref = st.m == -INFINITY ? 0.f : st.m;
         if (fabsf(ref) < T::kNear) {
             // two at a time.  -inf stands as the type's lowest number: its weight is 0 against such
             // a reference, and 0 times the difference stays 0
@@ -267,96 +292,79 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
                     s2 = add2(s2, e);
                     w2 = fma2(e, d, w2);
                 }
-            part.s = s2.x + s2.y, part.w = w2.x + w2.y;
+            st.s += s2.x + s2.y, st.w += w2.x + w2.y;
         } else {
-            #pragma unroll 1
-            for (int u = 0; u < U; ++u) {
-                const int64_t j = j0 + u * kLpThreads;
-                const uint4 again = load(j, j * VEC - shift);
+            #pragma unroll
+            for (int u = 0; u < U; ++u)
                 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    const float d = max_nan(T::get(again, i) - ref, -300.f);
+                    const float d = max_nan(T::get(v[u], i) - ref, -300.f);
                     const float e = ex2(d * kLog2e);
-                    part.s += e;
-                    part.w = fmaf(e, d, part.w);
+                    st.s += e;
+                    st.w = fmaf(e, d, st.w);
                 }
-            }
         }
-        // --- rank: entries above the token, and before it as high ---
-        typename T::Count before_n = T::zero(), after_n = T::zero();
+        typename T::Count n = T::zero();
         #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t e0 = (j0 + u * kLpThreads) * VEC - shift;
-            if (e0 + VEC <= tok) {
-                T::count_ge(before_n, v[u], xt);
-                // entries before the row's first one are no part of it
-                if (e0 < 0 && xt == -INFINITY) part.above += int(e0);
-            } else if (e0 > tok) {
-                T::count_gt(after_n, v[u], xt);
-            } else {
-                #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const float xi = T::get(v[u], i);
-                    part.above += xi > xt || (xi == xt && e0 + i >= 0 && e0 + i < tok);
-                }
-            }
-        }
-        part.above += T::total(before_n) + T::total(after_n);
-        lp_join(st, part);
+        for (int u = 0; u < U; ++u) T::count(n, v[u], j0 + tid + u * kLpThreads < tok_vec ? from_t : above_t);
+        st.above += T::total(n);
+    }
 
-        // --- alternatives ---
-        if constexpr (!TOP) continue;
-        uint32_t gm = sortable(mx);
-        if (!__syncthreads_or(gm >= uint32_t(bound >> 32))) continue;
+    // --- alternatives ---
+    if constexpr (TOP) {
+        const uint32_t own = sortable(mx_all);
+        uint32_t gm = own;
         gm = max(gm, __shfl_xor_sync(0xffffffffu, gm, 1));
         gm = max(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
         gm = max(gm, __shfl_xor_sync(0xffffffffu, gm, 4));
         if ((lane & 7) == 0) group_max[tid >> 3] = gm;
+        if (tid == 0) count = 0, n_flagged = 0, bound = 0;
         __syncthreads();
         if (warp == 0) {
             const uint32_t g = group_max[lane];
-            int r = 0;
+            int rank = 0;
             #pragma unroll
             for (int i = 0; i < 32; ++i) {
                 const uint32_t o = __shfl_sync(0xffffffffu, g, i);
-                r += o > g || (o == g && i < lane);
+                rank += o > g || (o == g && i < lane);
             }
-            if (r == a.top - 1) bound = max(bound, uint64_t(g) << 32);
+            if (rank == a.top - 1) bound = uint64_t(g) << 32;  // every key of the value g is above this
         }
         __syncthreads();
-        uint64_t pushed = 0;
-        for (;;) {
-            const uint64_t least = bound;
-            const uint32_t least_hi = uint32_t(least >> 32);
-            bool full = false;
-            if (sortable(mx) >= least_hi) {
-                #pragma unroll 1
-                for (int u = 0; u < U; ++u) {
-                    const int64_t j = j0 + u * kLpThreads, e0 = j * VEC - shift;
-                    const uint4 again = load(j, e0);
+        if (own >= uint32_t(bound >> 32)) flagged[atomicAdd(&n_flagged, 1)] = uint16_t(tid);
+        if (single >= 0) {
+            const uint64_t key = (uint64_t(sortable(T::at(x, single))) << 32) | (0xffffffffu - uint32_t(single));
+            if (key > bound) cand[atomicAdd(&count, 1)] = key;
+        }
+        __syncthreads();
+        // 32 vectors of 8 flagged threads a round: a warp to each
+        const int per = (v1 - v0 + kLpThreads - 1) / kLpThreads, rounds = (per + 31) / 32;
+        for (int f0 = 0; f0 < n_flagged; f0 += kLpWarps) {
+            for (int k = 0; k < rounds; ++k) {
+                const int n = count;
+                __syncthreads();
+                if (n > kLpCap - kLpRound) {
+                    lp_reduce(cand, best, n, a.top);
+                    if (tid == 0) {
+                        count = min(n, a.top);
+                        if (n >= a.top) bound = max(bound, cand[a.top - 1]);
+                    }
+                    __syncthreads();
+                }
+                const uint64_t least = bound;
+                const int j = f0 + warp < n_flagged ? v0 + flagged[f0 + warp] + (32 * k + lane) * kLpThreads : v1;
+                if (j < v1) {
+                    const uint4 v = __ldg(vecs + j);
                     #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        const uint32_t sv = sortable(T::get(again, i));
-                        if (sv < least_hi || e0 + i < 0 || e0 + i >= a.vocab) continue;
-                        const uint64_t key = (uint64_t(sv) << 32) | (0xffffffffu - uint32_t(e0 + i));
-                        if (key <= least || (pushed >> (u * VEC + i) & 1)) continue;
-                        const int at = atomicAdd(&count, 1);
-                        if (at < kLpCap) cand[at] = key, pushed |= uint64_t(1) << (u * VEC + i);
-                        else full = true;
+                        const uint64_t key = (uint64_t(sortable(T::get(v, i))) << 32) | (0xffffffffu - uint32_t(head + j * VEC + i));
+                        if (key > least) cand[atomicAdd(&count, 1)] = key;
                     }
                 }
+                __syncthreads();
             }
-            const bool again = __syncthreads_or(full);
-            const int n = min(count, kLpCap);
-            lp_reduce(cand, best, n, a.top);
-            if (tid == 0) {
-                count = min(n, a.top);
-                // keys at or below the last of a full list cannot enter it
-                if (n >= a.top) bound = max(bound, cand[a.top - 1]);
-            }
-            __syncthreads();
-            if (!again) break;
         }
+        lp_reduce(cand, best, count, a.top);
     }
 
     // --- join the threads ---
@@ -365,7 +373,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
     __syncthreads();
     st = LpStats{wr[0], ws[0], ww[0], wc[0]};
     for (int w = 1; w < kLpWarps; ++w) lp_join(st, LpStats{wr[w], ws[w], ww[w], wc[w]});
-    int have = a.top ? count : 0;
+    const int have = TOP ? min(count, a.top) : 0;
 
     if (a.splits > 1) {
         const int64_t slot = row * a.splits + split;
@@ -425,51 +433,51 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
     }
 }
 
-// A row's chunks of 256 threads x U vectors (one vector more than the row's
-// own where its start is not aligned), and over how many CTAs it is split:
-// what runs at once (4 CTAs per SM).
-struct LpPlan {
-    int U, chunks, splits;
-};
-static LpPlan lp_plan(const LogprobsCall& c, int sms) {
-    const int vec = c.x_dtype == DT_F32 ? 4 : 8;
-    auto chunks = [&](int U) { return int((c.vocab + vec - 1 + int64_t(vec) * kLpThreads * U - 1) / (int64_t(vec) * kLpThreads * U)); };
-    // few rows: chunks of 2 vectors, so that a row spreads over four times the CTAs
-    const int U = c.rows * chunks(8) < sms ? 2 : 8;
-    LpPlan p{U, chunks(U), 1};
-    const int64_t want = 4 * int64_t(sms) / c.rows;
-    p.splits = int(want < 1 ? 1 : want < p.chunks ? want : p.chunks);
-    if (p.splits > kLpMaxSplit) p.splits = kLpMaxSplit;
-    return p;
+// Over how many CTAs a row is split.  Few rows: as many as run at once (4 per
+// SM), no less than two vectors a thread.  Many rows: where whole rows would
+// leave the last wave mostly empty and are long, up to 4 parts, each counted as
+// 3 % of a wave more (its start and the join): 2048 rows of 131072 bf16 are
+// 3.46 waves of 592 and take LP_A us whole, LP_B us in halves.
+static int lp_splits(const LogprobsCall& c, int sms) {
+    const int64_t vectors = c.vocab / (c.x_dtype == DT_F32 ? 4 : 8), slots = 4 * int64_t(sms);
+    if (c.rows <= 2 * sms) {
+        const int64_t want = slots / c.rows, most = vectors / (2 * kLpThreads);
+        const int64_t n = want < most ? want : most;
+        return int(n < 1 ? 1 : n > kLpMaxSplit ? kLpMaxSplit : n);
+    }
+    int best = 1;
+    double least = 0.;
+    for (int n = 1; n <= 4 && (n == 1 || (vectors >= int64_t(n) * 16 * kLpThreads && c.rows <= kLpSplitRows * sms)); ++n) {
+        const double t = double((c.rows * n + slots - 1) / slots) / n * (1. + 0.03 * (n - 1));
+        if (n == 1 || t < least) best = n, least = t;
+    }
+    return best;
 }
 
-// a row is split only where there are at most two rows per SM
-int logprobs_counters(int sms) { return 2 * sms; }
+// one per row that can be split
+int logprobs_counters(int sms) { return kLpSplitRows * sms; }
 
 size_t logprobs_workspace(const LogprobsCall& c, int sms) {
-    const LpPlan p = lp_plan(c, sms);
-    return p.splits > 1 ? size_t(c.rows) * p.splits * (16 + 8 * size_t(c.top)) : 0;
+    const int splits = lp_splits(c, sms);
+    return splits > 1 ? size_t(c.rows) * splits * (16 + 8 * size_t(c.top)) : 0;
 }
 
 cudaError_t run_logprobs(const LogprobsCall& c, int sms, cudaStream_t s) {
     if (c.rows <= 0) return cudaSuccess;
-    const LpPlan p = lp_plan(c, sms);
     LpArgs a;
     a.x = static_cast<const char*>(c.logits), a.stride = c.stride * (c.x_dtype == DT_F32 ? 4 : 2);
     a.rows = c.rows, a.vocab = c.vocab, a.tokens = c.tokens, a.ids_dtype = c.ids_dtype;
-    a.top = c.top, a.splits = p.splits, a.chunks = p.chunks;
+    a.top = c.top, a.splits = lp_splits(c, sms);
     a.logprob = c.logprob, a.entropy = c.entropy, a.rank = c.rank;
     a.top_logprobs = c.top_logprobs, a.top_ids = c.top_ids, a.counters = c.counters;
     a.stats = reinterpret_cast<float4*>(c.ws);
-    a.keys = reinterpret_cast<uint64_t*>(c.ws + size_t(c.rows) * p.splits * 16);
+    a.keys = reinterpret_cast<uint64_t*>(c.ws + size_t(c.rows) * a.splits * 16);
     const size_t smem = c.top ? size_t(kLpCap + kLpMaxSplit) * 8 : 0;
-    const unsigned grid = unsigned(c.rows * p.splits);
+    const unsigned grid = unsigned(c.rows * a.splits);
     const auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (p.U == 8 && c.top) logprobs_kernel<DT, 8, true><<<grid, kLpThreads, smem, s>>>(a);
-        else if (p.U == 8) logprobs_kernel<DT, 8, false><<<grid, kLpThreads, smem, s>>>(a);
-        else if (c.top) logprobs_kernel<DT, 2, true><<<grid, kLpThreads, smem, s>>>(a);
-        else logprobs_kernel<DT, 2, false><<<grid, kLpThreads, smem, s>>>(a);
+        if (c.top) logprobs_kernel<DT, true><<<grid, kLpThreads, smem, s>>>(a);
+        else logprobs_kernel<DT, false><<<grid, kLpThreads, smem, s>>>(a);
     };
     if (c.x_dtype == DT_F32) go(std::integral_constant<int, DT_F32>());
     else if (c.x_dtype == DT_F16) go(std::integral_constant<int, DT_F16>());

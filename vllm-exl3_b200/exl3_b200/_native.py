@@ -7,9 +7,9 @@ torch's current stream of the tensors' device.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -74,16 +74,24 @@ SIGNATURES = {
                                   ctypes.POINTER(SZ)]),
     "exl3_ngram_dequant": (I32, [P, I64, I32, P, P, I32, P, I32, P]),
     "exl3_ngram_lookup": (I32, [P, I64, I32, P, I32, I64, P, I32, P, P, I32, P, P]),
-    "exl3_kv_plan": (I32, [P, P, I32, P, I32, P, I32, P, I32, I32, P, P, P, P, P, P, P]),
-    "exl3_kv_append": (I32, [P, I64, I64, P, I64, I64, I32, P, I64, P, P, P, P, I32, I64, I32, I32, I32, P, P]),
+    # the serving entries take a packed struct of 8-byte fields (see Args)
+    "exl3_kv_plan": (I32, [P, P]),
+    "exl3_kv_append": (I32, [P, P]),
     "exl3_kv_attend_workspace_size": (SZ, [I32, I32, I32, I32, I32, I64]),
-    "exl3_kv_attend": (I32, [P, I64, I64, I32, I64, I32, P, P, P, P, I32, I64, I32, I32, I32, P, I32, I32, P, P, I32,
-                             F32, I64, P, P, P, SZ, P]),
+    "exl3_kv_attend": (I32, [P, P]),
     "exl3_token_logprobs_workspace_size": (SZ, [I64, I64, I32, I32]),
-    "exl3_token_logprobs": (I32, [P, I32, I64, I64, I64, P, I32, I32, P, P, P, P, P, P, SZ, P]),
+    "exl3_token_logprobs": (I32, [P, P]),
     "exl3_profile_enable": (I32, [I32, ctypes.c_longlong]),
     "exl3_profile_read": (I32, [ctypes.POINTER(F32), I32, ctypes.POINTER(I32)]),
 }
+
+
+# exl3_*_args structs: one 8-byte field per argument, in the header's order
+# (pointers and integers "q", the attention scale "d")
+PACK_KV_PLAN = struct.Struct("16q").pack
+PACK_KV_APPEND = struct.Struct("19q").pack
+PACK_KV_ATTEND = struct.Struct("21qd5q").pack
+PACK_TOKEN_LOGPROBS = struct.Struct("15q").pack
 
 
 def lib_path() -> str:
@@ -93,6 +101,8 @@ def lib_path() -> str:
 def load():
     """Load (building first if the sources are newer) and bind the library."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -136,17 +146,10 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
-def raw_stream(device: torch.device) -> int:
-    """torch's current stream of ``device`` as a raw handle."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-_NO_SWITCH = contextlib.nullcontext()
-
-
-def on_device(device: torch.device):
-    """A guard that makes ``device`` current; free of cost where it is already."""
-    return _NO_SWITCH if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+# torch's current stream of a device (by index) as a raw handle, and the current device
+raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
 def require_cuda(*tensors: torch.Tensor | None, who: str) -> None:
@@ -204,21 +207,26 @@ def workspace(device: torch.device, nbytes: int, stream: torch.cuda.Stream | Non
     return buf
 
 
-def zeroed_workspace(device: torch.device, nbytes: int, stream: int) -> torch.Tensor:
-    """The workspace of the cache and log-probability entries for the raw
-    ``stream`` of ``device``: kept apart from :func:`workspace` because those
-    entries need its counters zero and leave them zero.  Grows and is retained
-    in the same way."""
-    key = (device.type, device.index, stream, "zeroed")
-    buf = _ws_cache.get(key)
-    if buf is None or buf.numel() < nbytes:
+_serve_ws: dict[tuple[int, int], tuple[int, int]] = {}
+
+
+def serve_workspace(index: int, stream: int, nbytes: int = 0) -> tuple[int, int]:
+    """(address, bytes) of the workspace of the cache and log-probability
+    entries for the raw ``stream`` of device ``index``.  It is kept apart from
+    :func:`workspace` because those entries need its counters zero and leave
+    them zero.  Grows and is retained in the same way."""
+    have = _serve_ws.get((index, stream))
+    if have is None or have[1] < nbytes:
+        key = ("cuda", index, stream, "serve")
         size = max(int(nbytes), 1 << 20)
-        if buf is not None:
-            size = max(size, 2 * buf.numel())
-            _ws_retired.append(buf)
-        buf = torch.zeros(size, dtype=torch.uint8, device=device)
+        old = _ws_cache.get(key)
+        if old is not None:
+            size = max(size, 2 * old.numel())
+            _ws_retired.append(old)
+        buf = torch.zeros(size, dtype=torch.uint8, device=torch.device("cuda", index))
         _ws_cache[key] = buf
-    return buf
+        have = _serve_ws[(index, stream)] = (buf.data_ptr(), size)
+    return have
 
 
 def device_workspaces(device: torch.device) -> list[torch.Tensor]:

@@ -13,6 +13,7 @@ three can be captured in a CUDA graph once each shape has run before.
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -33,13 +34,19 @@ class KvPlan(NamedTuple):
     cursor: torch.Tensor     # int32 [1] the free list's cursor after the step
 
 
-def _int32(t: torch.Tensor, name: str, who: str, dim: int = 1) -> None:
-    if t.dtype != torch.int32 or t.dim() != dim or not t.is_contiguous():
-        raise ValueError(f"{who}: {name} must be a contiguous int32 tensor of {dim} dimension(s)")
+# The operators run for a few microseconds, so a call first asks whether all is
+# well in one expression; only a call that is not goes through _explain, which
+# says what is wrong.
+
+def _explain(who: str, *wrong: tuple[bool, str]):
+    for bad, what in wrong:
+        if bad:
+            raise ValueError(f"{who}: {what}")
+    raise ValueError(f"{who}: arguments do not fit together")
 
 
-def _workspace(dev: torch.device, stream: int, nbytes: int = 0) -> torch.Tensor:
-    return _n.zeroed_workspace(dev, nbytes, stream)
+def _is_i32(t: torch.Tensor, dim: int = 1) -> bool:
+    return t.dtype is torch.int32 and t.dim() == dim and t.is_contiguous()
 
 
 def kv_plan(lens: torch.Tensor, new_tokens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
@@ -53,59 +60,73 @@ def kv_plan(lens: torch.Tensor, new_tokens: torch.Tensor, block_table: torch.Ten
     (int32 [requests, width], updated in place); the inputs ``lens``,
     ``cursor`` and ``free_pages`` stay as they are, the result carries their
     successors.  A free list or a table that runs out gives slots of -1 and
-    records status 7 (``_native`` workspaces, ``vllm_exl3_c.device_status``).
+    records status 7 (``vllm_exl3_c.device_status``).
     """
-    who = "kv_plan"
-    _n.require_cuda(lens, new_tokens, block_table, free_pages, cursor, who=who)
-    for t, name in ((lens, "lens"), (new_tokens, "new_tokens"), (free_pages, "free_pages"), (cursor, "cursor")):
-        _int32(t, name, who)
-    _int32(block_table, "block_table", who, 2)
     B = lens.numel()
-    if new_tokens.numel() != B or block_table.size(0) != B or cursor.numel() != 1:
-        raise ValueError(f"{who}: lens, new_tokens and block_table must have one row per request, cursor one value")
-    if page_size not in PAGES:
-        raise ValueError(f"{who}: page_size must be one of {PAGES}")
-    n_tokens = int(n_tokens)
-    if n_tokens < 0:
-        raise ValueError(f"{who}: n_tokens must be >= 0")
-    dev = lens.device
-    with _n.on_device(dev):
-        stream = _n.raw_stream(dev)
-        # one buffer: slots (8 bytes a token) first, then the int32 results
-        buf = torch.empty(3 * n_tokens + 2 * B + 2, dtype=torch.int32, device=dev)
-        at = buf.data_ptr()
-        p_pos, p_lens = at + 8 * n_tokens, at + 12 * n_tokens
-        p_cu = p_lens + 4 * B
-        _n.check(_n.load().exl3_kv_plan(
-            lens.data_ptr(), new_tokens.data_ptr(), B, block_table.data_ptr(), block_table.size(1),
-            free_pages.data_ptr(), free_pages.numel(), cursor.data_ptr(), page_size, n_tokens, p_lens, p_cu, p_pos, at,
-            p_cu + 4 * B + 4, _workspace(dev, stream).data_ptr(), stream), who)
-    slots, pos, kv_lens, cu, cur = buf.split((2 * n_tokens, n_tokens, B, B + 1, 1))
+    if not (lens.is_cuda and new_tokens.is_cuda and block_table.is_cuda and free_pages.is_cuda and cursor.is_cuda
+            and _is_i32(lens) and _is_i32(new_tokens) and _is_i32(free_pages) and _is_i32(cursor)
+            and _is_i32(block_table, 2) and new_tokens.numel() == B and block_table.size(0) == B
+            and cursor.numel() == 1 and page_size in PAGES and n_tokens >= 0):
+        who = "kv_plan"
+        _n.require_cuda(lens, new_tokens, block_table, free_pages, cursor, who=who)
+        named = (("lens", lens), ("new_tokens", new_tokens), ("free_pages", free_pages), ("cursor", cursor))
+        _explain(who, *((not _is_i32(t), f"{n} must be a contiguous int32 tensor of one dimension") for n, t in named),
+                 (not _is_i32(block_table, 2), "block_table must be a contiguous int32 tensor of two dimensions"),
+                 (page_size not in PAGES, f"page_size must be one of {PAGES}"),
+                 (n_tokens < 0, "n_tokens must be >= 0"),
+                 (True, "lens, new_tokens and block_table must have one row per request, cursor one value"))
+    dev = lens.device.index
+    if dev != _n.current_device():
+        with torch.cuda.device(dev):
+            return kv_plan(lens, new_tokens, block_table, free_pages, cursor, page_size=page_size, n_tokens=n_tokens)
+    stream = _n.raw_stream(dev)
+    # one buffer: slots (8 bytes a token) first, then the int32 results
+    buf = lens.new_empty(3 * n_tokens + 2 * B + 2)
+    at = buf.data_ptr()
+    p_lens = at + 12 * n_tokens
+    p_cu = p_lens + 4 * B
+    rc = _n.load().exl3_kv_plan(_n.PACK_KV_PLAN(
+        lens.data_ptr(), new_tokens.data_ptr(), B, block_table.data_ptr(), block_table.size(1), free_pages.data_ptr(),
+        free_pages.numel(), cursor.data_ptr(), page_size, n_tokens, p_lens, p_cu, at + 8 * n_tokens, at,
+        p_cu + 4 * B + 4, _n.serve_workspace(dev, stream)[0]), stream)
+    if rc:
+        _n.check(rc, "kv_plan")
+    slots, pos, kv_lens, cu, cur = torch.unsafe_split_with_sizes(buf, (2 * n_tokens, n_tokens, B, B + 1, 1))
     return KvPlan(kv_lens, cu, pos, slots.view(torch.int64), cur)
 
 
-def _check_cache(k_cache, v_cache, k_scale, v_scale, who: str) -> tuple[int, int, int, int, int]:
+def _bad_cache(who: str, k_cache, v_cache, k_scale, v_scale) -> None:
+    """Raises what is wrong with a cache, if anything."""
     _n.require_cuda(k_cache, v_cache, k_scale, v_scale, who=who)
-    code = _CODES.get(k_cache.dtype)
-    if code is None or v_cache.dtype != k_cache.dtype:
-        raise ValueError(f"{who}: the caches must both be float8_e4m3fn or both int8")
     shape = k_cache.shape
-    if len(shape) != 4 or v_cache.shape != shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
-        raise ValueError(f"{who}: the caches must be contiguous [pages, kv_heads, page, dim] of one shape")
-    pages, heads, page, dim = shape
-    if page not in PAGES or dim not in DIMS:
-        raise ValueError(f"{who}: page must be one of {PAGES} and dim one of {DIMS} (got {page}, {dim})")
-    for s in (k_scale, v_scale):
-        if s.dtype != torch.float32 or s.shape != (pages, heads) or not s.is_contiguous():
-            raise ValueError(f"{who}: scales must be contiguous fp32 [pages, kv_heads]")
-    return code, pages, heads, page, dim
+    four = len(shape) == 4 and v_cache.shape == shape and k_cache.is_contiguous() and v_cache.is_contiguous()
+    wrong = [(k_cache.dtype not in _CODES or v_cache.dtype != k_cache.dtype,
+              "the caches must both be float8_e4m3fn or both int8"),
+             (not four, "the caches must be contiguous [pages, kv_heads, page, dim] of one shape")]
+    if four:
+        wrong += [(shape[2] not in PAGES or shape[3] not in DIMS,
+                   f"page must be one of {PAGES} and dim one of {DIMS} (got {shape[2]}, {shape[3]})")]
+        wrong += [(t.dtype != torch.float32 or t.shape != shape[:2] or not t.is_contiguous(),
+                   "scales must be contiguous fp32 [pages, kv_heads]") for t in (k_scale, v_scale)]
+    for bad, what in wrong:
+        if bad:
+            raise ValueError(f"{who}: {what}")
 
 
-def _rows(x: torch.Tensor, bytes_: int) -> torch.Tensor:
-    """x, or a copy of it, with rows that start at multiples of ``bytes_``."""
+def _cache_ok(k_cache, v_cache, k_scale, v_scale) -> bool:
+    shape = k_cache.shape
+    return (k_cache.is_cuda and v_cache.is_cuda and k_scale.is_cuda and v_scale.is_cuda and k_cache.dtype in _CODES
+            and v_cache.dtype is k_cache.dtype and len(shape) == 4 and v_cache.shape == shape
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and shape[2] in PAGES and shape[3] in DIMS
+            and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
+            and k_scale.shape == shape[:2] and v_scale.shape == shape[:2]
+            and k_scale.is_contiguous() and v_scale.is_contiguous())
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x, or a copy of it, with rows that start at multiples of 16 bytes."""
     a, b, c = x.stride()
-    n = bytes_ // 2
-    return x if c == 1 and a % n == 0 and b % n == 0 and x.data_ptr() % bytes_ == 0 else x.contiguous()
+    return x if c == 1 and not (a | b) & 7 and not x.data_ptr() & 15 else x.clone(memory_format=torch.contiguous_format)
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -116,28 +137,42 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
 
     A page's scale is set by the call that writes its first token and grows
     when a later token needs it, the older codes being rounded to it again.
+    In e4m3 a NaN of ``v`` is kept in the token's key (attention rows that see
+    the token become NaN, others do not); int8 has no NaN and takes 0.
     """
-    who = "kv_append"
-    code, pages, heads, page, dim = _check_cache(k_cache, v_cache, k_scale, v_scale, who)
-    _n.require_cuda(k, v, slots, who=who)
-    x = _ROWS.get(k.dtype)
-    if x is None or v.dtype != k.dtype:
-        raise ValueError(f"{who}: k and v must both be fp16 or both bf16")
     n = slots.numel()
-    if k.shape != (n, heads, dim) or v.shape != (n, heads, dim):
-        raise ValueError(f"{who}: k and v must be [{n}, {heads}, {dim}] (slots, kv heads, dim)")
-    if slots.dtype != torch.int64 or not slots.is_contiguous():
-        raise ValueError(f"{who}: slots must be contiguous int64")
+    x = _ROWS.get(k.dtype)
+    if not (_cache_ok(k_cache, v_cache, k_scale, v_scale) and k.is_cuda and v.is_cuda and slots.is_cuda
+            and x is not None and v.dtype is k.dtype and slots.dtype is torch.int64 and slots.is_contiguous()
+            and k.dim() == 3 and k.size(0) == n and k.shape[1:] == k_cache.shape[1::2] and v.shape == k.shape):
+        who = "kv_append"
+        _bad_cache(who, k_cache, v_cache, k_scale, v_scale)
+        _n.require_cuda(k, v, slots, who=who)
+        _, heads, _, dim = k_cache.shape
+        _explain(who, (x is None or v.dtype != k.dtype, "k and v must both be fp16 or both bf16"),
+                 (slots.dtype != torch.int64 or not slots.is_contiguous(), "slots must be contiguous int64"),
+                 (True, f"k and v must be [{n}, {heads}, {dim}] (slots, kv heads, dim)"))
     if n == 0:
         return
-    k, v = _rows(k, 8), _rows(v, 8)
-    dev = k_cache.device
-    with _n.on_device(dev):
-        stream = _n.raw_stream(dev)
-        _n.check(_n.load().exl3_kv_append(
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), x, slots.data_ptr(), n,
-            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), code, pages, heads, page,
-            dim, _workspace(dev, stream).data_ptr(), stream), who)
+    dev = k_cache.device.index
+    if dev != _n.current_device():
+        with torch.cuda.device(dev):
+            return kv_append(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+    stream = _n.raw_stream(dev)
+    k, v = _rows(k), _rows(v)
+    kt, kh, _ = k.stride()
+    vt, vh, _ = v.stride()
+    rc = _n.load().exl3_kv_append(_n.PACK_KV_APPEND(
+        k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, x, slots.data_ptr(), n, k_cache.data_ptr(), v_cache.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), _CODES[k_cache.dtype], *k_cache.shape,
+        _n.serve_workspace(dev, stream)[0]), stream)
+    if rc:
+        _n.check(rc, "kv_append")
+
+
+@functools.lru_cache(maxsize=1024)
+def _attend_bytes(device: int, heads: int, kv_heads: int, dim: int, max_new: int, requests: int, rows: int) -> int:
+    return _n.load().exl3_kv_attend_workspace_size(heads, kv_heads, dim, max_new, requests, rows)
 
 
 def kv_attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -153,43 +188,48 @@ def kv_attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
     ``window`` keys, its own included (0: no limit); ``scale`` defaults to
     dim ** -0.5.  Rows that see no key are zeros (lse -inf).
     """
-    who = "kv_attend"
-    code, pages, kv_heads, page, dim = _check_cache(k_cache, v_cache, k_scale, v_scale, who)
-    _n.require_cuda(q, block_table, kv_lens, cu_tokens, who=who)
     x = _ROWS.get(q.dtype)
-    if x is None or q.dim() != 3 or q.size(2) != dim:
-        raise ValueError(f"{who}: q must be fp16 or bf16 [rows, heads, {dim}]")
-    rows, heads, _ = q.shape
-    if heads == 0 or heads % kv_heads:
-        raise ValueError(f"{who}: heads ({heads}) must be a multiple of kv_heads ({kv_heads})")
-    _int32(block_table, "block_table", who, 2)
-    _int32(kv_lens, "kv_lens", who)
     B = kv_lens.numel()
-    if block_table.size(0) != B:
-        raise ValueError(f"{who}: block_table must have one row per request")
-    if cu_tokens is None:
-        if rows != B or max_new != 1:
-            raise ValueError(f"{who}: without cu_tokens every request has one row of q")
-    else:
-        _int32(cu_tokens, "cu_tokens", who)
-        if cu_tokens.numel() != B + 1:
-            raise ValueError(f"{who}: cu_tokens must have one entry more than there are requests")
-    if max_new < 1 or window < 0:
-        raise ValueError(f"{who}: max_new must be >= 1 and window >= 0")
-    q = _rows(q, 16)
-    dev = k_cache.device
-    out = torch.empty((rows, heads, dim), dtype=q.dtype, device=dev)
-    lse = torch.empty((rows, heads), dtype=torch.float32, device=dev) if return_lse else None
-    with _n.on_device(dev):
-        lib = _n.load()
-        stream = _n.raw_stream(dev)
-        ws = _workspace(dev, stream, lib.exl3_kv_attend_workspace_size(heads, kv_heads, dim, max_new, B, rows))
-        _n.check(lib.exl3_kv_attend(
-            q.data_ptr(), q.stride(0), q.stride(1), x, rows, heads, k_cache.data_ptr(), v_cache.data_ptr(),
-            k_scale.data_ptr(), v_scale.data_ptr(), code, pages, kv_heads, page, dim, block_table.data_ptr(),
-            block_table.size(1), B, kv_lens.data_ptr(), _n.ptr(cu_tokens), max_new,
-            dim ** -0.5 if scale is None else float(scale), int(window), out.data_ptr(), _n.ptr(lse), ws.data_ptr(),
-            ws.numel(), stream), who)
+    if not (_cache_ok(k_cache, v_cache, k_scale, v_scale) and q.is_cuda and block_table.is_cuda and kv_lens.is_cuda
+            and x is not None and q.dim() == 3 and q.size(2) == k_cache.size(3) and q.size(1)
+            and not q.size(1) % k_cache.size(1) and _is_i32(block_table, 2) and _is_i32(kv_lens)
+            and block_table.size(0) == B and max_new >= 1 and window >= 0
+            and ((q.size(0) == B and max_new == 1) if cu_tokens is None
+                 else cu_tokens.is_cuda and _is_i32(cu_tokens) and cu_tokens.numel() == B + 1)):
+        who = "kv_attend"
+        _bad_cache(who, k_cache, v_cache, k_scale, v_scale)
+        _n.require_cuda(q, block_table, kv_lens, cu_tokens, who=who)
+        _, kv_heads, _, dim = k_cache.shape
+        _explain(who, (x is None or q.dim() != 3 or q.size(-1) != dim, f"q must be fp16 or bf16 [rows, heads, {dim}]"),
+                 (q.dim() == 3 and (q.size(1) == 0 or q.size(1) % kv_heads != 0),
+                  f"heads ({q.size(min(1, q.dim() - 1))}) must be a multiple of kv_heads ({kv_heads})"),
+                 (not _is_i32(block_table, 2) or block_table.size(0) != B,
+                  "block_table must be contiguous int32 with one row per request"),
+                 (not _is_i32(kv_lens), "kv_lens must be a contiguous int32 tensor of one dimension"),
+                 (max_new < 1 or window < 0, "max_new must be >= 1 and window >= 0"),
+                 (cu_tokens is None, "without cu_tokens every request has one row of q"),
+                 (True, "cu_tokens must be contiguous int32 with one entry more than there are requests"))
+    dev = k_cache.device.index
+    if dev != _n.current_device():
+        with torch.cuda.device(dev):
+            return kv_attend(q, k_cache, v_cache, k_scale, v_scale, block_table, kv_lens, cu_tokens=cu_tokens,
+                             max_new=max_new, scale=scale, window=window, return_lse=return_lse)
+    stream = _n.raw_stream(dev)
+    rows, heads, dim = shape = q.shape
+    pages, kv_heads, page, _ = k_cache.shape
+    q = _rows(q)
+    qt, qh, _ = q.stride()
+    out = q.new_empty(shape)
+    lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
+    ws, ws_bytes = _n.serve_workspace(dev, stream, _attend_bytes(dev, heads, kv_heads, dim, max_new, B, rows))
+    rc = _n.load().exl3_kv_attend(_n.PACK_KV_ATTEND(
+        q.data_ptr(), qt, qh, x, rows, heads, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), _CODES[k_cache.dtype], pages, kv_heads, page, dim, block_table.data_ptr(),
+        block_table.size(1), B, kv_lens.data_ptr(), 0 if cu_tokens is None else cu_tokens.data_ptr(), max_new,
+        dim ** -0.5 if scale is None else scale, window, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        ws, ws_bytes), stream)
+    if rc:
+        _n.check(rc, "kv_attend")
     return (out, lse) if return_lse else out
 
 

@@ -4,6 +4,7 @@ what scoring a text with a quantised pack sums up."""
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -11,6 +12,7 @@ import torch
 from . import _native as _n
 
 MAX_TOP = 32
+_LOGITS = {torch.float32: _n.DT_F32, torch.float16: _n.DT_F16, torch.bfloat16: _n.DT_BF16}
 _IDS = {torch.int32: _n.DT_I32, torch.int64: _n.DT_I64}
 
 
@@ -22,39 +24,55 @@ class TokenLogprobs(NamedTuple):
     top_ids: torch.Tensor       # int32 [rows, top]
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(device: int, rows: int, vocab: int, top: int, x: int) -> int:
+    return _n.load().exl3_token_logprobs_workspace_size(rows, vocab, top, x)
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) -> TokenLogprobs:
     """log softmax of ``logits`` (fp32, fp16 or bf16 [rows, vocab]) at
     ``tokens`` (int32 or int64 [rows]) in one pass over the logits, computed in
     fp32.  Equal logits rank lowest index first.  Tokens outside the vocabulary
     (padding) get logprob -inf and rank 0.  ``top``: 0 to 32 alternatives."""
-    who = "token_logprobs"
-    _n.require_cuda(logits, tokens, who=who)
-    if logits.dim() != 2 or not logits.is_floating_point():
-        raise ValueError(f"{who}: logits must be fp32, fp16 or bf16 [rows, vocab]")
-    x = _n.dtype_code(logits)
+    x, ids = _LOGITS.get(logits.dtype), _IDS.get(tokens.dtype)
+    if not (logits.is_cuda and tokens.is_cuda and x is not None and ids is not None and logits.dim() == 2
+            and tokens.shape == logits.shape[:1] and 0 <= top <= MAX_TOP and top <= logits.size(1)):
+        who = "token_logprobs"
+        _n.require_cuda(logits, tokens, who=who)
+        if x is None or logits.dim() != 2:
+            raise ValueError(f"{who}: logits must be fp32, fp16 or bf16 [rows, vocab]")
+        if ids is None or tokens.shape != logits.shape[:1]:
+            raise ValueError(f"{who}: tokens must be int32 or int64 [{logits.size(0)}]")
+        raise ValueError(f"{who}: top must be in 0..{min(MAX_TOP, logits.size(1))}")
+    dev = logits.device.index
+    if dev != _n.current_device():
+        with torch.cuda.device(dev):
+            return token_logprobs(logits, tokens, top=top)
     rows, vocab = logits.shape
-    ids = _IDS.get(tokens.dtype)
-    if ids is None or tokens.shape != (rows,):
-        raise ValueError(f"{who}: tokens must be int32 or int64 [{rows}]")
-    if not 0 <= top <= min(MAX_TOP, vocab):
-        raise ValueError(f"{who}: top must be in 0..{min(MAX_TOP, vocab)}")
-    if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
-        logits = logits.contiguous()
-    tokens = tokens.contiguous()
-    dev = logits.device
-    # one buffer: logprob, entropy, rank, alternatives
-    buf = torch.empty(rows * (3 + 2 * top), dtype=torch.float32, device=dev)
+    row_stride, step = logits.stride()
+    if step != 1 or (rows > 1 and row_stride < vocab):
+        logits = logits.clone(memory_format=torch.contiguous_format)
+        row_stride = vocab
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    # one buffer: logprob and entropy, the alternatives' values; rank, their ids
+    buf = logits.new_empty(rows * (2 + top), dtype=torch.float32)
+    whole = logits.new_empty(rows * (1 + top), dtype=torch.int32)
     if rows:
-        with _n.on_device(dev):
-            lib = _n.load()
-            stream = _n.raw_stream(dev)
-            ws = _n.zeroed_workspace(dev, lib.exl3_token_logprobs_workspace_size(rows, vocab, top, x), stream)
-            at, n = buf.data_ptr(), 4 * rows
-            _n.check(lib.exl3_token_logprobs(
-                logits.data_ptr(), x, rows, logits.stride(0), vocab, tokens.data_ptr(), ids, top, at, at + n,
-                at + 2 * n, at + 3 * n, at + (3 + top) * n, ws.data_ptr(), ws.numel(), stream), who)
-    lp, ent, rank, tlp, tid = buf.split((rows, rows, rows, rows * top, rows * top))
-    return TokenLogprobs(lp, ent, rank.view(torch.int32), tlp.view(rows, top), tid.view(torch.int32).view(rows, top))
+        stream = _n.raw_stream(dev)
+        ws, ws_bytes = _n.serve_workspace(dev, stream, _workspace_bytes(dev, rows, vocab, top, x))
+        at, to, n = buf.data_ptr(), whole.data_ptr(), 4 * rows
+        rc = _n.load().exl3_token_logprobs(_n.PACK_TOKEN_LOGPROBS(
+            logits.data_ptr(), x, rows, row_stride, vocab, tokens.data_ptr(), ids, top, at, at + n, to, at + 2 * n,
+            to + n, ws, ws_bytes), stream)
+        if rc:
+            _n.check(rc, "token_logprobs")
+    if top == 0:
+        lp, ent = torch.unsafe_split_with_sizes(buf, (rows, rows))
+        return TokenLogprobs(lp, ent, whole, buf.new_empty((rows, 0)), whole.new_empty((rows, 0)))
+    lp, ent, vals = torch.unsafe_split_with_sizes(buf, (rows, rows, rows * top))
+    rank, best = torch.unsafe_split_with_sizes(whole, (rows, rows * top))
+    return TokenLogprobs(lp, ent, rank, vals.view(rows, top), best.view(rows, top))
 
 
 __all__ = ["MAX_TOP", "TokenLogprobs", "token_logprobs"]
