@@ -16,15 +16,18 @@
 // none of them.  An item cut by a CTA boundary is joined from fp32 partials by
 // the CTA that finishes it last, in key order (results do not depend on timing).
 //
-// Bound: every code is read once, 2 D bytes per (key, kv head): HBM.  A warp
-// holds the next 16 keys' codes in registers while it works on the present
-// ones (32 lanes x 128 bytes), which with 16 warps keeps 64 KB in flight per
-// SM and needs no shared memory or barrier inside the loop.  The products run
-// as S^T = K Q^T and O^T = V^T P^T on m16n8k16: the keys (then the dims) are
-// the 16 rows, so 8 query columns fill an MMA, and both operands come straight
-// from the loaded words.  A dim may sit at any place of the contraction, so
-// each lane's 16-byte loads already are its A fragment of K; for V, words of
-// two keys are interleaved with one byte permute.
+// Bound: every code is read once, 2 D bytes per (key, kv head): HBM.  Each
+// warp copies its own 16-key tiles into a ring of its own in shared memory
+// (cp.async, 16 bytes a lane), two or more tiles ahead: some 128 KB in flight
+// per SM and no CTA barrier inside the loop.  The tiles are swizzled (16-byte
+// chunk ^= row mod 8) so that the fragments' 16-byte loads are free of bank
+// conflicts.  The products run as S^T = K Q^T and O^T = V^T P^T on m16n8k16:
+// the keys (then the dims) are the 16 rows, so 8 query columns fill an MMA.  A
+// dim may sit at any place of the contraction, so a lane's 16 bytes already
+// are its A fragment of K; for V, words of two keys are interleaved with one
+// byte permute.  Like the prompt kernel, a column's reference follows its
+// maximum only when that has grown by more than 2^8, so that the usual tile
+// needs no exchange between lanes and no rescaling.
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -36,7 +39,22 @@
 namespace exl3 {
 
 constexpr int kAttWarps = 8, kAttThreads = kAttWarps * 32, kAttUnit = 16 * kAttWarps;
-constexpr int kAttCtasPerSm = 2;
+constexpr float kAttSlack = 8.f;  // log2: growth of the maximum that is let pass
+
+// Tiles of 8 query columns an item has at most: up to two with two CTAs per
+// SM; three or four need the registers of one.
+template <int D, int NT>
+struct AttShape {
+    static constexpr int NC = 8 * NT;
+    static constexpr int kCtas = NT <= 2 ? 2 : 1;
+    static constexpr int kTile = 16 * D;                          // bytes of 16 keys of K, or of V
+    static constexpr int kStages = (NT <= 2 ? 3 : 6) * 128 / D;   // 96 KB of ring per CTA, 192 KB where it is alone
+    static constexpr int kRing = kAttWarps * kStages * 2 * kTile;
+    static constexpr int kRed = kAttWarps * NC * D * 4;           // the warps' outputs take the ring's place
+    static_assert(kRed <= kRing, "the ring holds the join");
+    static constexpr int kQ = NT * (D / 16) * 32 * 8;             // Q fragments
+    static constexpr int kSmem = kRing + kQ + (2 * kAttWarps * NC + 3 * NC) * 4 + kAttWarps * kStages * 8;
+};
 
 // Requests of more query columns (rows x heads per kv head) than this go to
 // the prompt kernel when the call has such requests at all.
@@ -62,16 +80,34 @@ __device__ __forceinline__ AttReq att_request(const KvAttendArgs& a, int b) {
     return r;
 }
 
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+
 template <bool E4M3, bool BF16, int D, int NT>
-__global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) kv_attend_kernel(const KvAttendArgs a) {
+__global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_attend_kernel(const KvAttendArgs a) {
+    using Shape = AttShape<D, NT>;
     constexpr int NC = 8 * NT;
     constexpr int KS = D / 16;  // contraction steps of S, row tiles of O
     constexpr int PART = NC * (D + 2);
-    extern __shared__ float att_smem[];
-    float* red = att_smem;                            // [warps][NC][D]
-    float* wm = red + kAttWarps * NC * D;             // [warps][NC] maxima, then factors
+    constexpr int S = Shape::kStages;
+    constexpr bool kQRegs = NT == 1;                  // Q fragments in registers, else read from shared memory
+    extern __shared__ __align__(128) char att_smem[];
+    float* red = reinterpret_cast<float*>(att_smem);  // [warps][NC][D], in the ring's place
+    uint2* qs = reinterpret_cast<uint2*>(att_smem + Shape::kRing);                    // [NT][KS][32]
+    float* wm = reinterpret_cast<float*>(att_smem + Shape::kRing + Shape::kQ);        // [warps][NC] maxima, then factors
     float* wl = wm + kAttWarps * NC;                  // [warps][NC] sums
     float* fin = wl + kAttWarps * NC;                 // [2][NC] joined maximum, sum
+    float* qfac = fin + 2 * NC;                       // [NC] factor of a column's scores
+    float2* tile_sc = reinterpret_cast<float2*>(qfac + NC);  // [warps][S] a tile's K and V scale
     __shared__ int64_t scan[kAttWarps];
     __shared__ int64_t found_base;
     __shared__ int found_b, last_flag;
@@ -146,54 +182,60 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) kv_attend_kernel(c
         const int64_t u_item = u - off;
         u += n_units;
 
-        // --- the query columns: B fragments of Q^T, and each column's key range ---
-        uint32_t qf[NT][KS][2];
-        float cfac[NT][2];           // columns 2c, 2c + 1: softmax scale (and Q's power of two)
-        int hi[NT][2], lo[NT][2];    // keys [lo, hi)
-        #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        // --- the query columns: B fragments of Q^T (a warp to each 8), and each column's key range ---
+        for (int t = warp; t < NT; t += kAttWarps) {
             const int n = 8 * t + g, f = cg * NC + n;
             const int64_t row = rq.row0 + f / G;
             const bool live = n < ncols && row < a.q_rows;
             const uint16_t* qp = a.q + (live ? row * a.q_tok + int64_t(hk * G + f % G) * a.q_head : 0);
             float fac = a.scale_log2;
-            float amax = 0.f;
+            uint2 w[KS];
             #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                const int dim = D == 128 ? (s >> 2) * 64 + c * 16 + (s & 3) * 4 : c * 16 + s * 4;
-                const uint2 w = live ? *reinterpret_cast<const uint2*>(qp + dim) : make_uint2(0u, 0u);
-                qf[t][s][0] = w.x, qf[t][s][1] = w.y;
-                if constexpr (BF16) {
-                    const uint32_t m = __vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
-                    amax = fmaxf(amax, fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u)));
-                }
+                // contraction step s takes word s % 4 of this lane's chunk of K
+                const int dim = (D == 128 ? (2 * c + (s >> 2)) * 16 : c * 16) + (s & 3) * 4;
+                w[s] = live ? *reinterpret_cast<const uint2*>(qp + dim) : make_uint2(0u, 0u);
             }
             if constexpr (BF16) {
                 // the tensor core takes Q in f16 like the codes: a power of two per row puts its
                 // largest magnitude in [2^14, 2^15), where f16 keeps all 8 bits of a bf16 value
                 // down to 2^-31 of that largest one
+                uint32_t m2 = 0;
+                #pragma unroll
+                for (int s = 0; s < KS; ++s) m2 = __vmaxu2(m2, __vmaxu2(w[s].x & 0x7fff7fffu, w[s].y & 0x7fff7fffu));
+                float amax = fmaxf(__uint_as_float(m2 << 16), __uint_as_float(m2 & 0xffff0000u));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 const int e = min(max((__float_as_int(amax) >> 23) - 127, -100), 100);
                 const float mul = exp2_int(14 - e);
                 fac *= exp2_int(e - 14);
+                auto conv = [&](uint32_t v) { return pack_half2(__uint_as_float(v << 16) * mul, __uint_as_float(v & 0xffff0000u) * mul); };
                 #pragma unroll
-                for (int s = 0; s < KS; ++s)
-                    #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t w = qf[t][s][i];
-                        qf[t][s][i] = pack_half2(__uint_as_float(w << 16) * mul, __uint_as_float(w & 0xffff0000u) * mul);
-                    }
+                for (int s = 0; s < KS; ++s) w[s] = make_uint2(conv(w[s].x), conv(w[s].y));
             }
             #pragma unroll
+            for (int s = 0; s < KS; ++s) qs[(t * KS + s) * 32 + lane] = w[s];
+            if (c == 0) qfac[8 * t + g] = fac;
+        }
+        __syncthreads();
+        uint2 qf[kQRegs ? NT : 1][KS];
+        if constexpr (kQRegs) {
+            #pragma unroll
+            for (int t = 0; t < NT; ++t)
+                #pragma unroll
+                for (int s = 0; s < KS; ++s) qf[t][s] = qs[(t * KS + s) * 32 + lane];
+        }
+        float cfac[NT][2];           // columns 2c, 2c + 1
+        int hi[NT][2], lo[NT][2];    // keys [lo, hi)
+        #pragma unroll
+        for (int t = 0; t < NT; ++t)
+            #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int col = 2 * c + i, fc = cg * NC + 8 * t + col;
-                cfac[t][i] = __shfl_sync(0xffffffffu, fac, 4 * col);
-                const int pos = rq.len - rq.fresh + fc / G;
-                hi[t][i] = 8 * t + col < ncols ? min(pos + 1, rq.len) : 0;
+                const int col = 8 * t + 2 * c + i, pos = rq.len - rq.fresh + (cg * NC + col) / G;
+                cfac[t][i] = qfac[col];
+                hi[t][i] = col < ncols ? min(pos + 1, rq.len) : 0;
                 lo[t][i] = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
             }
-        }
         int full_lo = 0, full_hi = 0x7fffffff;  // keys in [full_lo, full_hi) need no test
         #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -220,98 +262,139 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) kv_attend_kernel(c
         const int first = rq.lo16 + off * kAttUnit + warp * 16;
         const int end = min(rq.len, rq.lo16 + (off + n_units) * kAttUnit);
         const int32_t* row_table = a.table + int64_t(b) * a.width;
-        auto page_at = [&](int tok) { return tok < end ? row_table[tok >> a.shift] : 0; };
+        auto page_at = [&](int tok) { return tok < end ? __ldg(row_table + (tok >> a.shift)) : -1; };
 
-        // codes of 16 keys: K rows g and g + 8, V rows 2c, 2c + 1, 2c + 8, 2c + 9
-        uint4 kr[2][D / 64];
-        uint32_t vr[4][D / 32];
-        float ks = 0.f, vs = 0.f;
-        bool got = false;  // the tile's page exists
-        auto load_k = [&](int tok, int page) {
-            got = tok < end && page >= 0 && page < a.pages;
-            if (tok < end && !got && lane == 0) set_status(a.status, DEV_BAD_INDEX);
-            const int64_t tile = int64_t(got ? page : 0) * Hk + hk;
-            ks = got ? a.k_scale[tile] : 0.f;
-            vs = got ? a.v_scale[tile] : 1.f;
-            const uint8_t* p = a.k + ((tile << a.shift) + (tok & (P - 1)) + g) * D + c * 16;
-            #pragma unroll
-            for (int i = 0; i < 2; ++i)
+        const uint32_t ring = smem_u32(att_smem) + warp * (S * 2 * Shape::kTile);
+        const uint32_t ring_sc = smem_u32(tile_sc) + warp * (S * 8);
+        // where chunk lane (+ 32, + 64, ...) of a tile goes: 16-byte chunk ^= row mod 8 (rows of 64 bytes: row / 2 mod 4)
+        constexpr int CH = D / 16;
+        const int cr = lane / CH, cc = lane % CH;
+        auto fetch = [&](int tok, int page, int stage) {
+            const bool get = tok < end && page >= 0 && page < a.pages;
+            if (get) {
+                const int64_t tile = int64_t(page) * Hk + hk;
+                const int64_t at = ((tile << a.shift) + (tok & (P - 1))) * D + lane * 16;
+                const uint32_t dst = ring + stage * (2 * Shape::kTile);
                 #pragma unroll
-                for (int h = 0; h < D / 64; ++h)
-                    kr[i][h] = got ? __ldg(reinterpret_cast<const uint4*>(p + i * 8 * D + h * 64)) : make_uint4(0, 0, 0, 0);
-        };
-        auto load_v = [&](int tok, int page, bool ok) {
-            const int64_t tile = int64_t(ok ? page : 0) * Hk + hk;
-            const uint8_t* p = a.v + ((tile << a.shift) + (tok & (P - 1)) + 2 * c) * D + g * (D / 8);
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint8_t* r = p + ((i & 1) + (i >> 1) * 8) * D;
-                if constexpr (D == 128) {
-                    const uint4 w = ok ? __ldg(reinterpret_cast<const uint4*>(r)) : make_uint4(0, 0, 0, 0);
-                    vr[i][0] = w.x, vr[i][1] = w.y, vr[i][2] = w.z, vr[i][3] = w.w;
-                } else {
-                    const uint2 w = ok ? __ldg(reinterpret_cast<const uint2*>(r)) : make_uint2(0, 0);
-                    vr[i][0] = w.x, vr[i][1] = w.y;
+                for (int i = 0; i < CH / 2; ++i) {
+                    const int row = cr + i * (32 / CH);
+                    const uint32_t to = dst + row * D + ((cc ^ (D == 128 ? row & 7 : (row >> 1) & 3)) << 4);
+                    copy_async16(to, a.k + at + i * 512);
+                    copy_async16(to + Shape::kTile, a.v + at + i * 512);
                 }
+                if (lane < 2) copy_async4(ring_sc + stage * 8 + lane * 4, (lane ? a.v_scale : a.k_scale) + tile);
+            } else if (tok < end && lane == 0) {
+                set_status(a.status, DEV_BAD_INDEX);
             }
+            copy_commit();
+            return get;
         };
-        int page = page_at(first), page_next = page_at(first + kAttUnit);
-        load_k(first, page);
-        load_v(first, page, got);
-
+        // this warp's tiles: first, first + kAttUnit, ...; S - 1 of them are on their way
+        uint32_t have = 0;  // bit i: tile (present + i) exists
+        {
+            int ahead[S - 1];
+            #pragma unroll
+            for (int i = 0; i < S - 1; ++i) ahead[i] = page_at(first + i * kAttUnit);
+            #pragma unroll
+            for (int i = 0; i < S - 1; ++i) have |= uint32_t(fetch(first + i * kAttUnit, ahead[i], i)) << i;
+        }
+        int page_next = page_at(first + (S - 1) * kAttUnit);
+        int stage = 0;
         for (int tok = first; tok < end; tok += kAttUnit) {
-            // --- S^T = K Q^T ---
+            copy_wait<S - 2>();
+            __syncwarp();  // the tile is here, for all lanes, and the one before it is done with
+            {
+                const int page = page_next, t = tok + (S - 1) * kAttUnit;
+                page_next = page_at(t + kAttUnit);
+                have |= uint32_t(fetch(t, page, stage == 0 ? S - 1 : stage - 1)) << (S - 1);
+            }
+            const bool here = have & 1u;
+            have >>= 1;
+            const char* kt = att_smem + warp * (S * 2 * Shape::kTile) + stage * (2 * Shape::kTile);
+            const char* vt = kt + Shape::kTile;
+            const float2 sc = tile_sc[warp * S + stage];
+            stage = stage == S - 1 ? 0 : stage + 1;
+            if (!here) continue;
+
+            // --- S^T = K Q^T: keys g and g + 8 ---
             float s[NT][4];
             #pragma unroll
             for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
             #pragma unroll
-            for (int st = 0; st < KS; ++st) {
-                auto word = [&](const uint4& q4) {
-                    return code_word<E4M3>((st & 3) == 0 ? q4.x : (st & 3) == 1 ? q4.y : (st & 3) == 2 ? q4.z : q4.w);
-                };
-                const uint32_t w0 = word(kr[0][D == 128 ? st >> 2 : 0]), w1 = word(kr[1][D == 128 ? st >> 2 : 0]);
-                const uint32_t af[4] = {half2_lo<E4M3>(w0), half2_lo<E4M3>(w1), half2_hi<E4M3>(w0), half2_hi<E4M3>(w1)};
+            for (int h = 0; h < D / 64; ++h) {
+                const int sw = D == 128 ? ((2 * c + h) ^ (g & 7)) << 4 : (c ^ ((g >> 1) & 3)) << 4;
+                const uint4 x = *reinterpret_cast<const uint4*>(kt + g * D + sw);
+                const uint4 y = *reinterpret_cast<const uint4*>(kt + (g + 8) * D + sw);
                 #pragma unroll
-                for (int t = 0; t < NT; ++t) mma_16816(s[t], af, qf[t][st][0], qf[t][st][1]);
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t w0 = code_word<E4M3>(q == 0 ? x.x : q == 1 ? x.y : q == 2 ? x.z : x.w);
+                    const uint32_t w1 = code_word<E4M3>(q == 0 ? y.x : q == 1 ? y.y : q == 2 ? y.z : y.w);
+                    const uint32_t af[4] = {half2_lo<E4M3>(w0), half2_lo<E4M3>(w1), half2_hi<E4M3>(w0), half2_hi<E4M3>(w1)};
+                    #pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const uint2 bq = kQRegs ? qf[kQRegs ? t : 0][4 * h + q] : qs[(t * KS + 4 * h + q) * 32 + lane];
+                        mma_16816(s[t], af, bq.x, bq.y);
+                    }
+                }
             }
-            const bool have = got;
-            const float kscale = ks;
-            const int ve = stored_exponent(vs);
-            page = page_next;
-            page_next = page_at(tok + 2 * kAttUnit);
-            load_k(tok + kAttUnit, page);
+            // V: keys 2c, 2c + 1, 2c + 8, 2c + 9, dims g * D / 8 and on
+            uint32_t vr[4][D / 32];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 2 * c + (i & 1) + (i >> 1) * 8;
+                if constexpr (D == 128) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(vt + row * D + ((g ^ (row & 7)) << 4));
+                    vr[i][0] = w.x, vr[i][1] = w.y, vr[i][2] = w.z, vr[i][3] = w.w;
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(vt + row * D + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
+                    vr[i][0] = w.x, vr[i][1] = w.y;
+                }
+            }
 
-            // --- softmax over these 16 keys ---
-            const bool edge = tok < full_lo || tok + 16 > full_hi || !have;
+            // --- weights of these 16 keys ---
+            const int ve = stored_exponent(sc.y);
             const float vexp = float(ve), vinv = exp2_int(-ve);
-            uint32_t pf[NT][2];
+            const bool edge = tok < full_lo || tok + 16 > full_hi;
+            bool grown = false;
             #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[t][i] = fmaf(s[t][i], cfac[t][i & 1] * kscale, vexp);
+                for (int i = 0; i < 4; ++i) s[t][i] = fmaf(s[t][i], cfac[t][i & 1] * sc.x, vexp);
                 if (edge) {
                     #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int key = tok + g + 8 * (i >> 1);
-                        if (!have || key >= hi[t][i & 1] || key < lo[t][i & 1]) s[t][i] = -INFINITY;
+                        if (key >= hi[t][i & 1] || key < lo[t][i & 1]) s[t][i] = -INFINITY;
                     }
                 }
-                float p[4];
                 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float mx = fmaxf(s[t][i], s[t][i + 2]);
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const float mn = fmaxf(m[t][i], mx), ref = mn == -INFINITY ? 0.f : mn;
-                    const float alpha = ex2(m[t][i] - ref);  // 0 while nothing has been seen
-                    m[t][i] = mn;
-                    p[i] = ex2(s[t][i] - ref), p[i + 2] = ex2(s[t][i + 2] - ref);
-                    l[t][i] = fmaf(l[t][i], alpha, (p[i] + p[i + 2]) * vinv);
-                    if (__any_sync(0xffffffffu, alpha != 1.f)) {
+                for (int i = 0; i < 2; ++i) grown |= fmaxf(s[t][i], s[t][i + 2]) > m[t][i] + kAttSlack;
+            }
+            if (__any_sync(0xffffffffu, grown)) {  // -inf + slack is -inf: the first key that is seen counts as growth
+                #pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    #pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float mx = fmaxf(m[t][i], fmaxf(s[t][i], s[t][i + 2]));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        const float alpha = mx == m[t][i] ? 1.f : ex2(m[t][i] - mx);  // 0 where nothing has been seen
+                        m[t][i] = mx;
+                        l[t][i] *= alpha;
                         #pragma unroll
                         for (int j = 0; j < KS; ++j) o[t][j][i] *= alpha, o[t][j][i + 2] *= alpha;
                     }
+            }
+            uint32_t pf[NT][2];
+            #pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float p[4];
+                #pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float ref = m[t][i] == -INFINITY ? 0.f : m[t][i];
+                    p[i] = ex2(s[t][i] - ref), p[i + 2] = ex2(s[t][i + 2] - ref);
+                    l[t][i] = fmaf(p[i] + p[i + 2], vinv, l[t][i]);
                 }
                 pf[t][0] = transpose8x8(pack_half2(p[0], p[1]));
                 pf[t][1] = transpose8x8(pack_half2(p[2], p[3]));
@@ -338,8 +421,9 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) kv_attend_kernel(c
                     for (int t = 0; t < NT; ++t) mma_16816(o[t][2 * w + h], af, pf[t][0], pf[t][1]);
                 }
             }
-            load_v(tok + kAttUnit, page, got);
         }
+        copy_wait<0>();
+        __syncthreads();  // the ring is free
 
         // --- join the warps ---
         #pragma unroll
@@ -429,13 +513,17 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) kv_attend_kernel(c
     }
 }
 
-// counters: one per CTA of the kernel here, one per item of a split prompt (fewer than SMs)
-int kv_attend_counters(int sms) { return sms * (kAttCtasPerSm + 1); }
+// counters: one per CTA of the kernel here (two per SM), one per item of a split prompt (fewer than SMs)
+int kv_attend_counters(int sms) { return sms * 3; }
 
 static int64_t att_columns(const KvAttendCall& c) { return int64_t(c.max_new) * (c.heads / c.kv_heads); }
-static int att_tiles(const KvAttendCall& c) { return att_columns(c) > 8 ? 2 : 1; }
+static int att_tiles(const KvAttendCall& c) {
+    const int64_t n = (att_columns(c) + 7) / 8;
+    return int(n < 4 ? n : 4);
+}
 static size_t att_bytes(const KvAttendCall& c, int sms) {
-    return size_t(sms) * kAttCtasPerSm * 2 * (8 * att_tiles(c)) * (c.dim + 2) * 4;
+    const int nt = att_tiles(c);
+    return size_t(sms) * (nt <= 2 ? 2 : 1) * 2 * (8 * nt) * (c.dim + 2) * 4;
 }
 
 size_t kv_attend_workspace(const KvAttendCall& c, int sms) {
@@ -444,13 +532,12 @@ size_t kv_attend_workspace(const KvAttendCall& c, int sms) {
 
 template <bool E4M3, bool BF16, int D, int NT>
 static cudaError_t launch_attend(const KvAttendArgs& a, int sms, cudaStream_t s) {
-    constexpr int NC = 8 * NT;
-    const size_t smem = size_t(kAttWarps * NC * (D + 2) + 2 * NC) * 4;
+    using Shape = AttShape<D, NT>;
     auto* kernel = kv_attend_kernel<E4M3, BF16, D, NT>;
     static std::atomic<uint64_t> done{0};
-    const cudaError_t e = raise_smem(kernel, smem, done);
+    const cudaError_t e = raise_smem(kernel, Shape::kSmem, done);
     if (e != cudaSuccess) return e;
-    kernel<<<sms * kAttCtasPerSm, kAttThreads, smem, s>>>(a);
+    kernel<<<sms * Shape::kCtas, kAttThreads, Shape::kSmem, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -469,16 +556,20 @@ cudaError_t run_kv_attend(const KvAttendCall& c, int sms, cudaStream_t s) {
     if (att_columns(c) > kAttFew) {
         a.few = kAttFew;
         KvAttendArgs p = a;
-        p.counters = c.counters + sms * kAttCtasPerSm;
+        p.counters = c.counters + sms * 2;
         p.part = reinterpret_cast<float*>(c.ws + att_bytes(c, sms));
         const cudaError_t e = run_kv_prompt(c, p, kv_prompt_plan(c, sms), s);
         if (e != cudaSuccess) return e;
     }
-    const bool bf16 = c.x_dtype == DT_BF16, wide = att_tiles(c) == 2, d128 = c.dim == 128;
+    const bool bf16 = c.x_dtype == DT_BF16, d128 = c.dim == 128;
+    const int nt = att_tiles(c);
     const auto pick = [&](auto e4, auto bf, auto dim) {
         constexpr bool E = decltype(e4)::value, B = decltype(bf)::value;
         constexpr int Dm = decltype(dim)::value;
-        return wide ? launch_attend<E, B, Dm, 2>(a, sms, s) : launch_attend<E, B, Dm, 1>(a, sms, s);
+        return nt == 1   ? launch_attend<E, B, Dm, 1>(a, sms, s)
+               : nt == 2 ? launch_attend<E, B, Dm, 2>(a, sms, s)
+               : nt == 3 ? launch_attend<E, B, Dm, 3>(a, sms, s)
+                         : launch_attend<E, B, Dm, 4>(a, sms, s);
     };
     const auto by_dim = [&](auto e4, auto bf) {
         return d128 ? pick(e4, bf, std::integral_constant<int, 128>()) : pick(e4, bf, std::integral_constant<int, 64>());
