@@ -610,6 +610,8 @@ static int check_cache(const char* who, const void* k, const void* v, const floa
     return EXL3_OK;
 }
 
+static_assert(exl3::kKvMaxRequests == EXL3_KV_MAX_REQUESTS, "one limit");
+
 // status word, counters and partial results of a serving workspace
 static constexpr size_t kServeCounters = 256;
 static size_t serve_partials(int n_counters) { return (kServeCounters + size_t(n_counters) * 4 + 255) & ~size_t(255); }
@@ -680,8 +682,8 @@ int exl3_kv_attend(const exl3_kv_attend_args* a, void* stream) {
         return fail(EXL3_ERR_ARG, "%s: heads (%lld) must be a multiple of kv_heads (%lld)", who, (long long)a->heads, (long long)a->kv_heads);
     if (a->heads > 65535) return fail(EXL3_ERR_ARG, "%s: heads must be at most 65535", who);
     if (a->q_rows < 0 || a->q_rows > INT32_MAX / a->heads) return fail(EXL3_ERR_ARG, "%s: q rows x heads must be in 0..2^31-1", who);
-    if (a->requests < 0 || a->requests > INT32_MAX || a->width < 0)
-        return fail(EXL3_ERR_ARG, "%s: requests and table width must be >= 0", who);
+    if (a->requests < 0 || a->requests > EXL3_KV_MAX_REQUESTS || a->width < 0)
+        return fail(EXL3_ERR_ARG, "%s: requests must be in 0..%d and the table width >= 0", who, EXL3_KV_MAX_REQUESTS);
     if (a->width > INT32_MAX / a->page) return fail(EXL3_ERR_ARG, "%s: the table holds more than 2^31-1 tokens", who);
     if (a->max_new < 1 || a->max_new > INT32_MAX) return fail(EXL3_ERR_ARG, "%s: max_new must be >= 1", who);
     if (!a->cu_tokens && (a->max_new != 1 || a->q_rows != a->requests))

@@ -200,6 +200,8 @@ cudaError_t run_ngram(const uint16_t* rows, int64_t n, int64_t n_rows, int bits,
 // pages hold 1 << page_shift(page) tokens; page is 16, 32, 64 or 128
 inline int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
 
+constexpr int kKvMaxRequests = 16384;  // EXL3_KV_MAX_REQUESTS: their sums fit shared memory
+
 struct KvPlanCall {
     const int32_t *lens = nullptr, *fresh = nullptr;  // [requests] cached and new tokens
     int requests = 0;

@@ -513,8 +513,8 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
     }
 }
 
-// counters: one per CTA of the kernel here (two per SM), one per item of a split prompt (fewer than SMs)
-int kv_attend_counters(int sms) { return sms * 3; }
+// counters: one per CTA of the kernel here, two per CTA of the prompt kernel
+int kv_attend_counters(int sms) { return sms * 4; }
 
 static int64_t att_columns(const KvAttendCall& c) { return int64_t(c.max_new) * (c.heads / c.kv_heads); }
 static int att_tiles(const KvAttendCall& c) {
@@ -527,7 +527,7 @@ static size_t att_bytes(const KvAttendCall& c, int sms) {
 }
 
 size_t kv_attend_workspace(const KvAttendCall& c, int sms) {
-    return att_bytes(c, sms) + (att_columns(c) > kAttFew ? kv_prompt_plan(c, sms).bytes : 0);
+    return att_bytes(c, sms) + (att_columns(c) > kAttFew ? kv_prompt_bytes(c, sms) : 0);
 }
 
 template <bool E4M3, bool BF16, int D, int NT>
@@ -558,7 +558,7 @@ cudaError_t run_kv_attend(const KvAttendCall& c, int sms, cudaStream_t s) {
         KvAttendArgs p = a;
         p.counters = c.counters + sms * 2;
         p.part = reinterpret_cast<float*>(c.ws + att_bytes(c, sms));
-        const cudaError_t e = run_kv_prompt(c, p, kv_prompt_plan(c, sms), s);
+        const cudaError_t e = run_kv_prompt(c, p, sms, s);
         if (e != cudaSuccess) return e;
     }
     const bool bf16 = c.x_dtype == DT_BF16, d128 = c.dim == 128;

@@ -65,12 +65,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 }
 
 // kv_prompt.cu: requests with more than `few` query columns
-struct KvPromptPlan {
-    int64_t tiles;  // at most: 256-column tiles of all requests
-    int splits;     // at most: parts of a tile's keys
-    size_t bytes;   // workspace for partial results
-};
-KvPromptPlan kv_prompt_plan(const KvAttendCall& c, int sms);
-cudaError_t run_kv_prompt(const KvAttendCall& c, const KvAttendArgs& a, const KvPromptPlan& p, cudaStream_t s);
+size_t kv_prompt_bytes(const KvAttendCall& c, int sms);  // of its partial results
+cudaError_t run_kv_prompt(const KvAttendCall& c, const KvAttendArgs& a, int sms, cudaStream_t s);
 
 }  // namespace exl3

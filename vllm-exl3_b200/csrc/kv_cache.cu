@@ -29,7 +29,6 @@
 namespace exl3 {
 
 constexpr int kPlanThreads = 512;
-constexpr int kKvMaxRequests = 16384;  // EXL3_KV_MAX_REQUESTS: their sums fit shared memory
 
 struct KvPlanArgs {
     const int32_t *lens, *fresh;  // [B]

@@ -12,13 +12,20 @@
 //   0-3, 4-7  one row per thread: running maximum, weights, sums (tiles 0 and 1)
 //   8-11      codes of 128 keys from global memory to f16 in shared memory
 //             (128-byte swizzle; K is a K-major operand, V an MN-major one: the same bytes)
+//   13        pages and scales of the steps to come, four steps at a time, into a ring
 //   12        an elected lane issues S = Q K^T and O += P V (tcgen05, fp32 in TMEM)
-//   13-15     leave at once: they make up the warpgroup whose registers the first eight warps take
+//   14-15     idle: they make up the warpgroup whose registers the first eight warps take
 //             (184 a thread: a row's 128 scores are read from TMEM once and stay in registers)
 // TMEM: S0 S1 (128 columns each; the weights, f16, take the place of the
 // scores that they came from and are the A operand of P V), O0 O1.
 // The order of the issue S0 S1 | PV0 S0' PV1 S1' | ... keeps one tile's
 // products behind the other's weights; tcgen05 runs one thread's products in order.
+//
+// Work: an item is (request, 256 rows, kv head), its steps are the 128-key
+// blocks that its rows see; all items' steps form one line that the CTAs, one
+// per SM, split evenly, whatever the lengths and the causal mask.  An item cut
+// by a CTA boundary is joined from fp32 partials by the CTA that finishes it
+// last, in key order.
 //
 // O is rescaled only when a row's maximum grows by more than 2^8 over the
 // reference its weights are taken against: until then weights up to 2^8 (f16
@@ -38,26 +45,41 @@ namespace exl3 {
 constexpr int kPrThreads = 16 * 32;
 constexpr int kPrKeys = 128;        // keys per step
 constexpr int kPrRows = 256;        // query rows per CTA
-constexpr int kPrScaleSlots = 4;
-constexpr int kPrMaxSplits = 64;    // weights of the parts fit shared memory
+constexpr int kPrSlots = 8;         // steps whose pages and scales are kept
 constexpr float kPrSlack = 8.f;     // log2: growth of the maximum that is let pass
+constexpr int kPrLeast = 4;         // steps a CTA takes at least: joining costs more than they do
 constexpr uint32_t kPrTmem = 512;
 
+// pages and scales of a step
+struct PrStep {
+    float4 sc[8];  // of 16 keys: K scale, log2 V scale, 1 / V scale, 1 if the page exists
+    int page[8];   // of 16 keys, -1: not seen, or no such page
+    int from, to;  // the keys of the step that any row sees
+    int hk, pad;
+};
+
 struct PrSmem {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], sc_full[kPrScaleSlots];
+    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
+    uint64_t step_full[kPrSlots], step_free[kPrSlots];
+    uint64_t join[2];  // of a tile's rows among themselves
+    uint64_t done;
     uint32_t tmem;
-    int abort_flag, last;
+    int abort_flag, last[2];
     int64_t scan[kPrThreads / 32];
-    int found_b;
+    int found_b, found_tile;
     int64_t found_base;
-    float4 sc[kPrScaleSlots][8];  // of 16 keys: K scale, log2 V scale, 1 / V scale, 1 if the page exists
-    float wt[kPrRows];
+    PrStep step[kPrSlots];
 };
 
 template <int D>
 constexpr size_t pr_smem_bytes() {
     return 1024 + size_t(kPrRows) * D * 2 + 4 * size_t(kPrKeys) * D * 2 + sizeof(PrSmem);
 }
+static_assert((4 * kPrKeys + kPrRows) * 64 * 2 >= (kKvMaxRequests + 1) * 4, "the tile sums fit the place of the operands");
+
+// fp32 partial of one 128-row tile: {reference, sum} per row, then O in 16-byte pieces, rows side by side
+template <int D>
+__host__ __device__ constexpr int pr_part() { return 128 * (D + 2); }
 
 __device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, int* status, volatile int* abort_flag) {
     if (*abort_flag) return false;
@@ -65,6 +87,57 @@ __device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, int* sta
     *abort_flag = 1;
     return false;
 }
+
+__device__ __forceinline__ int64_t pr_columns(const KvAttendArgs& a, int b) {
+    return int64_t(a.cu ? max(a.cu[b + 1] - a.cu[b], 0) : 1) * a.group;
+}
+__device__ __forceinline__ int pr_tiles(const KvAttendArgs& a, int b) {
+    const int64_t cols = pr_columns(a, b);
+    return cols > a.few ? int((cols + kPrRows - 1) / kPrRows) : 0;
+}
+
+// 256 rows of a request and the keys that any of them sees
+struct PrTile {
+    int64_t row0, col0;
+    int fresh, len, rows, lo, hi, k_begin, steps;
+};
+__device__ __forceinline__ PrTile pr_tile(const KvAttendArgs& a, int b, int tile) {
+    PrTile t;
+    t.row0 = a.cu ? a.cu[b] : b;
+    t.fresh = a.cu ? a.cu[b + 1] - int(t.row0) : 1;
+    t.len = int(min(int64_t(max(a.kv_lens[b], 0)), int64_t(a.width) << a.shift));
+    t.col0 = int64_t(tile) * kPrRows;
+    t.rows = int(min(int64_t(t.fresh) * a.group - t.col0, int64_t(kPrRows)));
+    const int first = t.len - t.fresh + int(t.col0 / a.group), last = t.len - t.fresh + int((t.col0 + t.rows - 1) / a.group);
+    t.hi = max(min(last + 1, t.len), 0);
+    t.lo = min(a.window > 0 ? max(first + 1 - a.window, 0) : 0, t.hi);
+    t.k_begin = t.lo & ~(kPrKeys - 1);
+    t.steps = max((t.hi - t.k_begin + kPrKeys - 1) / kPrKeys, 1);  // rows that see nothing take one step too
+    return t;
+}
+
+// A place on the line of steps, ordered by request, tile, kv head, keys
+struct PrWalk {
+    int64_t base;  // of the tile's first step
+    int b, tile, tiles;
+    PrTile t;
+    __device__ __forceinline__ void start(const KvAttendArgs& a, const PrSmem& sm) {
+        base = sm.found_base, b = sm.found_b, tile = sm.found_tile;
+        tiles = pr_tiles(a, b);
+        t = pr_tile(a, b, tile);
+    }
+    __device__ __forceinline__ void seek(const KvAttendArgs& a, int64_t u) {  // forwards, to a step below the total
+        while (u >= base + int64_t(a.kv_heads) * t.steps) {
+            base += int64_t(a.kv_heads) * t.steps;
+            if (++tile >= tiles) {
+                do tiles = pr_tiles(a, ++b);
+                while (tiles == 0);
+                tile = 0;
+            }
+            t = pr_tile(a, b, tile);
+        }
+    }
+};
 
 // MN-major operand, 128-byte swizzle: 64-element (128-byte) rows along MN, one
 // per k; 8 k to an atom (SBO 1024); the next 64 of MN are `lbo` bytes on.
@@ -147,16 +220,10 @@ __device__ __forceinline__ uint2 load_early(const uint8_t* p, bool get) {
     return v;
 }
 
-struct PrArgs {
-    KvAttendArgs a;
-    int splits;  // parts of a tile's keys (at most; no more than its steps)
-};
-
 template <bool E4M3, bool BF16, int D>
-__global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs args) {
+__global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttendArgs a) {
     constexpr int kBlk = kPrKeys * 128;        // bytes of a 64-dim block of 128 rows
     constexpr int kTile = (D / 64) * kBlk;     // a 128-row f16 tile
-    const KvAttendArgs& a = args.a;
     extern __shared__ char pr_raw[];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(pr_raw) + 1023) & ~uintptr_t(1023));
     char* vst = smem;              // 2 stages
@@ -168,67 +235,76 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // warp: uniform
     const int Hk = a.kv_heads, G = a.group, P = 1 << a.shift;
 
-    // --- which tile ---
-    auto tiles_of = [&](int b) {
-        const int64_t cols = int64_t(a.cu ? max(a.cu[b + 1] - a.cu[b], 0) : 1) * G;
-        return cols > a.few ? (cols + kPrRows - 1) / kPrRows : int64_t(0);
-    };
-    const int64_t item = blockIdx.x / args.splits;
-    const int split = int(blockIdx.x % args.splits);
-    int b = 0;
-    int64_t tile = item / Hk;
-    const int hk = int(item % Hk);
-    {
-        const int per = (a.requests + kPrThreads - 1) / kPrThreads;
-        int64_t mine = 0;
-        for (int i = 0; i < per; ++i)
-            if (tid * per + i < a.requests) mine += tiles_of(tid * per + i);
-        int64_t incl = mine;
+    // --- this CTA's share of the line of steps ---
+    // Block-wide sum of one value per thread; returns the sum of the threads up to and with this one
+    auto scan = [&](int64_t v, int64_t& total) {
         #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int64_t o = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += o;
+            const int64_t o = __shfl_up_sync(0xffffffffu, v, d);
+            if (lane >= d) v += o;
         }
-        if (lane == 31) sm.scan[warp] = incl;
+        if (lane == 31) sm.scan[warp] = v;
         __syncthreads();
-        int64_t total = 0;
+        total = 0;
         for (int w = 0; w < kPrThreads / 32; ++w) {
-            if (w == warp) incl += total;
+            if (w == warp) v += total;
             total += sm.scan[w];
         }
-        if (tile >= total) return;  // the grid covers the most tiles there could be
-        tile = total - 1 - tile;    // a request's last rows, whose keys are the most, first
-        if (tile >= incl - mine && tile < incl) {
-            int64_t base = incl - mine;
-            int i = tid * per;
-            for (int64_t n; tile >= base + (n = tiles_of(i)); ++i) base += n;
-            sm.found_b = i, sm.found_base = base;
-        }
         __syncthreads();
-        b = sm.found_b;
-        tile -= sm.found_base;
+        return v;
+    };
+    int32_t* sums = reinterpret_cast<int32_t*>(smem);  // [requests + 1] tiles of the requests before; the operands come later
+    {
+        const int per = (a.requests + kPrThreads - 1) / kPrThreads;
+        int64_t mine = 0, n_tiles, total;
+        for (int i = 0; i < per; ++i)
+            if (tid * per + i < a.requests) mine += pr_tiles(a, tid * per + i);
+        int64_t at = scan(mine, n_tiles) - mine;
+        for (int i = 0; i < per; ++i)
+            if (tid * per + i < a.requests) {
+                sums[tid * per + i] = int32_t(at);
+                at += pr_tiles(a, tid * per + i);
+            }
+        if (tid == 0) sums[a.requests] = int32_t(n_tiles);
+        __syncthreads();
+        const int each = int((n_tiles + kPrThreads - 1) / kPrThreads);
+        const int64_t t0 = int64_t(tid) * each, t1 = min(t0 + each, n_tiles);
+        auto request = [&](int64_t t) {  // of tile t: the last b with sums[b] <= t
+            int lo = 0, hi = a.requests;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (sums[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            return lo;
+        };
+        mine = 0;
+        for (int64_t t = t0; t < t1; ++t) {
+            const int b = request(t);
+            mine += int64_t(Hk) * pr_tile(a, b, int(t - sums[b])).steps;
+        }
+        const int64_t end = scan(mine, total);
+        const int64_t want = (total + kPrLeast - 1) / kPrLeast;
+        const int ctas = int(min(int64_t(gridDim.x), want));
+        if (int(blockIdx.x) >= ctas) return;
+        const int64_t u0 = total * blockIdx.x / ctas;
+        if (u0 >= end - mine && u0 < end) {
+            int64_t base = end - mine, t = t0;
+            for (;; ++t) {
+                const int b = request(t);
+                const int64_t n = int64_t(Hk) * pr_tile(a, b, int(t - sums[b])).steps;
+                if (u0 < base + n) {
+                    sm.found_b = b, sm.found_tile = int(t - sums[b]), sm.found_base = base;
+                    break;
+                }
+                base += n;
+            }
+        }
+        if (tid == 0) sm.scan[0] = total;
     }
-    const int64_t row0 = a.cu ? a.cu[b] : b;
-    const int fresh = a.cu ? a.cu[b + 1] - int(row0) : 1;
-    const int len = int(min(int64_t(max(a.kv_lens[b], 0)), int64_t(a.width) << a.shift));
-    const int64_t col0 = tile * kPrRows;
-    const int rows = int(min(int64_t(fresh) * G - col0, int64_t(kPrRows)));
-    const int nt = rows > 128 ? 2 : 1;
-    // keys that any row of the tile sees
-    const int pos_first = len - fresh + int(col0 / G), pos_last = len - fresh + int((col0 + rows - 1) / G);
-    const int hi_all = max(min(pos_last + 1, len), 0);
-    const int lo_all = a.window > 0 ? max(pos_first + 1 - a.window, 0) : 0;
-    const int k_begin = min(lo_all, hi_all) & ~(kPrKeys - 1);
-    const int steps_all = (hi_all - k_begin + kPrKeys - 1) / kPrKeys;
-    const int ns = max(min(args.splits, steps_all), 1);
-    if (split >= ns) return;
-    const int step0 = int(int64_t(steps_all) * split / ns);
-    const int steps = int(int64_t(steps_all) * (split + 1) / ns) - step0;
-    const int key0 = k_begin + step0 * kPrKeys;
-
     if (tid == 0) {
-        mbar_init(&sm.q_full, 128 * nt);
         for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.q_full[i], 128);
             mbar_init(&sm.k_full[i], 4);
             mbar_init(&sm.v_full[i], 4);
             mbar_init(&sm.k_empty[i], 1);
@@ -236,8 +312,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
             mbar_init(&sm.s_full[i], 1);
             mbar_init(&sm.o_full[i], 1);
             mbar_init(&sm.p_full[i], 128);
+            mbar_init(&sm.join[i], 128);
         }
-        for (int i = 0; i < kPrScaleSlots; ++i) mbar_init(&sm.sc_full[i], 1);
+        for (int i = 0; i < kPrSlots; ++i) {
+            mbar_init(&sm.step_full[i], 1);
+            mbar_init(&sm.step_free[i], 4);
+        }
+        mbar_init(&sm.done, 1);
         sm.abort_flag = 0;
         mbar_fence_init();
     }
@@ -246,35 +327,51 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
     __syncthreads();
     tc_fence_after();
     const uint32_t tm = __shfl_sync(0xffffffffu, sm.tmem, 0);
-    // columns: S0 0, S1 128, O0 256, O1 384.  Registers: 512 x 128 at launch = 256 x 184 + 128 x 96 + 128 x 48
+    const int64_t total = sm.scan[0];
+    const int ctas = int(min(int64_t(gridDim.x), (total + kPrLeast - 1) / kPrLeast)), cta = blockIdx.x;
+    const int64_t u0 = total * cta / ctas, u1 = total * (cta + 1) / ctas;
+    // TMEM columns: S0 0, S1 128, O0 256, O1 384.  Registers: 512 x 128 at launch = 256 x 184 + 128 x 96 + 128 x 48
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 184;\n");
-        const int t = warp >> 2;
-        if (t < nt) {
+        const int t = warp >> 2, r = tid & 127, f = t * 128 + r;
+        const uint32_t lane_base = uint32_t(32 * (warp & 3)) << 16;
+        const uint32_t ts = tm + lane_base + uint32_t(128 * t), to = tm + lane_base + uint32_t(256 + 128 * t);
+        PrWalk w;
+        w.start(a, sm);
+        uint32_t n = 0;    // steps of this CTA so far
+        uint32_t nt_n = 0; // those that this tile took part in
+        uint32_t joins = 0;
+        bool ok = true;
+        for (int64_t u = u0; ok && u < u1;) {
+            w.seek(a, u);
+            const int64_t item = (u - w.base) / w.t.steps;
+            const int off = int(u - w.base - item * w.t.steps), hk = int(item);
+            const int steps = int(min(int64_t(w.t.steps - off), u1 - u));
+            const int64_t u_item = u - off;
+            u += steps;
+            if (t * 128 >= w.t.rows) {  // the request's last tile is a narrow one
+                n += steps;
+                continue;
+            }
             // --- this thread's row ---
-            const int r = tid & 127, f = t * 128 + r;
-            const uint32_t lane_base = uint32_t(32 * (warp & 3)) << 16;
-            const uint32_t ts = tm + lane_base + uint32_t(128 * t), to = tm + lane_base + uint32_t(256 + 128 * t);
-            const int64_t fc = col0 + f, row = row0 + fc / G;
-            const bool live = f < rows && row < a.q_rows;
+            const int64_t fc = w.t.col0 + f, row = w.t.row0 + fc / G;
+            const bool mine = f < w.t.rows, live = mine && row < a.q_rows;
             float cfac = fabsf(a.scale_log2);
             {
                 const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;  // group maxima below need a factor >= 0
                 const uint4* qp = reinterpret_cast<const uint4*>(a.q + (live ? row * a.q_tok + int64_t(hk * G + fc % G) * a.q_head : 0));
-                uint4 w[D / 8];
+                uint4 x[D / 8];
                 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) w[i] = live ? __ldg(qp + i) : make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < D / 8; ++i) x[i] = live ? __ldg(qp + i) : make_uint4(0, 0, 0, 0);
                 float mul = sign;
                 if constexpr (BF16) {
                     // to f16 by a power of two per row: largest magnitude in [2^14, 2^15), so that
                     // values down to 2^-31 of it keep all 8 bits
                     uint32_t m2 = 0;
                     #pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        const uint32_t x = __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu),
-                                                    __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu));
-                        m2 = __vmaxu2(m2, x);
-                    }
+                    for (int i = 0; i < D / 8; ++i)
+                        m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu),
+                                                   __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu)));
                     const float amax = fmaxf(__uint_as_float(m2 << 16), __uint_as_float(m2 & 0xffff0000u));
                     const int e = min(max((__float_as_int(amax) >> 23) - 127, -100), 100);
                     mul *= exp2_int(14 - e);
@@ -288,33 +385,43 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
                         else
                             return sign < 0.f ? v ^ 0x80008000u : v;
                     };
-                    const uint4 o = make_uint4(conv(w[i].x), conv(w[i].y), conv(w[i].z), conv(w[i].w));
-                    *reinterpret_cast<uint4*>(qs + t * kTile + (i >> 3) * kBlk + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = o;
+                    // the products that read the tile's last rows here are done: this thread has waited for the outputs after them
+                    *reinterpret_cast<uint4*>(qs + t * kTile + (i >> 3) * kBlk + r * 128 + (((i & 7) ^ (r & 7)) << 4)) =
+                        make_uint4(conv(x[i].x), conv(x[i].y), conv(x[i].z), conv(x[i].w));
                 }
                 fence_async_smem();
-                mbar_arrive(&sm.q_full);
+                tc_fence_before();
+                mbar_arrive(&sm.q_full[t]);
             }
-            const int pos = len - fresh + int(fc / G);
-            const int hi = f < rows ? min(pos + 1, len) : 0;
+            const int pos = w.t.len - w.t.fresh + int(fc / G);
+            const int hi = mine ? min(pos + 1, w.t.len) : 0;
             const int lo = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
             float ref = -INFINITY, l = 0.f;
-            bool ok = true;
             // of scores: above 0 whatever the scales, so that -inf stays -inf
             auto factor = [&](float kscale) { return fmaxf(cfac * kscale, 1e-37f); };
-            // Scores of 128 keys to weights.  `edge`: some row of the warp does not see all of them.
-            auto weigh = [&](bool edge, int base, int j, const float4* sc) {
+            for (int j = 0; j < steps; ++j, ++n, ++nt_n) {
+                const int base = w.t.k_begin + (off + j) * kPrKeys;
+                const PrStep& st = sm.step[n % kPrSlots];
+                ok = pr_wait(&sm.step_full[n % kPrSlots], (n / kPrSlots) & 1, a.status, abort_flag) &&
+                     pr_wait(&sm.s_full[t], nt_n & 1, a.status, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
                 uint32_t v[4][32];
                 #pragma unroll
                 for (int h = 0; h < 4; ++h) tmem_load32(ts + 32 * h, v[h]);
+                bool dead = mine && (base + kPrKeys > hi || base < lo);  // rows past the tile's end see nothing and give nothing
+                #pragma unroll
+                for (int g = 0; g < 8; ++g) dead |= st.sc[g].w == 0.f;
                 #pragma unroll
                 for (int h = 0; h < 4; ++h) tmem_load_wait(v[h]);
-                if (edge) {
+                if (__any_sync(0xffffffffu, dead)) {  // some row of the warp does not see all of them
                     #pragma unroll
                     for (int g = 0; g < 8; ++g) {
                         // bit i: key base + 16 g + i is seen
-                        const int from = min(max(lo - base - 16 * g, 0), 16), to = min(max(hi - base - 16 * g, 0), 16);
-                        uint32_t bits = ((1u << to) - 1u) & ~((1u << from) - 1u);
-                        if (sc[g].w == 0.f) bits = 0u;
+                        const int from = min(max(lo - base - 16 * g, 0), 16), upto = min(max(hi - base - 16 * g, 0), 16);
+                        uint32_t bits = ((1u << upto) - 1u) & ~((1u << from) - 1u);
+                        if (st.sc[g].w == 0.f) bits = 0u;
                         #pragma unroll
                         for (int i = 0; i < 16; ++i)
                             if (!(bits >> i & 1u)) v[g >> 1][16 * (g & 1) + i] = 0xff800000u;  // -inf
@@ -324,23 +431,24 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
                 float mx = -INFINITY;
                 #pragma unroll
                 for (int g = 0; g < 8; ++g) {
-                    const float4 s4 = sc[g];
+                    const float4 s4 = st.sc[g];
                     float x[16];
                     #pragma unroll
                     for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(v[g >> 1][16 * (g & 1) + i]);
                     #pragma unroll
-                    for (int n = 8; n; n >>= 1)
+                    for (int m = 8; m; m >>= 1)
                         #pragma unroll
-                        for (int i = 0; i < n; ++i) x[i] = fmaxf(x[i], x[i + n]);
+                        for (int i = 0; i < m; ++i) x[i] = fmaxf(x[i], x[i + m]);
                     mx = fmaxf(mx, fmaf(x[0], factor(s4.x), s4.y));
                 }
-                if (__any_sync(0xffffffffu, mx > ref + kPrSlack || (ref == -INFINITY && mx > ref))) {
+                if (__any_sync(0xffffffffu, mx > ref + kPrSlack)) {  // -inf + slack is -inf: the first key that is seen counts as growth
                     const float nref = fmaxf(ref, mx);
                     const float alpha = ref == nref ? 1.f : ex2(ref - nref);  // 0 where nothing has been seen
                     l *= alpha;
                     ref = nref;
                     if (j > 0) {
-                        if (!__all_sync(0xffffffffu, pr_wait(&sm.o_full[t], (j - 1) & 1, a.status, abort_flag))) return false;
+                        ok = __all_sync(0xffffffffu, pr_wait(&sm.o_full[t], (nt_n - 1) & 1, a.status, abort_flag));
+                        if (!ok) break;
                         tc_fence_after();
                         #pragma unroll 1
                         for (int h = 0; h < D / 32; ++h) {
@@ -353,15 +461,15 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
                         }
                     }
                 }
-                const float off = ref == -INFINITY ? 0.f : ref;
+                const float less = ref == -INFINITY ? 0.f : ref;
                 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     uint32_t p[16];
                     #pragma unroll
                     for (int g = 0; g < 2; ++g) {
-                        const float4 s4 = sc[2 * h + g];
-                        const float f = factor(s4.x);
-                        const float2 mul = make_float2(f, f), add = make_float2(s4.y - off, s4.y - off);
+                        const float4 s4 = st.sc[2 * h + g];
+                        const float fg = factor(s4.x);
+                        const float2 mul = make_float2(fg, fg), add = make_float2(s4.y - less, s4.y - less);
                         float2 sum = make_float2(0.f, 0.f);
                         #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
@@ -375,133 +483,112 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
                     }
                     tmem_store16(ts + 16 * h, p);
                 }
-                return true;
-            };
-            for (int j = 0; j < steps; ++j) {
-                const int base = key0 + j * kPrKeys;
-                ok = pr_wait(&sm.sc_full[j & 3], (j >> 2) & 1, a.status, abort_flag) &&
-                     pr_wait(&sm.s_full[t], j & 1, a.status, abort_flag);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_after();
-                const float4* sc = sm.sc[j & 3];
-                bool dead = f < rows && (base + kPrKeys > hi || base < lo);  // rows past the tile's end see nothing and give nothing
-                #pragma unroll
-                for (int g = 0; g < 8; ++g) dead |= sc[g].w == 0.f;
-                const bool edge = __any_sync(0xffffffffu, dead);
-
-                ok = weigh(edge, base, j, sc);
-                if (!ok) break;
                 tmem_store_wait();
                 tc_fence_before();
                 mbar_arrive(&sm.p_full[t]);
             }
             // --- the row's result ---
-            if (steps > 0 && ok) ok = __all_sync(0xffffffffu, pr_wait(&sm.o_full[t], (steps - 1) & 1, a.status, abort_flag));
+            ok = ok && __all_sync(0xffffffffu, pr_wait(&sm.o_full[t], (nt_n - 1) & 1, a.status, abort_flag));
+            if (!ok) break;
             tc_fence_after();
-            if (ok && ns == 1) {
-                const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
-                const int64_t at = row * a.heads + hk * G + fc % G;
-                #pragma unroll 1
-                for (int h = 0; h < D / 32; ++h) {
-                    uint32_t o[32];
-                    if (steps > 0) {
-                        tmem_load32(to + 32 * h, o);
-                        tmem_load_wait(o);
+            const int64_t at = row * a.heads + hk * G + fc % G;
+            // 32 dims of a row from h on
+            auto emit = [&](int h, const float (&o)[32], float inv) {
+                uint32_t x[16];
+                #pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if constexpr (BF16) {
+                        const __nv_bfloat162 q2 = __floats2bfloat162_rn(o[2 * i] * inv, o[2 * i + 1] * inv);
+                        x[i] = *reinterpret_cast<const uint32_t*>(&q2);
                     } else {
-                        #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = 0u;
+                        x[i] = pack_half2(o[2 * i] * inv, o[2 * i + 1] * inv);
                     }
-                    uint32_t w[16];
-                    #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float x = __uint_as_float(o[2 * i]) * inv, y = __uint_as_float(o[2 * i + 1]) * inv;
-                        if constexpr (BF16) {
-                            const __nv_bfloat162 q2 = __floats2bfloat162_rn(x, y);
-                            w[i] = *reinterpret_cast<const uint32_t*>(&q2);
-                        } else {
-                            w[i] = pack_half2(x, y);
-                        }
-                        if (l == 0.f) w[i] = 0u;
-                    }
-                    if (live) {
-                        uint4* dst = reinterpret_cast<uint4*>(a.out + at * D + 32 * h);
-                        #pragma unroll
-                        for (int i = 0; i < 4; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-                    }
+                    if (inv == 0.f) x[i] = 0u;
                 }
-                if (live && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (ref + log2f(l)) * 0.6931471805599453f;
-            } else if (ok) {
-                // partial: [item][split] of {reference, sum} per row, then O rows
-                float* part = a.part + (item * args.splits + split) * int64_t(kPrRows) * (D + 2);
-                __stcg(part + f, ref);
-                __stcg(part + kPrRows + f, l);
+                uint4* dst = reinterpret_cast<uint4*>(a.out + at * D + 32 * h);
+                if (live)
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) dst[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            };
+            auto emit_lse = [&](float m, float sum) {
+                if (live && a.lse) a.lse[at] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+            };
+            const bool whole = steps == w.t.steps;
+            float* part = a.part + (int64_t(2 * cta + (off == 0 ? 1 : 0)) * 2 + t) * pr_part<D>();
+            if (!whole) {
+                __stcg(part + r, ref);
+                __stcg(part + 128 + r, l);
+            }
+            #pragma unroll 1
+            for (int h = 0; h < D / 32; ++h) {
+                uint32_t o[32];
+                tmem_load32(to + 32 * h, o);
+                tmem_load_wait(o);
+                float x[32];
+                #pragma unroll
+                for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(o[i]);
+                if (whole) {
+                    emit(h, x, l == 0.f ? 0.f : 1.f / l);  // a row that sees no key is zero
+                } else {
+                    float4* dst = reinterpret_cast<float4*>(part + 256) + 8 * h * 128 + r;
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i) __stcg(dst + i * 128, make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
+                }
+            }
+            if (whole) {
+                emit_lse(ref, l);
+                continue;
+            }
+            // --- join the parts: the CTA that ends last, in key order ---
+            const int c0 = int(((u_item + 1) * ctas - 1) / total), c1 = int(((u_item + w.t.steps) * ctas - 1) / total);
+            // the tile's 128 threads; bounded like every other wait, since a warp may have given up before
+            auto together = [&]() {
+                mbar_arrive(&sm.join[t]);
+                ok = __all_sync(0xffffffffu, pr_wait(&sm.join[t], joins++ & 1, a.status, abort_flag));
+                return ok;
+            };
+            if (!together()) break;
+            if (r == 0) {
+                int prev;
+                int32_t* counter = a.counters + 2 * c0 + t;
+                asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(prev) : "l"(counter) : "memory");
+                sm.last[t] = prev == c1 - c0;
+                if (prev == c1 - c0) *counter = 0;  // ready for the next call
+            }
+            if (!together()) break;
+            if (sm.last[t]) {
+                auto piece = [&](int c) { return a.part + (int64_t(2 * c + (c == c0 ? 1 : 0)) * 2 + t) * pr_part<D>(); };
+                float m = -INFINITY, sum = 0.f;
+                #pragma unroll 4
+                for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(piece(c) + r));
+                const float less = m == -INFINITY ? 0.f : m;
+                #pragma unroll 4
+                for (int c = c0; c <= c1; ++c) sum = fmaf(__ldcg(piece(c) + 128 + r), ex2(__ldcg(piece(c) + r) - less), sum);
                 #pragma unroll 1
                 for (int h = 0; h < D / 32; ++h) {
-                    uint32_t o[32];
-                    tmem_load32(to + 32 * h, o);
-                    tmem_load_wait(o);
-                    float4* dst = reinterpret_cast<float4*>(part + 2 * kPrRows + f * D + 32 * h);
+                    float x[32];
                     #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        __stcg(dst + i, make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                                    __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])));
+                    for (int i = 0; i < 32; ++i) x[i] = 0.f;
+                    #pragma unroll 1
+                    for (int c = c0; c <= c1; ++c) {
+                        const float* pc = piece(c);
+                        const float wc = ex2(__ldcg(pc + r) - less);
+                        const float4* src = reinterpret_cast<const float4*>(pc + 256) + 8 * h * 128 + r;
+                        #pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float4 o = __ldcg(src + i * 128);
+                            x[4 * i] = fmaf(o.x, wc, x[4 * i]), x[4 * i + 1] = fmaf(o.y, wc, x[4 * i + 1]);
+                            x[4 * i + 2] = fmaf(o.z, wc, x[4 * i + 2]), x[4 * i + 3] = fmaf(o.w, wc, x[4 * i + 3]);
+                        }
+                    }
+                    emit(h, x, sum == 0.f ? 0.f : 1.f / sum);
                 }
+                emit_lse(m, sum);
             }
-            tc_fence_before();
+            if (!together()) break;  // sm.last is the next item's
         }
+        tc_fence_before();
         named_bar_arrive(1, 288);
-        if (ns == 1) return;
-
-        // --- join the parts of the keys: the CTA that ends last, in key order ---
-        named_bar_sync(2, 256);
-        if (tid == 0) {
-            int prev;
-            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(prev) : "l"(a.counters + item) : "memory");
-            sm.last = prev == ns - 1;
-            if (prev == ns - 1) a.counters[item] = 0;  // ready for the next call
-        }
-        named_bar_sync(2, 256);
-        if (!sm.last) return;
-        const float* parts = a.part + item * args.splits * int64_t(kPrRows) * (D + 2);
-        const int64_t pitch = int64_t(kPrRows) * (D + 2);
-        float* wt = reinterpret_cast<float*>(smem);  // [ns][rows]
-        for (int f = tid; f < rows; f += 256) {
-            float mx = -INFINITY, sum = 0.f;
-            for (int p = 0; p < ns; ++p) mx = fmaxf(mx, __ldcg(parts + p * pitch + f));
-            for (int p = 0; p < ns; ++p) {
-                const float w = mx == -INFINITY ? 0.f : ex2(__ldcg(parts + p * pitch + f) - mx);
-                wt[p * kPrRows + f] = w;
-                sum = fmaf(__ldcg(parts + p * pitch + kPrRows + f), w, sum);
-            }
-            sm.wt[f] = sum;
-            const int64_t row = row0 + (col0 + f) / G;
-            if (a.lse && row < a.q_rows)
-                a.lse[row * a.heads + hk * G + (col0 + f) % G] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
-        }
-        named_bar_sync(2, 256);
-        for (int i = tid; i < rows * (D / 4); i += 256) {
-            const int f = i / (D / 4), d = 4 * (i % (D / 4));
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            #pragma unroll 4
-            for (int p = 0; p < ns; ++p) {
-                const float4 o = __ldcg(reinterpret_cast<const float4*>(parts + p * pitch + 2 * kPrRows + f * D + d));
-                const float w = wt[p * kPrRows + f];
-                v.x = fmaf(o.x, w, v.x), v.y = fmaf(o.y, w, v.y), v.z = fmaf(o.z, w, v.z), v.w = fmaf(o.w, w, v.w);
-            }
-            const float sum = sm.wt[f], inv = sum == 0.f ? 0.f : 1.f / sum;
-            const int64_t row = row0 + (col0 + f) / G;
-            if (row >= a.q_rows) continue;
-            uint2 w;
-            if constexpr (BF16) {
-                const __nv_bfloat162 x = __floats2bfloat162_rn(v.x * inv, v.y * inv), y = __floats2bfloat162_rn(v.z * inv, v.w * inv);
-                w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-            } else {
-                w = make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
-            }
-            if (sum == 0.f) w = make_uint2(0u, 0u);
-            *reinterpret_cast<uint2*>(a.out + (row * a.heads + hk * G + (col0 + f) % G) * D + d) = w;
-        }
     } else if (warp < 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
         // --- codes to f16 ---
@@ -510,28 +597,19 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
         constexpr int NB = D / 64;
         constexpr int NP = 4;                // passes of 16 keys (of one page) to half a step
         const int ct = tid - 256, kr = ct >> 3, ch = ct & 7;
-        const int32_t* row_table = a.table + int64_t(b) * a.width;
-        // Of the 16 keys (lane & 7) of a step: whether the tile sees any, and their page as the
-        // table has it.  It is looked at one step later, when its load has long arrived.
-        auto key_of = [&](int j) { return key0 + j * kPrKeys + 16 * (lane & 7); };
-        auto some = [&](int j) { return j < steps && key_of(j) + 16 > lo_all && key_of(j) < hi_all; };
-        auto raw_page = [&](int j) { return some(j) ? __ldg(row_table + (key_of(j) >> a.shift)) : -1; };
-        auto page_of = [&](int j, int raw) {
-            const bool in = raw >= 0 && raw < a.pages;
-            if (some(j) && !in) set_status(a.status, DEV_BAD_INDEX);
-            return in ? raw : -1;
-        };
         const int64_t page_bytes = (int64_t(Hk) * D) << a.shift;
-        const int64_t mine = (int64_t(hk) * D << a.shift) + kr * D + ch * 8;
-        auto load = [&](const uint8_t* codes, int j, int half, int pg, uint2 (&w)[NP][NB]) {
+        const int mine = kr * D + ch * 8;
+        auto load = [&](const uint8_t* codes, const PrStep& st, int half, uint2 (&w)[NP][NB]) {
+            const uint8_t* head = codes + ((int64_t(st.hk) * D) << a.shift) + mine;
+            const int from = st.from, to = st.to;
             #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                const int key = key0 + j * kPrKeys + (half * NP + i) * 16, pi = __shfl_sync(0xffffffffu, pg, half * NP + i);
-                const uint8_t* p = codes + pi * page_bytes + mine + (key & (P - 1)) * D;
+                const int key = (half * NP + i) * 16, pi = st.page[half * NP + i];
+                const uint8_t* p = head + pi * page_bytes + (key & (P - 1)) * D;  // steps begin at whole pages
                 // keys that no row sees are zeros: their codes may be NaN, and 0 * NaN is not 0
-                const bool get = pi >= 0 && key + kr >= lo_all && key + kr < hi_all;
+                const bool get = pi >= 0 && key + kr >= from && key + kr < to;
                 #pragma unroll
-                for (int n = 0; n < NB; ++n) w[i][n] = load_early(p + 64 * n, get);
+                for (int m = 0; m < NB; ++m) w[i][m] = load_early(p + 64 * m, get);
             }
         };
         const uint32_t place = uint32_t(kr * 128 + ((ch ^ (kr & 7)) << 4));
@@ -539,9 +617,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
             #pragma unroll
             for (int i = 0; i < NP; ++i)
                 #pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    const uint32_t x = code_word<E4M3>(w[i][n].x), y = code_word<E4M3>(w[i][n].y);
-                    *reinterpret_cast<uint4*>(dst + n * kBlk + (half * NP + i) * (16 * 128) + place) =
+                for (int m = 0; m < NB; ++m) {
+                    const uint32_t x = code_word<E4M3>(w[i][m].x), y = code_word<E4M3>(w[i][m].y);
+                    *reinterpret_cast<uint4*>(dst + m * kBlk + (half * NP + i) * (16 * 128) + place) =
                         make_uint4(half2_lo<E4M3>(x), half2_hi<E4M3>(x), half2_lo<E4M3>(y), half2_hi<E4M3>(y));
                 }
         };
@@ -550,60 +628,96 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
-        float ks = 0.f, vs = 1.f;  // of lanes 0-7 of warp 8: their 16 keys' scales
-        auto scales = [&](int pg) {
-            if (warp != 8 || pg < 0) return;
-            ks = __ldg(a.k_scale + int64_t(pg) * Hk + hk);
-            vs = __ldg(a.v_scale + int64_t(pg) * Hk + hk);
+        const uint32_t steps = uint32_t(u1 - u0);
+        auto known = [&](uint32_t n) {
+            return __all_sync(0xffffffffu, pr_wait(&sm.step_full[n % kPrSlots], (n / kPrSlots) & 1, a.status, abort_flag)) != 0;
         };
         // two halves are on their way while a third is written
         uint2 k0[NP][NB], k1[NP][NB], v0[NP][NB], v1[NP][NB];
-        int pg = page_of(0, raw_page(0)), raw = raw_page(1);
-        load(a.k, 0, 0, pg, k0);
-        load(a.k, 0, 1, pg, k1);
-        scales(pg);
-        for (int j = 0; j < steps; ++j) {
-            const int s = j & 1;
-            bool ok = j < 2 || pr_wait(&sm.k_empty[s], ((j >> 1) - 1) & 1, a.status, abort_flag);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            put(kst + s * kTile, 0, k0);
-            load(a.v, j, 0, pg, v0);
-            put(kst + s * kTile, 1, k1);
-            load(a.v, j, 1, pg, v1);
-            if (warp == 8) {
-                const int ve = stored_exponent(vs);
-                if (lane < 8)
-                    sm.sc[j & 3][lane] = pg < 0 ? make_float4(0.f, 0.f, 1.f, some(j) ? 0.f : 1.f)
-                                                : make_float4(ks, float(ve), exp2_int(-ve), 1.f);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.sc_full[j & 3]);
+        if (known(0)) {
+            load(a.k, sm.step[0], 0, k0);
+            load(a.k, sm.step[0], 1, k1);
+            for (uint32_t n = 0; n < steps; ++n) {
+                const uint32_t s = n & 1;
+                bool ok = n < 2 || pr_wait(&sm.k_empty[s], ((n >> 1) - 1) & 1, a.status, abort_flag);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                const PrStep& st = sm.step[n % kPrSlots];
+                put(kst + s * kTile, 0, k0);
+                load(a.v, st, 0, v0);
+                put(kst + s * kTile, 1, k1);
+                load(a.v, st, 1, v1);
+                handed(&sm.k_full[s]);
+                // K of step n is in place of step n - 2's, whose products, and those of n - 3's weights, are
+                // done: every row has left step n - 3, and its slot is free
+                if (n >= 3 && lane == 0) mbar_arrive(&sm.step_free[(n - 3) % kPrSlots]);
+                const bool more = n + 1 < steps;
+                if (more && !known(n + 1)) break;
+                ok = n < 2 || pr_wait(&sm.v_empty[s], ((n >> 1) - 1) & 1, a.status, abort_flag);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                const PrStep& next = sm.step[(n + 1) % kPrSlots];
+                put(vst + s * kTile, 0, v0);
+                if (more) load(a.k, next, 0, k0);
+                put(vst + s * kTile, 1, v1);
+                if (more) load(a.k, next, 1, k1);
+                handed(&sm.v_full[s]);
             }
-            handed(&sm.k_full[s]);
-            pg = page_of(j + 1, raw);
-            raw = raw_page(j + 2);
-            scales(pg);
-            ok = j < 2 || pr_wait(&sm.v_empty[s], ((j >> 1) - 1) & 1, a.status, abort_flag);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            put(vst + s * kTile, 0, v0);
-            load(a.k, j + 1, 0, pg, k0);
-            put(vst + s * kTile, 1, v1);
-            load(a.k, j + 1, 1, pg, k1);
-            handed(&sm.v_full[s]);
         }
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
-      if (warp > 12) return;
-      if (steps > 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
+        if (warp == 13) {
+            // --- pages and scales: lanes 8 i .. 8 i + 7 have the 16-key groups of every fourth step from step i on ---
+            PrWalk w;
+            w.start(a, sm);
+            const int g = lane & 7;
+            const uint32_t steps = uint32_t(u1 - u0);
+            for (uint32_t n0 = 0; n0 < steps; n0 += 4) {
+                const uint32_t n = n0 + (lane >> 3);
+                float4 sc = make_float4(0.f, 0.f, 1.f, 1.f);
+                int page = -1, from = 0, to = 0, hk = 0;
+                if (n < steps) {
+                    const int64_t u = u0 + n;
+                    w.seek(a, u);
+                    hk = int((u - w.base) / w.t.steps);
+                    const int k0 = w.t.k_begin + int(u - w.base - int64_t(hk) * w.t.steps) * kPrKeys, key = k0 + 16 * g;
+                    from = max(w.t.lo - k0, 0), to = min(w.t.hi - k0, kPrKeys);
+                    if (key + 16 > w.t.lo && key < w.t.hi) {
+                        page = __ldg(a.table + int64_t(w.b) * a.width + (key >> a.shift));
+                        if (page >= 0 && page < a.pages) {
+                            const int64_t at = int64_t(page) * Hk + hk;
+                            const int ve = stored_exponent(__ldg(a.v_scale + at));
+                            sc = make_float4(__ldg(a.k_scale + at), float(ve), exp2_int(-ve), 1.f);
+                        } else {
+                            set_status(a.status, DEV_BAD_INDEX);
+                            page = -1;
+                            sc.w = 0.f;
+                        }
+                    }
+                }
+                // slot of step n0 + 3: the last of the four to be free
+                bool ok = true;
+                if (n < steps && n >= kPrSlots)
+                    ok = pr_wait(&sm.step_free[n % kPrSlots], (n / kPrSlots - 1) & 1, a.status, abort_flag);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                if (n < steps) {
+                    PrStep& st = sm.step[n % kPrSlots];
+                    st.sc[g] = sc;
+                    st.page[g] = page;
+                    if (g == 0) st.from = from, st.to = to, st.hk = hk;
+                }
+                __syncwarp();
+                if (n < steps && g == 0) mbar_arrive(&sm.step_full[n % kPrSlots]);
+            }
+        }
+        if (warp != 12) return;
         // --- the products.  The whole warp runs this, so that addresses stay in uniform registers; an
-        // elected lane issues.  A stage is handed back only where it will be filled again, so the last
-        // arrival on its way is one that somebody waits for ---
+        // elected lane issues ---
         constexpr uint32_t idesc_s = umma_idesc_f16_f32(128, kPrKeys);
         constexpr uint32_t idesc_o = umma_idesc_f16_f32(128, D) | (1u << 16);  // V: MN-major
         constexpr uint32_t kStep = kTile >> 4;
         const uint64_t q0 = umma_desc_k_sw128(smem_u32(qs)), k0 = umma_desc_k_sw128(smem_u32(kst));
         const uint64_t v0 = umma_desc_mn_sw128(smem_u32(vst), kBlk);
-        auto scores = [&](int t, int s) {
-            const uint64_t qd = q0 + uint32_t(t) * kStep, kd = k0 + uint32_t(s) * kStep;
+        auto scores = [&](int t, uint32_t s) {
+            const uint64_t qd = q0 + uint32_t(t) * kStep, kd = k0 + s * kStep;
             #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 const uint32_t at = uint32_t((i >> 2) * kBlk + (i & 3) * 32) >> 4;
@@ -614,85 +728,77 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const PrArgs a
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             return __all_sync(0xffffffffu, pr_wait(bar, parity, a.status, abort_flag)) != 0;
         };
-        bool ok = wait(&sm.q_full, 0) && wait(&sm.k_full[0], 0);
-        tc_fence_after();
-        if (ok) {
-            for (int t = 0; t < nt; ++t) scores(t, 0);
-            if (steps > 2) elect_commit(&sm.k_empty[0]);
-        }
-        for (int j = 0; ok && j < steps; ++j) {
-            const int s = j & 1, sn = (j + 1) & 1;
-            const bool more = j + 1 < steps;
-            if (more) ok = wait(&sm.k_full[sn], ((j + 1) >> 1) & 1);
-            ok = ok && wait(&sm.v_full[s], (j >> 1) & 1);
+        PrWalk w;
+        w.start(a, sm);
+        uint32_t n = 0, n1 = 0, items = 0, items1 = 0;  // steps and items so far; those with a second tile
+        bool ok = true;
+        for (int64_t u = u0; ok && u < u1;) {
+            w.seek(a, u);
+            const int off = int((u - w.base) % w.t.steps);
+            const int steps = int(min(int64_t(w.t.steps - off), u1 - u)), nt = w.t.rows > 128 ? 2 : 1;
+            u += steps;
+            ok = wait(&sm.k_full[n & 1], (n >> 1) & 1);
             for (int t = 0; ok && t < nt; ++t) {
-                ok = wait(&sm.p_full[t], j & 1);
+                ok = wait(&sm.q_full[t], (t ? items1 : items) & 1);
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t vd = v0 + uint32_t(s) * kStep;
-                #pragma unroll
-                for (int i = 0; i < kPrKeys / 16; ++i)
-                    elect_umma_ts(tm + 256 + 128 * t, tm + 128 * t + 8 * i, vd + uint32_t(2048 * i >> 4), idesc_o,
-                                  i > 0 ? 1u : uint32_t(j > 0));
-                elect_commit(&sm.o_full[t]);
-                if (more) scores(t, sn);
+                scores(t, n & 1);
             }
             if (!ok) break;
-            if (j + 2 < steps) elect_commit(&sm.v_empty[s]);
-            if (j + 3 < steps) elect_commit(&sm.k_empty[sn]);
-        }
-        // after a wait that ran out: the products in flight still use TMEM and shared memory
-        if (!ok) {
-            if (lane == 0) {
-                mbar_init(&sm.q_full, 1);
-                mbar_fence_init();
+            elect_commit(&sm.k_empty[n & 1]);
+            ++items, items1 += nt - 1;
+            for (int j = 0; j < steps; ++j, ++n, n1 += nt - 1) {
+                const uint32_t s = n & 1, sn = s ^ 1;
+                const bool more = j + 1 < steps;
+                if (more) ok = wait(&sm.k_full[sn], ((n + 1) >> 1) & 1);
+                ok = ok && wait(&sm.v_full[s], (n >> 1) & 1);
+                for (int t = 0; ok && t < nt; ++t) {
+                    ok = wait(&sm.p_full[t], (t ? n1 : n) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t vd = v0 + s * kStep;
+                    #pragma unroll
+                    for (int i = 0; i < kPrKeys / 16; ++i)
+                        elect_umma_ts(tm + 256 + 128 * t, tm + 128 * t + 8 * i, vd + uint32_t(2048 * i >> 4), idesc_o,
+                                      i > 0 ? 1u : uint32_t(j > 0));
+                    elect_commit(&sm.o_full[t]);
+                    if (more) scores(t, sn);
+                }
+                if (!ok) break;
+                elect_commit(&sm.v_empty[s]);
+                if (more) elect_commit(&sm.k_empty[sn]);
             }
-            __syncwarp();
-            elect_commit(&sm.q_full);
-            mbar_wait(&sm.q_full, 0, a.status);
         }
-      }
-      __syncwarp();
-      named_bar_sync(1, 288);  // the rows are read
-      tc_fence_after();
-      tmem_dealloc(tm, kPrTmem);
+        // all products are done, also after a wait that ran out: TMEM and shared memory are free to go
+        elect_commit(&sm.done);
+        mbar_wait(&sm.done, 0, a.status);
+        __syncwarp();
+        named_bar_sync(1, 288);  // the rows are read
+        tc_fence_after();
+        tmem_dealloc(tm, kPrTmem);
     }
 }
 
-// The host knows the rows in all, not the requests' own: at most one part
-// tile more per request.  Fewer CTAs than SMs: the keys of a tile are split.
-KvPromptPlan kv_prompt_plan(const KvAttendCall& c, int sms) {
-    const int64_t group = c.heads / c.kv_heads;
-    KvPromptPlan p;
-    p.tiles = c.q_rows * group / kPrRows + c.requests;
-    const int64_t items = p.tiles * c.kv_heads;
-    p.splits = items > 0 && items * 2 <= sms ? int(sms / items < kPrMaxSplits ? sms / items : kPrMaxSplits) : 1;
-    p.bytes = p.splits > 1 ? size_t(items) * p.splits * kPrRows * (c.dim + 2) * 4 : 0;
-    return p;
-}
+// One CTA per SM, each with at most two items that it shares with others.
+size_t kv_prompt_bytes(const KvAttendCall& c, int sms) { return size_t(sms) * 2 * 2 * 128 * (c.dim + 2) * 4; }
 
 template <bool E4M3, bool BF16, int D>
-static cudaError_t launch_prompt(const PrArgs& a, unsigned grid, cudaStream_t s) {
+static cudaError_t launch_prompt(const KvAttendArgs& a, int sms, cudaStream_t s) {
     constexpr size_t smem = pr_smem_bytes<D>();
-    static_assert(smem <= 227 * 1024 && kPrMaxSplits * kPrRows * 4 + sizeof(PrSmem) + 1024 <= smem, "shared memory");
+    static_assert(smem <= 227 * 1024, "shared memory");
     auto* kernel = kv_prompt_kernel<E4M3, BF16, D>;
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = raise_smem(kernel, smem, done);
     if (e != cudaSuccess) return e;
-    kernel<<<grid, kPrThreads, smem, s>>>(a);
+    kernel<<<sms, kPrThreads, smem, s>>>(a);
     return cudaGetLastError();
 }
 
-cudaError_t run_kv_prompt(const KvAttendCall& c, const KvAttendArgs& args, const KvPromptPlan& p, cudaStream_t s) {
-    PrArgs a;
-    a.a = args, a.splits = p.splits;
-    const int64_t n = p.tiles * c.kv_heads * p.splits;
-    if (n <= 0) return cudaSuccess;
-    if (n > INT32_MAX) return cudaErrorInvalidConfiguration;
-    const unsigned grid = unsigned(n);
+cudaError_t run_kv_prompt(const KvAttendCall& c, const KvAttendArgs& a, int sms, cudaStream_t s) {
+    if (c.requests == 0) return cudaSuccess;
     const auto by_dim = [&](auto e4, auto bf) {
         constexpr bool E = decltype(e4)::value, B = decltype(bf)::value;
-        return c.dim == 128 ? launch_prompt<E, B, 128>(a, grid, s) : launch_prompt<E, B, 64>(a, grid, s);
+        return c.dim == 128 ? launch_prompt<E, B, 128>(a, sms, s) : launch_prompt<E, B, 64>(a, sms, s);
     };
     const bool bf16 = c.x_dtype == DT_BF16;
     if (c.e4m3) return bf16 ? by_dim(std::true_type(), std::true_type()) : by_dim(std::true_type(), std::false_type());
