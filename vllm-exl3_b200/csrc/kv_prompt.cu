@@ -13,8 +13,9 @@
 //   8-11      codes of 128 keys from global memory to f16 in shared memory
 //             (128-byte swizzle; K is a K-major operand, V an MN-major one: the same bytes)
 //   13        pages and scales of the steps to come, four steps at a time, into a ring
+//   14        the items to come into another: what every warp needs to know of them stays in shared memory
 //   12        an elected lane issues S = Q K^T and O += P V (tcgen05, fp32 in TMEM)
-//   14-15     idle: they make up the warpgroup whose registers the first eight warps take
+//   15        idle: it makes up the warpgroup whose registers the first eight warps take
 //             (184 a thread: a row's 128 scores are read from TMEM once and stay in registers)
 // TMEM: S0 S1 (128 columns each; the weights, f16, take the place of the
 // scores that they came from and are the A operand of P V), O0 O1.
@@ -58,9 +59,18 @@ struct PrStep {
     int hk, pad;
 };
 
+// an item's share of this CTA: `steps` of its `all` steps, from `off` on
+struct PrItem {
+    int64_t row0, col0;
+    int steps, off, all;  // steps 0: no more items
+    int rows, hk, fresh, len, k_begin;
+    int c0, c1;           // the CTAs that share the item
+};
+constexpr int kPrItems = 4;
+
 struct PrSmem {
     uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
-    uint64_t step_full[kPrSlots], step_free[kPrSlots];
+    uint64_t step_full[kPrSlots], step_free[kPrSlots], item_full[kPrItems], item_free[kPrItems];
     uint64_t join[2];  // of a tile's rows among themselves
     uint64_t done;
     uint32_t tmem;
@@ -69,6 +79,7 @@ struct PrSmem {
     int found_b, found_tile;
     int64_t found_base;
     PrStep step[kPrSlots];
+    PrItem item[kPrItems];
 };
 
 template <int D>
@@ -220,6 +231,13 @@ __device__ __forceinline__ uint2 load_early(const uint8_t* p, bool get) {
     return v;
 }
 
+// the largest of three, NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 template <bool E4M3, bool BF16, int D>
 __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttendArgs a) {
     constexpr int kBlk = kPrKeys * 128;        // bytes of a 64-dim block of 128 rows
@@ -318,6 +336,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
             mbar_init(&sm.step_full[i], 1);
             mbar_init(&sm.step_free[i], 4);
         }
+        for (int i = 0; i < kPrItems; ++i) {
+            mbar_init(&sm.item_full[i], 1);
+            mbar_init(&sm.item_free[i], 9);  // the rows' warps and the products'
+        }
         mbar_init(&sm.done, 1);
         sm.abort_flag = 0;
         mbar_fence_init();
@@ -330,36 +352,39 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
     const int64_t total = sm.scan[0];
     const int ctas = int(min(int64_t(gridDim.x), (total + kPrLeast - 1) / kPrLeast)), cta = blockIdx.x;
     const int64_t u0 = total * cta / ctas, u1 = total * (cta + 1) / ctas;
-    // TMEM columns: S0 0, S1 128, O0 256, O1 384.  Registers: 512 x 128 at launch = 256 x 184 + 128 x 96 + 128 x 48
+    // TMEM columns: S0 0, S1 128, O0 256, O1 384.  Registers: 512 x 128 at launch = 256 x 184 + 128 x 88 + 128 x 56
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 184;\n");
         const int t = warp >> 2, r = tid & 127, f = t * 128 + r;
         const uint32_t lane_base = uint32_t(32 * (warp & 3)) << 16;
         const uint32_t ts = tm + lane_base + uint32_t(128 * t), to = tm + lane_base + uint32_t(256 + 128 * t);
-        PrWalk w;
-        w.start(a, sm);
         uint32_t n = 0;    // steps of this CTA so far
         uint32_t nt_n = 0; // those that this tile took part in
         uint32_t joins = 0;
         bool ok = true;
-        for (int64_t u = u0; ok && u < u1;) {
-            w.seek(a, u);
-            const int64_t item = (u - w.base) / w.t.steps;
-            const int off = int(u - w.base - item * w.t.steps), hk = int(item);
-            const int steps = int(min(int64_t(w.t.steps - off), u1 - u));
-            const int64_t u_item = u - off;
-            u += steps;
-            if (t * 128 >= w.t.rows) {  // the request's last tile is a narrow one
+        for (uint32_t it = 0;; ++it) {
+            const PrItem& im = sm.item[it % kPrItems];
+            ok = __all_sync(0xffffffffu, pr_wait(&sm.item_full[it % kPrItems], (it / kPrItems) & 1, a.status, abort_flag));
+            if (!ok) break;
+            const int steps = im.steps;
+            if (steps == 0) break;
+            auto leave = [&]() {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.item_free[it % kPrItems]);
+            };
+            if (t * 128 >= im.rows) {  // the request's last tile is a narrow one
                 n += steps;
+                leave();
                 continue;
             }
             // --- this thread's row ---
-            const int64_t fc = w.t.col0 + f, row = w.t.row0 + fc / G;
-            const bool mine = f < w.t.rows, live = mine && row < a.q_rows;
+            const int64_t fc = im.col0 + f, row = im.row0 + fc / G;
+            const bool mine = f < im.rows, live = mine && row < a.q_rows;
+            const int64_t at = row * a.heads + im.hk * G + fc % G;
             float cfac = fabsf(a.scale_log2);
             {
                 const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;  // group maxima below need a factor >= 0
-                const uint4* qp = reinterpret_cast<const uint4*>(a.q + (live ? row * a.q_tok + int64_t(hk * G + fc % G) * a.q_head : 0));
+                const uint4* qp = reinterpret_cast<const uint4*>(a.q + (live ? row * a.q_tok + int64_t(im.hk * G + fc % G) * a.q_head : 0));
                 uint4 x[D / 8];
                 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) x[i] = live ? __ldg(qp + i) : make_uint4(0, 0, 0, 0);
@@ -393,56 +418,58 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                 tc_fence_before();
                 mbar_arrive(&sm.q_full[t]);
             }
-            const int pos = w.t.len - w.t.fresh + int(fc / G);
-            const int hi = mine ? min(pos + 1, w.t.len) : 0;
+            const int pos = im.len - im.fresh + int(fc / G);
+            const int hi = mine ? min(pos + 1, im.len) : 0;
             const int lo = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
             float ref = -INFINITY, l = 0.f;
             // of scores: above 0 whatever the scales, so that -inf stays -inf
             auto factor = [&](float kscale) { return fmaxf(cfac * kscale, 1e-37f); };
-            for (int j = 0; j < steps; ++j, ++n, ++nt_n) {
-                const int base = w.t.k_begin + (off + j) * kPrKeys;
+            int base = im.k_begin + im.off * kPrKeys;
+            for (int j = 0; j < steps; ++j, ++n, ++nt_n, base += kPrKeys) {
                 const PrStep& st = sm.step[n % kPrSlots];
                 ok = pr_wait(&sm.step_full[n % kPrSlots], (n / kPrSlots) & 1, a.status, abort_flag) &&
                      pr_wait(&sm.s_full[t], nt_n & 1, a.status, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
+                // the row's scores, read once
                 uint32_t v[4][32];
                 #pragma unroll
                 for (int h = 0; h < 4; ++h) tmem_load32(ts + 32 * h, v[h]);
                 bool dead = mine && (base + kPrKeys > hi || base < lo);  // rows past the tile's end see nothing and give nothing
                 #pragma unroll
                 for (int g = 0; g < 8; ++g) dead |= st.sc[g].w == 0.f;
-                #pragma unroll
-                for (int h = 0; h < 4; ++h) tmem_load_wait(v[h]);
-                if (__any_sync(0xffffffffu, dead)) {  // some row of the warp does not see all of them
+                const bool edge = __any_sync(0xffffffffu, dead);  // some row of the warp does not see all of them
+                auto mask = [&](int h, uint32_t (&x)[32]) {
                     #pragma unroll
-                    for (int g = 0; g < 8; ++g) {
-                        // bit i: key base + 16 g + i is seen
-                        const int from = min(max(lo - base - 16 * g, 0), 16), upto = min(max(hi - base - 16 * g, 0), 16);
+                    for (int g = 0; g < 2; ++g) {
+                        // bit i: key base + 32 h + 16 g + i is seen
+                        const int k0 = base + 32 * h + 16 * g;
+                        const int from = min(max(lo - k0, 0), 16), upto = min(max(hi - k0, 0), 16);
                         uint32_t bits = ((1u << upto) - 1u) & ~((1u << from) - 1u);
-                        if (st.sc[g].w == 0.f) bits = 0u;
+                        if (st.sc[2 * h + g].w == 0.f) bits = 0u;
                         #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            if (!(bits >> i & 1u)) v[g >> 1][16 * (g & 1) + i] = 0xff800000u;  // -inf
+                            if (!(bits >> i & 1u)) x[16 * g + i] = 0xff800000u;  // -inf
                     }
-                }
-                // the row's largest
+                };
                 float mx = -INFINITY;
                 #pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    const float4 s4 = st.sc[g];
-                    float x[16];
+                for (int h = 0; h < 4; ++h) {
+                    tmem_load_wait(v[h]);
+                    if (edge) mask(h, v[h]);
                     #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(v[g >> 1][16 * (g & 1) + i]);
-                    #pragma unroll
-                    for (int m = 8; m; m >>= 1)
-                        #pragma unroll
-                        for (int i = 0; i < m; ++i) x[i] = fmaxf(x[i], x[i + m]);
-                    mx = fmaxf(mx, fmaf(x[0], factor(s4.x), s4.y));
+                    for (int g = 0; g < 2; ++g) {
+                        const float4 s4 = st.sc[2 * h + g];
+                        auto x = [&](int i) { return __uint_as_float(v[h][16 * g + i]); };
+                        const float m0 = max3(x(0), x(1), x(2)), m1 = max3(x(3), x(4), x(5)), m2 = max3(x(6), x(7), x(8));
+                        const float m3 = max3(x(9), x(10), x(11)), m4 = max3(x(12), x(13), x(14));
+                        const float top = max3(max3(m0, m1, m2), max3(m3, m4, x(15)), -INFINITY);
+                        mx = max3(mx, fmaf(top, factor(s4.x), s4.y), -INFINITY);
+                    }
                 }
                 if (__any_sync(0xffffffffu, mx > ref + kPrSlack)) {  // -inf + slack is -inf: the first key that is seen counts as growth
-                    const float nref = fmaxf(ref, mx);
+                    const float nref = fmaxf(ref, mx);  // of a NaN row: any
                     const float alpha = ref == nref ? 1.f : ex2(ref - nref);  // 0 where nothing has been seen
                     l *= alpha;
                     ref = nref;
@@ -474,10 +501,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                         #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
                             const float2 raw = make_float2(__uint_as_float(v[h][16 * g + i]), __uint_as_float(v[h][16 * g + i + 1]));
-                            float2 x = fma2(raw, mul, add);
-                            x = make_float2(ex2(x.x), ex2(x.y));
-                            sum = add2(sum, x);
-                            p[8 * g + i / 2] = pack_half2(x.x, x.y);
+                            const float2 x = fma2(raw, mul, add);
+                            const float2 e = make_float2(ex2(x.x), ex2(x.y));
+                            sum = add2(sum, e);
+                            p[8 * g + i / 2] = pack_half2(e.x, e.y);
                         }
                         l = fmaf(sum.x + sum.y, s4.z, l);
                     }
@@ -491,7 +518,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
             ok = ok && __all_sync(0xffffffffu, pr_wait(&sm.o_full[t], (nt_n - 1) & 1, a.status, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            const int64_t at = row * a.heads + hk * G + fc % G;
             // 32 dims of a row from h on
             auto emit = [&](int h, const float (&o)[32], float inv) {
                 uint32_t x[16];
@@ -513,8 +539,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
             auto emit_lse = [&](float m, float sum) {
                 if (live && a.lse) a.lse[at] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
             };
-            const bool whole = steps == w.t.steps;
-            float* part = a.part + (int64_t(2 * cta + (off == 0 ? 1 : 0)) * 2 + t) * pr_part<D>();
+            const bool whole = steps == im.all;
+            float* part = a.part + (int64_t(2 * cta + (im.off == 0 ? 1 : 0)) * 2 + t) * pr_part<D>();
             if (!whole) {
                 __stcg(part + r, ref);
                 __stcg(part + 128 + r, l);
@@ -537,10 +563,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
             }
             if (whole) {
                 emit_lse(ref, l);
+                leave();
                 continue;
             }
             // --- join the parts: the CTA that ends last, in key order ---
-            const int c0 = int(((u_item + 1) * ctas - 1) / total), c1 = int(((u_item + w.t.steps) * ctas - 1) / total);
+            const int c0 = im.c0, c1 = im.c1;
             // the tile's 128 threads; bounded like every other wait, since a warp may have given up before
             auto together = [&]() {
                 mbar_arrive(&sm.join[t]);
@@ -586,11 +613,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                 emit_lse(m, sum);
             }
             if (!together()) break;  // sm.last is the next item's
+            leave();
         }
         tc_fence_before();
         named_bar_arrive(1, 288);
     } else if (warp < 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
         // --- codes to f16 ---
         // a thread takes 8 dims of each 64-dim block of a key: 8 lanes' 16-byte stores of one block
         // fall on 8 different places of a swizzled 128-byte row
@@ -663,7 +691,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
         if (warp == 13) {
             // --- pages and scales: lanes 8 i .. 8 i + 7 have the 16-key groups of every fourth step from step i on ---
             PrWalk w;
@@ -708,6 +736,33 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                 if (n < steps && g == 0) mbar_arrive(&sm.step_full[n % kPrSlots]);
             }
         }
+        if (warp == 14) {
+            // --- items ---
+            PrWalk w;
+            w.start(a, sm);
+            int64_t u = u0;
+            for (uint32_t it = 0;; ++it) {
+                bool ok = it < kPrItems || pr_wait(&sm.item_free[it % kPrItems], (it / kPrItems - 1) & 1, a.status, abort_flag);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                PrItem im = {};
+                if (u < u1) {
+                    w.seek(a, u);
+                    im.hk = int((u - w.base) / w.t.steps);
+                    im.off = int(u - w.base - int64_t(im.hk) * w.t.steps);
+                    im.all = w.t.steps, im.steps = int(min(int64_t(w.t.steps - im.off), u1 - u));
+                    im.row0 = w.t.row0, im.col0 = w.t.col0, im.rows = w.t.rows, im.fresh = w.t.fresh, im.len = w.t.len;
+                    im.k_begin = w.t.k_begin;
+                    const int64_t first = u - im.off;
+                    im.c0 = int(((first + 1) * ctas - 1) / total), im.c1 = int(((first + im.all) * ctas - 1) / total);
+                    u += im.steps;
+                }
+                if (lane == 0) {
+                    sm.item[it % kPrItems] = im;
+                    mbar_arrive(&sm.item_full[it % kPrItems]);
+                }
+                if (im.steps == 0) break;
+            }
+        }
         if (warp != 12) return;
         // --- the products.  The whole warp runs this, so that addresses stay in uniform registers; an
         // elected lane issues ---
@@ -728,15 +783,15 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             return __all_sync(0xffffffffu, pr_wait(bar, parity, a.status, abort_flag)) != 0;
         };
-        PrWalk w;
-        w.start(a, sm);
-        uint32_t n = 0, n1 = 0, items = 0, items1 = 0;  // steps and items so far; those with a second tile
+        uint32_t n = 0, n1 = 0, items1 = 0;  // steps so far, those with a second tile, items with one
         bool ok = true;
-        for (int64_t u = u0; ok && u < u1;) {
-            w.seek(a, u);
-            const int off = int((u - w.base) % w.t.steps);
-            const int steps = int(min(int64_t(w.t.steps - off), u1 - u)), nt = w.t.rows > 128 ? 2 : 1;
-            u += steps;
+        for (uint32_t items = 0; ok;) {
+            ok = wait(&sm.item_full[items % kPrItems], (items / kPrItems) & 1);
+            if (!ok) break;
+            const int steps = sm.item[items % kPrItems].steps, nt = sm.item[items % kPrItems].rows > 128 ? 2 : 1;
+            if (steps == 0) break;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.item_free[items % kPrItems]);
             ok = wait(&sm.k_full[n & 1], (n >> 1) & 1);
             for (int t = 0; ok && t < nt; ++t) {
                 ok = wait(&sm.q_full[t], (t ? items1 : items) & 1);
@@ -753,10 +808,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                 if (more) ok = wait(&sm.k_full[sn], ((n + 1) >> 1) & 1);
                 ok = ok && wait(&sm.v_full[s], (n >> 1) & 1);
                 for (int t = 0; ok && t < nt; ++t) {
+                    const uint64_t vd = v0 + s * kStep;
                     ok = wait(&sm.p_full[t], (t ? n1 : n) & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t vd = v0 + s * kStep;
                     #pragma unroll
                     for (int i = 0; i < kPrKeys / 16; ++i)
                         elect_umma_ts(tm + 256 + 128 * t, tm + 128 * t + 8 * i, vd + uint32_t(2048 * i >> 4), idesc_o,
