@@ -54,9 +54,8 @@ constexpr uint32_t kPrTmem = 512;
 // pages and scales of a step
 struct PrStep {
     float4 sc[8];  // of 16 keys: K scale, log2 V scale, 1 / V scale, 1 if the page exists
-    int page[8];   // of 16 keys, -1: not seen, or no such page
-    int from, to;  // the keys of the step that any row sees
-    int hk, pad;
+    int64_t at[8];  // of 16 keys: where their codes begin, -1: not seen, or no such page
+    int from, count;  // the keys of the step that any row sees
 };
 
 // an item's share of this CTA: `steps` of its `all` steps, from `off` on
@@ -92,11 +91,27 @@ static_assert((4 * kPrKeys + kPrRows) * 64 * 2 >= (kKvMaxRequests + 1) * 4, "the
 template <int D>
 __host__ __device__ constexpr int pr_part() { return 128 * (D + 2); }
 
-__device__ __forceinline__ bool pr_wait(uint64_t* bar, uint32_t parity, int* status, volatile int* abort_flag) {
-    if (*abort_flag) return false;
-    if (mbar_wait(bar, parity, status)) return true;
-    *abort_flag = 1;
-    return false;
+// Waits for a phase.  One that runs out of its budget records the status and
+// raises the flag, after which no wait waits: every loop here ends by itself, so
+// the kernel runs through (its results are void) and no warp is left behind.
+__device__ __forceinline__ void pr_wait(uint64_t* bar, uint32_t parity, int* status, volatile int* abort_flag) {
+    const uint32_t addr = smem_u32(bar);
+    auto ready = [&]() {
+        uint32_t ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
+        return ok != 0;
+    };
+    if (ready()) return;
+    const long long t0 = clock64();
+    while (!ready()) {
+        if (*abort_flag) return;
+        if (clock64() - t0 > kWaitBudgetCycles) {
+            set_status(status, DEV_WAIT_TIMEOUT);
+            *abort_flag = 1;
+            return;
+        }
+    }
 }
 
 __device__ __forceinline__ int64_t pr_columns(const KvAttendArgs& a, int b) {
@@ -162,18 +177,21 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint3
     return d;
 }
 
-// D[tmem] (+)= A B by one elected lane of a converged warp; A in shared memory or in TMEM
-__device__ __forceinline__ void elect_umma_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A B by one elected lane of a converged warp; A in shared memory or in TMEM.  Descriptors
+// come as their low words (address, leading offset); `hi` is the high word that all of a kind share.
+__device__ __forceinline__ void elect_umma_ss(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
-        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+        "{\n .reg .pred p, q;\n .reg .b64 da, db;\n mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %3};\n"
+        " elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n}\n" ::"r"(tmem_d),
+        "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void elect_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void elect_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
-        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+        "{\n .reg .pred p, q;\n .reg .b64 db;\n mov.b64 db, {%2, %3};\n"
+        " elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}\n" ::"r"(tmem_d),
+        "r"(tmem_a), "r"(b), "r"(hi), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void elect_commit(uint64_t* bar) {
     asm volatile(
@@ -238,10 +256,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
+template <bool INC, int N>
+__device__ __forceinline__ void set_registers() {
+    if constexpr (INC) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N));
+}
+
 template <bool E4M3, bool BF16, int D>
 __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttendArgs a) {
     constexpr int kBlk = kPrKeys * 128;        // bytes of a 64-dim block of 128 rows
     constexpr int kTile = (D / 64) * kBlk;     // a 128-row f16 tile
+    // Registers a thread: 512 x 128 at launch are handed out as 256 rows', 128 codes', 128 others'
+    constexpr int kRowRegs = D == 128 ? 184 : 192, kCodeRegs = D == 128 ? 96 : 80, kRestRegs = 48;
+    static_assert(2 * kRowRegs + kCodeRegs + kRestRegs == 512, "what the launch has");
     extern __shared__ char pr_raw[];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(pr_raw) + 1023) & ~uintptr_t(1023));
     char* vst = smem;              // 2 stages
@@ -352,20 +379,19 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
     const int64_t total = sm.scan[0];
     const int ctas = int(min(int64_t(gridDim.x), (total + kPrLeast - 1) / kPrLeast)), cta = blockIdx.x;
     const int64_t u0 = total * cta / ctas, u1 = total * (cta + 1) / ctas;
-    // TMEM columns: S0 0, S1 128, O0 256, O1 384.  Registers: 512 x 128 at launch = 256 x 184 + 128 x 88 + 128 x 56
+    // TMEM columns: S0 0, S1 128, O0 256, O1 384
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;\n");
+        set_registers<true, kRowRegs>();
         const int t = warp >> 2, r = tid & 127, f = t * 128 + r;
         const uint32_t lane_base = uint32_t(32 * (warp & 3)) << 16;
         const uint32_t ts = tm + lane_base + uint32_t(128 * t), to = tm + lane_base + uint32_t(256 + 128 * t);
         uint32_t n = 0;    // steps of this CTA so far
         uint32_t nt_n = 0; // those that this tile took part in
         uint32_t joins = 0;
-        bool ok = true;
         for (uint32_t it = 0;; ++it) {
             const PrItem& im = sm.item[it % kPrItems];
-            ok = __all_sync(0xffffffffu, pr_wait(&sm.item_full[it % kPrItems], (it / kPrItems) & 1, a.status, abort_flag));
-            if (!ok) break;
+            pr_wait(&sm.item_full[it % kPrItems], (it / kPrItems) & 1, a.status, abort_flag);
+            if (__any_sync(0xffffffffu, *abort_flag)) break;
             const int steps = im.steps;
             if (steps == 0) break;
             auto leave = [&]() {
@@ -427,10 +453,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
             int base = im.k_begin + im.off * kPrKeys;
             for (int j = 0; j < steps; ++j, ++n, ++nt_n, base += kPrKeys) {
                 const PrStep& st = sm.step[n % kPrSlots];
-                ok = pr_wait(&sm.step_full[n % kPrSlots], (n / kPrSlots) & 1, a.status, abort_flag) &&
-                     pr_wait(&sm.s_full[t], nt_n & 1, a.status, abort_flag);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                pr_wait(&sm.step_full[n % kPrSlots], (n / kPrSlots) & 1, a.status, abort_flag);
+                pr_wait(&sm.s_full[t], nt_n & 1, a.status, abort_flag);
+                __syncwarp();
                 tc_fence_after();
                 // the row's scores, read once
                 uint32_t v[4][32];
@@ -474,8 +499,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                     l *= alpha;
                     ref = nref;
                     if (j > 0) {
-                        ok = __all_sync(0xffffffffu, pr_wait(&sm.o_full[t], (nt_n - 1) & 1, a.status, abort_flag));
-                        if (!ok) break;
+                        pr_wait(&sm.o_full[t], (nt_n - 1) & 1, a.status, abort_flag);
+                        __syncwarp();
                         tc_fence_after();
                         #pragma unroll 1
                         for (int h = 0; h < D / 32; ++h) {
@@ -515,8 +540,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                 mbar_arrive(&sm.p_full[t]);
             }
             // --- the row's result ---
-            ok = ok && __all_sync(0xffffffffu, pr_wait(&sm.o_full[t], (nt_n - 1) & 1, a.status, abort_flag));
-            if (!ok) break;
+            pr_wait(&sm.o_full[t], (nt_n - 1) & 1, a.status, abort_flag);
+            __syncwarp();
             tc_fence_after();
             // 32 dims of a row from h on
             auto emit = [&](int h, const float (&o)[32], float inv) {
@@ -571,10 +596,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
             // the tile's 128 threads; bounded like every other wait, since a warp may have given up before
             auto together = [&]() {
                 mbar_arrive(&sm.join[t]);
-                ok = __all_sync(0xffffffffu, pr_wait(&sm.join[t], joins++ & 1, a.status, abort_flag));
-                return ok;
+                pr_wait(&sm.join[t], joins++ & 1, a.status, abort_flag);
             };
-            if (!together()) break;
+            together();
             if (r == 0) {
                 int prev;
                 int32_t* counter = a.counters + 2 * c0 + t;
@@ -582,7 +606,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                 sm.last[t] = prev == c1 - c0;
                 if (prev == c1 - c0) *counter = 0;  // ready for the next call
             }
-            if (!together()) break;
+            together();
             if (sm.last[t]) {
                 auto piece = [&](int c) { return a.part + (int64_t(2 * c + (c == c0 ? 1 : 0)) * 2 + t) * pr_part<D>(); };
                 float m = -INFINITY, sum = 0.f;
@@ -612,32 +636,30 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                 }
                 emit_lse(m, sum);
             }
-            if (!together()) break;  // sm.last is the next item's
+            together();  // sm.last is the next item's
             leave();
         }
         tc_fence_before();
         named_bar_arrive(1, 288);
     } else if (warp < 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
+        set_registers<false, kCodeRegs>();
         // --- codes to f16 ---
         // a thread takes 8 dims of each 64-dim block of a key: 8 lanes' 16-byte stores of one block
         // fall on 8 different places of a swizzled 128-byte row
         constexpr int NB = D / 64;
         constexpr int NP = 4;                // passes of 16 keys (of one page) to half a step
         const int ct = tid - 256, kr = ct >> 3, ch = ct & 7;
-        const int64_t page_bytes = (int64_t(Hk) * D) << a.shift;
-        const int mine = kr * D + ch * 8;
+        const uint8_t* const k_mine = a.k + kr * D + ch * 8;
+        const uint8_t* const v_mine = a.v + kr * D + ch * 8;
         auto load = [&](const uint8_t* codes, const PrStep& st, int half, uint2 (&w)[NP][NB]) {
-            const uint8_t* head = codes + ((int64_t(st.hk) * D) << a.shift) + mine;
-            const int from = st.from, to = st.to;
+            const uint32_t first = uint32_t(half * NP * 16 + kr - st.from), count = uint32_t(st.count);
             #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                const int key = (half * NP + i) * 16, pi = st.page[half * NP + i];
-                const uint8_t* p = head + pi * page_bytes + (key & (P - 1)) * D;  // steps begin at whole pages
+                const int64_t at = st.at[half * NP + i];
                 // keys that no row sees are zeros: their codes may be NaN, and 0 * NaN is not 0
-                const bool get = pi >= 0 && key + kr >= from && key + kr < to;
+                const bool get = at >= 0 && first + 16 * i < count;
                 #pragma unroll
-                for (int m = 0; m < NB; ++m) w[i][m] = load_early(p + 64 * m, get);
+                for (int m = 0; m < NB; ++m) w[i][m] = load_early(codes + at + 64 * m, get);
             }
         };
         const uint32_t place = uint32_t(kr * 128 + ((ch ^ (kr & 7)) << 4));
@@ -657,41 +679,42 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
             if (lane == 0) mbar_arrive(bar);
         };
         const uint32_t steps = uint32_t(u1 - u0);
-        auto known = [&](uint32_t n) {
-            return __all_sync(0xffffffffu, pr_wait(&sm.step_full[n % kPrSlots], (n / kPrSlots) & 1, a.status, abort_flag)) != 0;
+        auto known = [&](uint32_t n) {  // false after a wait that ran out: the slot may hold anything
+            pr_wait(&sm.step_full[n % kPrSlots], (n / kPrSlots) & 1, a.status, abort_flag);
+            return !__any_sync(0xffffffffu, *abort_flag);
         };
         // two halves are on their way while a third is written
         uint2 k0[NP][NB], k1[NP][NB], v0[NP][NB], v1[NP][NB];
         if (known(0)) {
-            load(a.k, sm.step[0], 0, k0);
-            load(a.k, sm.step[0], 1, k1);
+            load(k_mine, sm.step[0], 0, k0);
+            load(k_mine, sm.step[0], 1, k1);
             for (uint32_t n = 0; n < steps; ++n) {
                 const uint32_t s = n & 1;
-                bool ok = n < 2 || pr_wait(&sm.k_empty[s], ((n >> 1) - 1) & 1, a.status, abort_flag);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                if (n >= 2) pr_wait(&sm.k_empty[s], ((n >> 1) - 1) & 1, a.status, abort_flag);
+                __syncwarp();
                 const PrStep& st = sm.step[n % kPrSlots];
                 put(kst + s * kTile, 0, k0);
-                load(a.v, st, 0, v0);
+                load(v_mine, st, 0, v0);
                 put(kst + s * kTile, 1, k1);
-                load(a.v, st, 1, v1);
+                load(v_mine, st, 1, v1);
                 handed(&sm.k_full[s]);
                 // K of step n is in place of step n - 2's, whose products, and those of n - 3's weights, are
                 // done: every row has left step n - 3, and its slot is free
                 if (n >= 3 && lane == 0) mbar_arrive(&sm.step_free[(n - 3) % kPrSlots]);
                 const bool more = n + 1 < steps;
                 if (more && !known(n + 1)) break;
-                ok = n < 2 || pr_wait(&sm.v_empty[s], ((n >> 1) - 1) & 1, a.status, abort_flag);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                if (n >= 2) pr_wait(&sm.v_empty[s], ((n >> 1) - 1) & 1, a.status, abort_flag);
+                __syncwarp();
                 const PrStep& next = sm.step[(n + 1) % kPrSlots];
                 put(vst + s * kTile, 0, v0);
-                if (more) load(a.k, next, 0, k0);
+                if (more) load(k_mine, next, 0, k0);
                 put(vst + s * kTile, 1, v1);
-                if (more) load(a.k, next, 1, k1);
+                if (more) load(k_mine, next, 1, k1);
                 handed(&sm.v_full[s]);
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
+        set_registers<false, kRestRegs>();
         if (warp == 13) {
             // --- pages and scales: lanes 8 i .. 8 i + 7 have the 16-key groups of every fourth step from step i on ---
             PrWalk w;
@@ -701,36 +724,36 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
             for (uint32_t n0 = 0; n0 < steps; n0 += 4) {
                 const uint32_t n = n0 + (lane >> 3);
                 float4 sc = make_float4(0.f, 0.f, 1.f, 1.f);
-                int page = -1, from = 0, to = 0, hk = 0;
+                int64_t codes = -1;
+                int from = 0, count = 0;
                 if (n < steps) {
                     const int64_t u = u0 + n;
                     w.seek(a, u);
-                    hk = int((u - w.base) / w.t.steps);
+                    const int hk = int((u - w.base) / w.t.steps);
                     const int k0 = w.t.k_begin + int(u - w.base - int64_t(hk) * w.t.steps) * kPrKeys, key = k0 + 16 * g;
-                    from = max(w.t.lo - k0, 0), to = min(w.t.hi - k0, kPrKeys);
+                    from = max(w.t.lo - k0, 0), count = max(min(w.t.hi - k0, kPrKeys) - from, 0);
                     if (key + 16 > w.t.lo && key < w.t.hi) {
-                        page = __ldg(a.table + int64_t(w.b) * a.width + (key >> a.shift));
+                        const int page = __ldg(a.table + int64_t(w.b) * a.width + (key >> a.shift));
                         if (page >= 0 && page < a.pages) {
                             const int64_t at = int64_t(page) * Hk + hk;
+                            codes = ((at << a.shift) + (key & (P - 1))) * D;
                             const int ve = stored_exponent(__ldg(a.v_scale + at));
                             sc = make_float4(__ldg(a.k_scale + at), float(ve), exp2_int(-ve), 1.f);
                         } else {
                             set_status(a.status, DEV_BAD_INDEX);
-                            page = -1;
                             sc.w = 0.f;
                         }
                     }
                 }
                 // slot of step n0 + 3: the last of the four to be free
-                bool ok = true;
                 if (n < steps && n >= kPrSlots)
-                    ok = pr_wait(&sm.step_free[n % kPrSlots], (n / kPrSlots - 1) & 1, a.status, abort_flag);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                    pr_wait(&sm.step_free[n % kPrSlots], (n / kPrSlots - 1) & 1, a.status, abort_flag);
+                if (__any_sync(0xffffffffu, *abort_flag)) break;
                 if (n < steps) {
                     PrStep& st = sm.step[n % kPrSlots];
                     st.sc[g] = sc;
-                    st.page[g] = page;
-                    if (g == 0) st.from = from, st.to = to, st.hk = hk;
+                    st.at[g] = codes;
+                    if (g == 0) st.from = from, st.count = count;
                 }
                 __syncwarp();
                 if (n < steps && g == 0) mbar_arrive(&sm.step_full[n % kPrSlots]);
@@ -742,8 +765,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
             w.start(a, sm);
             int64_t u = u0;
             for (uint32_t it = 0;; ++it) {
-                bool ok = it < kPrItems || pr_wait(&sm.item_free[it % kPrItems], (it / kPrItems - 1) & 1, a.status, abort_flag);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                if (it >= kPrItems) pr_wait(&sm.item_free[it % kPrItems], (it / kPrItems - 1) & 1, a.status, abort_flag);
+                if (__any_sync(0xffffffffu, *abort_flag)) break;
                 PrItem im = {};
                 if (u < u1) {
                     w.seek(a, u);
@@ -769,57 +792,55 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
         constexpr uint32_t idesc_s = umma_idesc_f16_f32(128, kPrKeys);
         constexpr uint32_t idesc_o = umma_idesc_f16_f32(128, D) | (1u << 16);  // V: MN-major
         constexpr uint32_t kStep = kTile >> 4;
-        const uint64_t q0 = umma_desc_k_sw128(smem_u32(qs)), k0 = umma_desc_k_sw128(smem_u32(kst));
-        const uint64_t v0 = umma_desc_mn_sw128(smem_u32(vst), kBlk);
+        const uint64_t qd64 = umma_desc_k_sw128(smem_u32(qs)), vd64 = umma_desc_mn_sw128(smem_u32(vst), kBlk);
+        const uint32_t q0 = uint32_t(qd64), k0 = uint32_t(umma_desc_k_sw128(smem_u32(kst))), v0 = uint32_t(vd64);
+        const uint32_t hi_k = uint32_t(qd64 >> 32), hi_v = uint32_t(vd64 >> 32);
         auto scores = [&](int t, uint32_t s) {
-            const uint64_t qd = q0 + uint32_t(t) * kStep, kd = k0 + s * kStep;
+            const uint32_t qd = q0 + uint32_t(t) * kStep, kd = k0 + s * kStep;
             #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 const uint32_t at = uint32_t((i >> 2) * kBlk + (i & 3) * 32) >> 4;
-                elect_umma_ss(tm + 128 * t, qd + at, kd + at, idesc_s, i > 0);
+                elect_umma_ss(tm + 128 * t, qd + at, kd + at, hi_k, idesc_s, i > 0);
             }
             elect_commit(&sm.s_full[t]);
         };
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            return __all_sync(0xffffffffu, pr_wait(bar, parity, a.status, abort_flag)) != 0;
+            pr_wait(bar, parity, a.status, abort_flag);
+            __syncwarp();
         };
         uint32_t n = 0, n1 = 0, items1 = 0;  // steps so far, those with a second tile, items with one
-        bool ok = true;
-        for (uint32_t items = 0; ok;) {
-            ok = wait(&sm.item_full[items % kPrItems], (items / kPrItems) & 1);
-            if (!ok) break;
-            const int steps = sm.item[items % kPrItems].steps, nt = sm.item[items % kPrItems].rows > 128 ? 2 : 1;
+        for (uint32_t items = 0;; ++items) {
+            wait(&sm.item_full[items % kPrItems], (items / kPrItems) & 1);
+            if (__any_sync(0xffffffffu, *abort_flag)) break;
+            const int steps = __shfl_sync(0xffffffffu, sm.item[items % kPrItems].steps, 0);
+            const int nt = __shfl_sync(0xffffffffu, sm.item[items % kPrItems].rows, 0) > 128 ? 2 : 1;
             if (steps == 0) break;
-            __syncwarp();
             if (lane == 0) mbar_arrive(&sm.item_free[items % kPrItems]);
-            ok = wait(&sm.k_full[n & 1], (n >> 1) & 1);
-            for (int t = 0; ok && t < nt; ++t) {
-                ok = wait(&sm.q_full[t], (t ? items1 : items) & 1);
-                if (!ok) break;
+            __syncwarp();
+            wait(&sm.k_full[n & 1], (n >> 1) & 1);
+            for (int t = 0; t < nt; ++t) {
+                wait(&sm.q_full[t], (t ? items1 : items) & 1);
                 tc_fence_after();
                 scores(t, n & 1);
             }
-            if (!ok) break;
             elect_commit(&sm.k_empty[n & 1]);
-            ++items, items1 += nt - 1;
+            items1 += nt - 1;
             for (int j = 0; j < steps; ++j, ++n, n1 += nt - 1) {
                 const uint32_t s = n & 1, sn = s ^ 1;
                 const bool more = j + 1 < steps;
-                if (more) ok = wait(&sm.k_full[sn], ((n + 1) >> 1) & 1);
-                ok = ok && wait(&sm.v_full[s], (n >> 1) & 1);
-                for (int t = 0; ok && t < nt; ++t) {
-                    const uint64_t vd = v0 + s * kStep;
-                    ok = wait(&sm.p_full[t], (t ? n1 : n) & 1);
-                    if (!ok) break;
+                if (more) wait(&sm.k_full[sn], ((n + 1) >> 1) & 1);
+                wait(&sm.v_full[s], (n >> 1) & 1);
+                for (int t = 0; t < nt; ++t) {
+                    const uint32_t vd = v0 + s * kStep;
+                    wait(&sm.p_full[t], (t ? n1 : n) & 1);
                     tc_fence_after();
                     #pragma unroll
                     for (int i = 0; i < kPrKeys / 16; ++i)
-                        elect_umma_ts(tm + 256 + 128 * t, tm + 128 * t + 8 * i, vd + uint32_t(2048 * i >> 4), idesc_o,
+                        elect_umma_ts(tm + 256 + 128 * t, tm + 128 * t + 8 * i, vd + uint32_t(2048 * i >> 4), hi_v, idesc_o,
                                       i > 0 ? 1u : uint32_t(j > 0));
                     elect_commit(&sm.o_full[t]);
                     if (more) scores(t, sn);
                 }
-                if (!ok) break;
                 elect_commit(&sm.v_empty[s]);
                 if (more) elect_commit(&sm.k_empty[sn]);
             }
