@@ -188,8 +188,27 @@ __device__ __forceinline__ float2 pair_to_float(uint32_t v) {
     else return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// the larger magnitude of two pairs, NaN if either is
+template <bool BF16>
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+    a &= 0x7fff7fffu, b &= 0x7fff7fffu;
+    if constexpr (BF16) {
+        const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&m);
+    } else {
+        const __half2 m = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&m);
+    }
+}
+
 template <bool E4M3, bool BF16, int D, int THREADS>
-__global__ void __launch_bounds__(THREADS, 768 / THREADS) kv_append_kernel(const KvAppendArgs a) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv_append_kernel(const KvAppendArgs a) {
     constexpr int LPR = D / 8;              // lanes per row (8 values each)
     constexpr int RPW = 32 / LPR;           // rows per warp and iteration; even rows are K's, odd ones V's
     constexpr int kWarps = THREADS / 32;
@@ -240,13 +259,27 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) kv_append_kernel(const
     float* scales = which ? a.scale[1] : a.scale[0];
     // Rows of tokens first + row / 2 (K where even): this lane's are row0, row0 + step, ...
     uint4 v[kAppendHold];
+    // over the lanes of a row, and over the warp's rows of the same kind; NaN if one is
+    auto over_lanes = [&](float m) {
+        #pragma unroll
+        for (int d = 1; d < LPR; d <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+        return RPW == 4 ? max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2 * LPR)) : m;
+    };
     auto load = [&](int first, int n, int row0, int step) {  // and their largest magnitude
-        float m = 0.f;
         #pragma unroll
         for (int i = 0; i < kAppendHold; ++i) {
             const int t = (row0 + i * step) >> 1;
             v[i] = t < n ? __ldg(reinterpret_cast<const uint4*>(x + (w0 + first + t) * ts)) : make_uint4(0, 0, 0, 0);
         }
+        uint32_t m = 0;
+        #pragma unroll
+        for (int i = 0; i < kAppendHold; ++i)
+            m = max_abs2<BF16>(m, max_abs2<BF16>(max_abs2<BF16>(v[i].x, v[i].y), max_abs2<BF16>(v[i].z, v[i].w)));
+        const float2 f = pair_to_float<BF16>(m);
+        return over_lanes(max_nan(fabsf(f.x), fabsf(f.y)));
+    };
+    auto largest_number = [&]() {  // of rows with NaN in them
+        float m = 0.f;
         #pragma unroll
         for (int i = 0; i < kAppendHold; ++i) {
             const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
@@ -256,12 +289,11 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) kv_append_kernel(const
                 m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));  // fmaxf leaves NaN out
             }
         }
-        #pragma unroll
-        for (int d = 1; d < LPR; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        if (RPW == 4) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2 * LPR));
-        return m;
+        return over_lanes(m);
     };
-    auto code = [&](int first, int n, int row0, int step, int e) {
+    // ODD: there may be NaN, or numbers beyond what the largest scale brings into the codes' range
+    auto code = [&](auto odd, int first, int n, int row0, int step, int e) {
+        constexpr bool ODD = decltype(odd)::value;
         const float inv = exp2_int(-e);
         const int64_t s = slot[first + 1];
         const int64_t base = (((s >> sh) * a.heads + h) << sh) + (s & (P - 1));
@@ -270,28 +302,39 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) kv_append_kernel(const
             const int t = (row0 + i * step) >> 1;
             const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
             float f[8];
-            bool nan = false;
             #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const float2 p = pair_to_float<BF16>(w[q]);
-                nan |= p.x != p.x || p.y != p.y;
                 f[2 * q] = p.x * inv, f[2 * q + 1] = p.y * inv;
             }
             uint2 c;
-            if constexpr (E4M3) {
-                // A NaN of V goes into the token's key instead: every row that sees the token becomes
-                // NaN, and no other (0 * NaN would reach those that do not).
-                uint32_t bad = __ballot_sync(0xffffffffu, nan && which);
-                bad = (bad >> ((sub | 1) * LPR)) & ((1u << LPR) - 1u);
-                if (bad) {
+            if constexpr (!ODD && !E4M3) {
+                // x / s + 1.5 * 2^23 has the rounded code in its low byte
+                uint32_t b[8];
+                #pragma unroll
+                for (int q = 0; q < 8; ++q) b[q] = __float_as_uint(f[q] + 12582912.f);
+                c.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+                c.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+            } else {
+                if constexpr (ODD && E4M3) {
+                    // A NaN of V goes into the token's key instead: every row that sees the token becomes
+                    // NaN, and no other (0 * NaN would reach those that do not).
+                    bool nan = false;
                     #pragma unroll
-                    for (int q = 0; q < 8; ++q) f[q] = which ? (f[q] == f[q] ? f[q] : 0.f) : NAN;
+                    for (int q = 0; q < 8; ++q) nan |= f[q] != f[q];
+                    uint32_t bad = __ballot_sync(0xffffffffu, nan && which);
+                    bad = (bad >> ((sub | 1) * LPR)) & ((1u << LPR) - 1u);
+                    if (bad) {
+                        #pragma unroll
+                        for (int q = 0; q < 8; ++q) f[q] = which ? (f[q] == f[q] ? f[q] : 0.f) : NAN;
+                    }
                 }
+                c.x = encode4<E4M3>(f[0], f[1], f[2], f[3]), c.y = encode4<E4M3>(f[4], f[5], f[6], f[7]);
             }
-            c.x = encode4<E4M3>(f[0], f[1], f[2], f[3]), c.y = encode4<E4M3>(f[4], f[5], f[6], f[7]);
             if (t < n) *reinterpret_cast<uint2*>(cache + (base + t) * D) = c;
         }
     };
+    constexpr float kMost = (E4M3 ? 448.f : 127.f) * 1099511627776.f;  // at the largest scale, 2^40
     // the scale of the run's tile, and the one it had
     auto settle = [&](int first, float m, int& old) {
         const int64_t s = slot[first + 1];
@@ -331,12 +374,15 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) kv_append_kernel(const
             longs = true;
             continue;
         }
-        const float m = load(first, n, sub, RPW);
+        float m = load(first, n, sub, RPW);
+        const bool odd = __any_sync(0xffffffffu, !(m <= kMost));
+        if (odd) m = largest_number();
         int old;
         const int e = settle(first, m, old);
         __syncwarp();
         if (lane % LPR == 0 && sub < 2) publish(first, e);
-        code(first, n, sub, RPW, e);
+        if (odd) code(std::true_type(), first, n, sub, RPW, e);
+        else code(std::false_type(), first, n, sub, RPW, e);
         if (old < e) again(first, sub, RPW, old, e);
     }
     if (!__syncthreads_or(longs)) return;
@@ -346,13 +392,23 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) kv_append_kernel(const
         if (tid < 2) amax[tid] = 0;
         __syncthreads();
         const float m = load(first, n, warp * RPW + sub, kWarps * RPW);
-        if (lane % LPR == 0 && sub < 2) atomicMax(&amax[which], __float_as_int(m));  // of floats >= 0
+        if (lane % LPR == 0 && sub < 2) atomicMax(&amax[which], __float_as_int(m));  // of floats >= 0; NaN is the largest
         __syncthreads();
+        const bool odd = !(__int_as_float(amax[0]) <= kMost && __int_as_float(amax[1]) <= kMost);
+        if (odd) {
+            const float number = largest_number();
+            __syncthreads();
+            if (tid < 2) amax[tid] = 0;
+            __syncthreads();
+            if (lane % LPR == 0 && sub < 2) atomicMax(&amax[which], __float_as_int(number));
+            __syncthreads();
+        }
         int old;
         const int e = settle(first, __int_as_float(amax[which]), old);
         __syncthreads();  // all have read the old scale
         if (warp == 0 && lane % LPR == 0 && sub < 2) publish(first, e);
-        code(first, n, warp * RPW + sub, kWarps * RPW, e);
+        if (odd) code(std::true_type(), first, n, warp * RPW + sub, kWarps * RPW, e);
+        else code(std::false_type(), first, n, warp * RPW + sub, kWarps * RPW, e);
         if (old < e) again(first, warp * RPW + sub, kWarps * RPW, old, e);
     }
 }
