@@ -41,6 +41,8 @@ namespace exl3 {
 constexpr int kAttWarps = 8, kAttThreads = kAttWarps * 32, kAttUnit = 16 * kAttWarps;
 constexpr float kAttSlack = 8.f;  // log2: growth of the maximum that is let pass
 
+constexpr int kAttMaxSms = 160;     // SMs that are used at most
+
 // Tiles of 8 query columns an item has at most: up to two with two CTAs per
 // SM; three or four need the registers of one.
 template <int D, int NT>
@@ -51,7 +53,8 @@ struct AttShape {
     static constexpr int kStages = (NT <= 2 ? 3 : 6) * 128 / D;   // 96 KB of ring per CTA, 192 KB where it is alone
     static constexpr int kRing = kAttWarps * kStages * 2 * kTile;
     static constexpr int kRed = kAttWarps * NC * D * 4;           // the warps' outputs take the ring's place
-    static_assert(kRed <= kRing, "the ring holds the join");
+    // the ring holds the join of the warps, and that of the pieces: one per CTA at most, of up to kAttMaxSms SMs
+    static_assert(kRed <= kRing && kAttMaxSms * kCtas * 2 * NC * 4 <= kRing, "the joins fit the ring");
     static constexpr int kQ = NT * (D / 16) * 32 * 8;             // Q fragments
     static constexpr int kSmem = kRing + kQ + (2 * kAttWarps * NC + 3 * NC) * 4 + kAttWarps * kStages * 8;
 };
@@ -110,6 +113,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
     float2* tile_sc = reinterpret_cast<float2*>(qfac + NC);  // [warps][S] a tile's K and V scale
     __shared__ int64_t scan[kAttWarps];
     __shared__ int64_t found_base;
+    __shared__ AttReq found;
     __shared__ int found_b, last_flag;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
@@ -118,11 +122,12 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
     // --- this CTA's share of the line of units ---
     const int per = (a.requests + kAttThreads - 1) / kAttThreads;
     int64_t mine = 0;
+    AttReq own = {};
     for (int i = 0; i < per; ++i) {
         const int b = tid * per + i;
         if (b < a.requests) {
-            const AttReq r = att_request<NC>(a, b);
-            mine += int64_t(r.groups) * Hk * r.units;
+            own = att_request<NC>(a, b);
+            mine += int64_t(own.groups) * Hk * own.units;
         }
     }
     int64_t incl = mine;
@@ -157,9 +162,12 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
         int64_t base = incl - mine;
         int b = tid * per;
         for (;;) {
-            const AttReq r = att_request<NC>(a, b);
+            const AttReq r = per == 1 ? own : att_request<NC>(a, b);
             const int64_t n = int64_t(r.groups) * Hk * r.units;
-            if (u < base + n) break;
+            if (u < base + n) {
+                found = r;
+                break;
+            }
             base += n, ++b;
         }
         found_b = b, found_base = base;
@@ -167,7 +175,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
     __syncthreads();
     int b = found_b;
     int64_t base = found_base;
-    AttReq rq = att_request<NC>(a, b);
+    AttReq rq = found;
 
     while (u < u_end) {
         while (u >= base + int64_t(rq.groups) * Hk * rq.units) {  // next request with work
@@ -487,15 +495,21 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
             __syncthreads();
             if (last_flag) {
                 auto piece = [&](int p) { return a.part + int64_t(2 * (c0 + p) + (p == 0 ? 1 : 0)) * PART; };
-                float* wt = red;  // [pieces][NC] weights
+                float* wt = red;                   // [pieces][NC] maxima, then weights
+                float* wsum = red + pieces * NC;   // [pieces][NC] sums
+                for (int i = tid; i < pieces * NC; i += kAttThreads) {
+                    const float* pc = piece(i / NC);
+                    wt[i] = __ldcg(pc + i % NC), wsum[i] = __ldcg(pc + NC + i % NC);
+                }
+                __syncthreads();
                 if (tid < NC) {
                     float mx = -INFINITY, sum = 0.f;
-                    for (int p = 0; p < pieces; ++p) mx = fmaxf(mx, __ldcg(piece(p) + tid));
+                    for (int p = 0; p < pieces; ++p) mx = fmaxf(mx, wt[p * NC + tid]);
                     const float ref = mx == -INFINITY ? 0.f : mx;
                     for (int p = 0; p < pieces; ++p) {
-                        const float f = ex2(__ldcg(piece(p) + tid) - ref);
+                        const float f = ex2(wt[p * NC + tid] - ref);
                         wt[p * NC + tid] = f;
-                        sum = fmaf(__ldcg(piece(p) + NC + tid), f, sum);
+                        sum = fmaf(wsum[p * NC + tid], f, sum);
                     }
                     fin[tid] = mx, fin[NC + tid] = sum;
                 }
@@ -503,7 +517,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
                 for (int i = tid; i < NC * D; i += kAttThreads) {
                     const int col = i / D;
                     float v = 0.f;
-                    #pragma unroll 4
+                    #pragma unroll 8
                     for (int p = 0; p < pieces; ++p) v = fmaf(__ldcg(piece(p) + 2 * NC + i), wt[p * NC + col], v);
                     emit(col, i % D, v, fin[NC + col], fin[col]);
                 }
@@ -537,7 +551,7 @@ static cudaError_t launch_attend(const KvAttendArgs& a, int sms, cudaStream_t s)
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = raise_smem(kernel, Shape::kSmem, done);
     if (e != cudaSuccess) return e;
-    kernel<<<sms * Shape::kCtas, kAttThreads, Shape::kSmem, s>>>(a);
+    kernel<<<(sms < kAttMaxSms ? sms : kAttMaxSms) * Shape::kCtas, kAttThreads, Shape::kSmem, s>>>(a);
     return cudaGetLastError();
 }
 
