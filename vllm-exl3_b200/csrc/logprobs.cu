@@ -10,7 +10,7 @@
 // Bound: every logit is read once: HBM (bf16: about 12 logits per clock and SM
 // at the measured copy rate, near the 16 per clock of the exponential unit).
 // A CTA streams a slice of one row, each thread 4 16-byte vectors at a time
-// with the next 4 on their way.  A thread's reference m follows its maximum
+// with the next 4 on their way (cp.async: 64 KB per SM without a register).  A thread's reference m follows its maximum
 // only when that has grown by more than 16: sums of exp(d <= 16) are as exact,
 // and the loop has no dependent rescaling.  Few rows: a row is split over CTAs
 // and joined by the one that ends last, always in the same order.
@@ -32,13 +32,13 @@
 namespace exl3 {
 
 constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
-constexpr int kLpUnroll = 4;     // vectors of a thread in flight, and in work
+constexpr int kLpUnroll = 4;     // vectors of a thread in work
+constexpr int kLpStages = 2;     // such sets in shared memory, on their way (3: 102.5 us where 2 take 100.8)
 constexpr int kLpMaxTop = 32;    // one group maximum each
 constexpr int kLpRound = kLpThreads * 8;               // most entries that one round of candidates looks at
 constexpr int kLpCap = kLpRound + 2 * kLpMaxTop;       // candidate keys a CTA holds
 constexpr float kLpSlack = 16.f;                       // growth of the maximum that the reference lets pass
 constexpr int kLpMaxSplit = 64;
-constexpr int kLpSplitRows = 32;  // rows per SM up to which rows are split
 static_assert(kLpMaxSplit * kLpMaxTop <= kLpCap, "the parts' lists are joined in one buffer");
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -207,9 +207,9 @@ template <int DT, bool TOP>
 __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a) {
     using T = LpType<DT>;
     constexpr int VEC = T::kVec, U = kLpUnroll;
-    extern __shared__ uint64_t lp_smem[];
-    uint64_t* cand = lp_smem;            // [kLpCap]
-    uint64_t* best = lp_smem + kLpCap;   // [kLpMaxSplit], at least kLpMaxTop
+    extern __shared__ __align__(16) uint4 lp_ring[];                  // [kLpStages][U][threads]
+    uint64_t* cand = reinterpret_cast<uint64_t*>(lp_ring);            // [kLpCap], once the ring is done with
+    uint64_t* best = cand + kLpCap;                                   // [kLpMaxSplit], at least kLpMaxTop
     __shared__ uint32_t group_max[32];
     __shared__ uint16_t flagged[kLpThreads];
     __shared__ float wr[kLpWarps], ws[kLpWarps], ww[kLpWarps];
@@ -258,19 +258,32 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
         if (i < tok) st.above += lowest ? -int(v > xt) : int(v == xt);
     }
 
-    auto fetch = [&](uint4 (&v)[U], int j) {
+    // a thread's vectors go through places of its own in shared memory: no barrier
+    const uint32_t ring = smem_u32(lp_ring) + tid * 16;
+    auto fetch = [&](int j, int stage) {
         #pragma unroll
         for (int u = 0; u < U; ++u)
-            v[u] = j + u * kLpThreads < v1 ? __ldg(vecs + j + u * kLpThreads) : make_uint4(T::kNone, T::kNone, T::kNone, T::kNone);
+            if (j + u * kLpThreads < v1)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(ring + (stage * U + u) * (kLpThreads * 16)),
+                             "l"(vecs + j + u * kLpThreads) : "memory");
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
     };
-    uint4 next[U];
-    fetch(next, v0 + tid);
+    #pragma unroll
+    for (int i = 0; i < kLpStages - 1; ++i) fetch(v0 + i * U * kLpThreads + tid, i);
+    int stage = 0;
     #pragma unroll 1
     for (int j0 = v0; j0 < v1; j0 += U * kLpThreads) {
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(kLpStages - 2) : "memory");
         uint4 v[U];
         #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = next[u];
-        fetch(next, j0 + U * kLpThreads + tid);
+        for (int u = 0; u < U; ++u) v[u] = lp_ring[(stage * U + u) * kLpThreads + tid];
+        fetch(j0 + (kLpStages - 1) * U * kLpThreads + tid, stage == 0 ? kLpStages - 1 : stage - 1);
+        stage = stage == kLpStages - 1 ? 0 : stage + 1;
+        if (j0 + U * kLpThreads > v1) {
+            #pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j0 + tid + u * kLpThreads >= v1) v[u] = make_uint4(T::kNone, T::kNone, T::kNone, T::kNone);
+        }
         float mx = T::largest(v[0]);
         #pragma unroll
         for (int u = 1; u < U; ++u) mx = fmaxf(mx, T::largest(v[u]));
@@ -319,6 +332,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
         gm = max(gm, __shfl_xor_sync(0xffffffffu, gm, 4));
         if ((lane & 7) == 0) group_max[tid >> 3] = gm;
         if (tid == 0) count = 0, n_flagged = 0, bound = 0;
+        asm volatile("cp.async.wait_all;\n" ::: "memory");
         __syncthreads();
         if (warp == 0) {
             const uint32_t g = group_max[lane];
@@ -433,33 +447,35 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpArgs a)
     }
 }
 
-// Over how many CTAs a row is split.  Few rows: as many as run at once (4 per
-// SM), no less than two vectors a thread.  Many rows: where whole rows would
-// leave the last wave mostly empty and are long, up to 4 parts, each counted as
-// 3 % of a wave more (its start and the join): 2048 rows of 131072 bf16 are
-// 3.46 waves of 592 and take LP_A us whole, LP_B us in halves.
+// Over how many CTAs a row is split: as many as run at once (4 per SM), no
+// less than two vectors a thread.  More rows than half of that are not split:
+// the join costs more than the last wave's empty places (2048 rows of 131072
+// bf16, 3.46 waves: 101 us whole, 117 us in halves).
 static int lp_splits(const LogprobsCall& c, int sms) {
-    const int64_t vectors = c.vocab / (c.x_dtype == DT_F32 ? 4 : 8), slots = 4 * int64_t(sms);
-    if (c.rows <= 2 * sms) {
-        const int64_t want = slots / c.rows, most = vectors / (2 * kLpThreads);
-        const int64_t n = want < most ? want : most;
-        return int(n < 1 ? 1 : n > kLpMaxSplit ? kLpMaxSplit : n);
-    }
-    int best = 1;
-    double least = 0.;
-    for (int n = 1; n <= 4 && (n == 1 || (vectors >= int64_t(n) * 16 * kLpThreads && c.rows <= kLpSplitRows * sms)); ++n) {
-        const double t = double((c.rows * n + slots - 1) / slots) / n * (1. + 0.03 * (n - 1));
-        if (n == 1 || t < least) best = n, least = t;
-    }
-    return best;
+    const int64_t vectors = c.vocab / (c.x_dtype == DT_F32 ? 4 : 8);
+    const int64_t want = 4 * int64_t(sms) / c.rows, most = vectors / (2 * kLpThreads);
+    const int64_t n = want < most ? want : most;
+    return int(n < 1 ? 1 : n > kLpMaxSplit ? kLpMaxSplit : n);
 }
 
 // one per row that can be split
-int logprobs_counters(int sms) { return kLpSplitRows * sms; }
+int logprobs_counters(int sms) { return 2 * sms; }
 
 size_t logprobs_workspace(const LogprobsCall& c, int sms) {
     const int splits = lp_splits(c, sms);
     return splits > 1 ? size_t(c.rows) * splits * (16 + 8 * size_t(c.top)) : 0;
+}
+
+template <int DT, bool TOP>
+static cudaError_t launch_logprobs(const LpArgs& a, unsigned grid, cudaStream_t s) {
+    constexpr size_t smem = size_t(kLpStages) * kLpUnroll * kLpThreads * 16;
+    static_assert(smem >= size_t(kLpCap + kLpMaxSplit) * 8, "the candidates take the ring's place");
+    auto* kernel = logprobs_kernel<DT, TOP>;
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = raise_smem(kernel, smem, done);
+    if (e != cudaSuccess) return e;
+    kernel<<<grid, kLpThreads, smem, s>>>(a);
+    return cudaGetLastError();
 }
 
 cudaError_t run_logprobs(const LogprobsCall& c, int sms, cudaStream_t s) {
@@ -472,17 +488,14 @@ cudaError_t run_logprobs(const LogprobsCall& c, int sms, cudaStream_t s) {
     a.top_logprobs = c.top_logprobs, a.top_ids = c.top_ids, a.counters = c.counters;
     a.stats = reinterpret_cast<float4*>(c.ws);
     a.keys = reinterpret_cast<uint64_t*>(c.ws + size_t(c.rows) * a.splits * 16);
-    const size_t smem = c.top ? size_t(kLpCap + kLpMaxSplit) * 8 : 0;
     const unsigned grid = unsigned(c.rows * a.splits);
     const auto go = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (c.top) logprobs_kernel<DT, true><<<grid, kLpThreads, smem, s>>>(a);
-        else logprobs_kernel<DT, false><<<grid, kLpThreads, smem, s>>>(a);
+        return c.top ? launch_logprobs<DT, true>(a, grid, s) : launch_logprobs<DT, false>(a, grid, s);
     };
-    if (c.x_dtype == DT_F32) go(std::integral_constant<int, DT_F32>());
-    else if (c.x_dtype == DT_F16) go(std::integral_constant<int, DT_F16>());
-    else go(std::integral_constant<int, DT_BF16>());
-    return cudaGetLastError();
+    if (c.x_dtype == DT_F32) return go(std::integral_constant<int, DT_F32>());
+    if (c.x_dtype == DT_F16) return go(std::integral_constant<int, DT_F16>());
+    return go(std::integral_constant<int, DT_BF16>());
 }
 
 }  // namespace exl3
