@@ -109,6 +109,25 @@ def test_packed_structs_match_the_header():
         assert getattr(lib, "exl3_" + name)(None, None) == ARG and "null" in err()
 
 
+def test_binding_loads_and_steps_aside():
+    """The compiled short way is there, and takes nothing it should not: CPU tensors, wrong kinds, wrong counts."""
+    import torch
+    from exl3_b200 import _native
+    short = _native.binding()
+    assert short is not _native._NoBinding and short.__name__ == "_serving_py"
+    t, f = torch.zeros(1, dtype=torch.int32), torch.zeros(2, 4)
+    c, s = torch.zeros(1, 1, 16, 64, dtype=torch.int8), torch.zeros(1, 1)
+    assert short.kv_plan(t, t, t.view(1, 1), t, t, 16, 1) is None
+    assert short.kv_plan(t, t, t.view(1, 1), t, t, 16, 1.5) is None
+    assert short.kv_append(f, f, t, c, c, s, s) is None
+    assert short.kv_attend(f, c, c, s, s, t.view(1, 1), t, None, 1, None, 0, False) is None
+    assert short.token_logprobs(f, t, 1) is None
+    assert short.token_logprobs(f, "tokens", 1) is None
+    assert short.token_logprobs(f, t, 1 << 70) is None
+    with pytest.raises(TypeError):
+        short.kv_plan(t)
+
+
 def test_cpu_tensors_fail_loudly():
     import torch
     from exl3_b200 import kv_cache, logprobs

@@ -8,6 +8,8 @@ torch's current stream of the tensors' device.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import struct
 import threading
@@ -120,6 +122,40 @@ def load():
             fn.argtypes = args
         _lib = lib
         return lib
+
+
+class _NoBinding:
+    """Stands for the serving binding where it could not be built or loaded: every call takes the long way."""
+
+    @staticmethod
+    def _none(*args):
+        return None
+
+    kv_plan = kv_append = kv_attend = token_logprobs = _none
+
+
+_binding = None
+
+
+def binding():
+    """The compiled short way into the serving entries (``_serving_py.so``).
+    Its functions return None where a call needs the checks or copies of the
+    Python function, which is complete without them."""
+    global _binding
+    if _binding is None:
+        lib = load()
+        try:
+            path = _build.build_binding()
+            loader = importlib.machinery.ExtensionFileLoader("_serving_py", path)
+            mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_serving_py", loader))
+            loader.exec_module(mod)
+            names = ("kv_plan", "kv_append", "kv_attend", "kv_attend_workspace_size", "token_logprobs",
+                     "token_logprobs_workspace_size")
+            mod.setup(*(ctypes.cast(getattr(lib, "exl3_" + n), P).value for n in names), serve_workspace, check)
+            _binding = mod
+        except (OSError, RuntimeError, ImportError):
+            _binding = _NoBinding
+    return _binding
 
 
 def last_error() -> str:

@@ -1,4 +1,5 @@
-"""Build the sm_100a shared library ``libexl3_b200.so`` in-tree with nvcc.
+"""Build the sm_100a shared library ``libexl3_b200.so`` in-tree with nvcc, and
+``_serving_py.so``, the short way from Python into its serving entries, with g++.
 
 The library exports the C ABI declared in ``include/exl3_b200.h``; it is
 loaded with ctypes by :mod:`exl3_b200._native`.  The CUDA runtime is linked
@@ -16,6 +17,8 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(ROOT, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libexl3_b200.so")
+BINDING_SRC = os.path.join(CSRC, "serving_py.cpp")
+BINDING_PATH = os.path.join(PKG_DIR, "_serving_py.so")
 
 SOURCES = ["capi.cu", "moe.cu", "reconstruct.cu", "noalloc.cu", "tc_gemm.cu", "ep.cu", "ngram.cu",
            "kv_cache.cu", "kv_attend.cu", "kv_prompt.cu", "logprobs.cu"]
@@ -39,6 +42,32 @@ def _nvcc() -> str:
 def _inputs() -> list[str]:
     hdr = os.path.join(os.path.dirname(ROOT), "include", "exl3_b200.h")
     return [os.path.join(CSRC, s) for s in SOURCES + HEADERS] + [hdr]
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    """Compile the serving binding against this interpreter and its torch."""
+    hdr = os.path.join(os.path.dirname(ROOT), "include", "exl3_b200.h")
+    if not force and os.path.exists(BINDING_PATH) and \
+            os.path.getmtime(BINDING_PATH) >= max(os.path.getmtime(p) for p in (BINDING_SRC, hdr)):
+        return BINDING_PATH
+    import sysconfig
+
+    import torch
+    home = os.path.dirname(torch.__file__)
+    include = [sysconfig.get_paths()["include"], os.path.join(home, "include"),
+               os.path.join(home, "include", "torch", "csrc", "api", "include"),
+               os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")]
+    tmp = BINDING_PATH + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{i}" for i in include),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", BINDING_SRC, "-o", tmp,
+           f"-L{os.path.join(home, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed ({res.returncode}):\n{res.stderr[-4000:]}")
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
 
 
 def up_to_date() -> bool:
@@ -65,3 +94,4 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 if __name__ == "__main__":
     print(build(force=True, verbose=True))
+    print(build_binding(force=True, verbose=True))

@@ -34,9 +34,10 @@ class KvPlan(NamedTuple):
     cursor: torch.Tensor     # int32 [1] the free list's cursor after the step
 
 
-# The operators run for a few microseconds, so a call first asks whether all is
-# well in one expression; only a call that is not goes through _explain, which
-# says what is wrong.
+# The operators run for a few microseconds.  A call whose arguments are as the
+# kernels want them goes the compiled way (_native.binding); one that needs a
+# copy, another device or a refusal goes the way written out here.  It asks
+# whether all is well in one expression; _explain says what is not.
 
 def _explain(who: str, *wrong: tuple[bool, str]):
     for bad, what in wrong:
@@ -62,6 +63,9 @@ def kv_plan(lens: torch.Tensor, new_tokens: torch.Tensor, block_table: torch.Ten
     successors.  A free list or a table that runs out gives slots of -1 and
     records status 7 (``vllm_exl3_c.device_status``).
     """
+    short = _n.binding().kv_plan(lens, new_tokens, block_table, free_pages, cursor, page_size, n_tokens)
+    if short is not None:
+        return KvPlan(*short)
     B = lens.numel()
     if not (lens.is_cuda and new_tokens.is_cuda and block_table.is_cuda and free_pages.is_cuda and cursor.is_cuda
             and _is_i32(lens) and _is_i32(new_tokens) and _is_i32(free_pages) and _is_i32(cursor)
@@ -140,6 +144,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
     In e4m3 a NaN of ``v`` is kept in the token's key (attention rows that see
     the token become NaN, others do not); int8 has no NaN and takes 0.
     """
+    if _n.binding().kv_append(k, v, slots, k_cache, v_cache, k_scale, v_scale):
+        return
     n = slots.numel()
     x = _ROWS.get(k.dtype)
     if not (_cache_ok(k_cache, v_cache, k_scale, v_scale) and k.is_cuda and v.is_cuda and slots.is_cuda
@@ -188,6 +194,10 @@ def kv_attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
     ``window`` keys, its own included (0: no limit); ``scale`` defaults to
     dim ** -0.5.  Rows that see no key are zeros (lse -inf).
     """
+    short = _n.binding().kv_attend(q, k_cache, v_cache, k_scale, v_scale, block_table, kv_lens, cu_tokens, max_new,
+                                   scale, window, return_lse)
+    if short is not None:
+        return short
     x = _ROWS.get(q.dtype)
     B = kv_lens.numel()
     if not (_cache_ok(k_cache, v_cache, k_scale, v_scale) and q.is_cuda and block_table.is_cuda and kv_lens.is_cuda

@@ -34,6 +34,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     ``tokens`` (int32 or int64 [rows]) in one pass over the logits, computed in
     fp32.  Equal logits rank lowest index first.  Tokens outside the vocabulary
     (padding) get logprob -inf and rank 0.  ``top``: 0 to 32 alternatives."""
+    short = _n.binding().token_logprobs(logits, tokens, top)
+    if short is not None:
+        return TokenLogprobs(*short)
     x, ids = _LOGITS.get(logits.dtype), _IDS.get(tokens.dtype)
     if not (logits.is_cuda and tokens.is_cuda and x is not None and ids is not None and logits.dim() == 2
             and tokens.shape == logits.shape[:1] and 0 <= top <= MAX_TOP and top <= logits.size(1)):
