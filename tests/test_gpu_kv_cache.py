@@ -415,6 +415,24 @@ def test_cache_object_steps(native, cuda):
     assert cache.lens.tolist() == [1, 52, 36]
 
 
+def test_operators_share_a_workspace(native, cuda):
+    """Log probabilities of split rows between attention calls of every kind: each leaves the shared counters zero."""
+    import torch
+    from exl3_b200.logprobs import token_logprobs
+    few = _problem(cuda, [3000, 500], [1, 2], heads=8, kv_heads=2, dim=64, page=16, x="f16", code="int8")
+    many = _problem(cuda, [900, 700], [300, 650], heads=8, kv_heads=2, dim=128, page=16, x="bf16", code="e4m3", seed=5)
+    logits = torch.randn(3, 120001, device=cuda)
+    tok = torch.tensor([1, 2, 3], device=cuda)
+    want = [_attend(cuda, few)[0], _attend(cuda, many)[0], token_logprobs(logits, tok, top=20)]
+    for order in ((2, 0, 2, 1, 2), (2, 1, 0, 2, 2), (1, 2, 1, 0, 2), (0, 0, 2, 1, 1)):
+        for i in order:
+            if i == 2:
+                got = token_logprobs(logits, tok, top=20)
+                assert all(torch.equal(a, b) for a, b in zip(got, want[2]))
+            else:
+                assert torch.equal(_attend(cuda, (few, many)[i])[0], want[i])
+
+
 def test_refusals(native, cuda):
     import torch
     kv = _kv()

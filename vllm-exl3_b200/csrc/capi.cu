@@ -612,9 +612,13 @@ static int check_cache(const char* who, const void* k, const void* v, const floa
 
 static_assert(exl3::kKvMaxRequests == EXL3_KV_MAX_REQUESTS, "one limit");
 
-// status word, counters and partial results of a serving workspace
+// A serving workspace: status word, counters, partial results.  The entries share
+// it, so the counters, which each leaves zero, have the same place for all.
 static constexpr size_t kServeCounters = 256;
-static size_t serve_partials(int n_counters) { return (kServeCounters + size_t(n_counters) * 4 + 255) & ~size_t(255); }
+static size_t serve_partials(int sms) {
+    const int a = exl3::kv_attend_counters(sms), b = exl3::logprobs_counters(sms);
+    return (kServeCounters + size_t(a > b ? a : b) * 4 + 255) & ~size_t(255);
+}
 
 int exl3_kv_plan(const exl3_kv_plan_args* a, void* stream) {
     const char* who = "exl3_kv_plan";
@@ -669,7 +673,7 @@ size_t exl3_kv_attend_workspace_size(int heads, int kv_heads, int dim, int max_n
     exl3::KvAttendCall c;
     c.heads = heads, c.kv_heads = kv_heads, c.dim = dim, c.max_new = max_new, c.requests = requests, c.q_rows = q_rows;
     const int sms = exl3::num_sms_cached();
-    return serve_partials(exl3::kv_attend_counters(sms)) + exl3::kv_attend_workspace(c, sms);
+    return serve_partials(sms) + exl3::kv_attend_workspace(c, sms);
 }
 
 int exl3_kv_attend(const exl3_kv_attend_args* a, void* stream) {
@@ -704,7 +708,7 @@ int exl3_kv_attend(const exl3_kv_attend_args* a, void* stream) {
     c.kv_lens = a->kv_lens, c.cu = a->cu_tokens, c.max_new = int(a->max_new), c.scale = float(a->scale);
     c.window = a->window > INT32_MAX / 2 ? 0 : int(a->window), c.out = a->out, c.lse = a->lse;
     const int sms = exl3::num_sms_cached();
-    const size_t partials = serve_partials(exl3::kv_attend_counters(sms)), need = partials + exl3::kv_attend_workspace(c, sms);
+    const size_t partials = serve_partials(sms), need = partials + exl3::kv_attend_workspace(c, sms);
     if (!a->workspace || a->workspace_bytes < 0 || size_t(a->workspace_bytes) < need)
         return fail(EXL3_ERR_WORKSPACE, "%s: workspace of %zu bytes required (got %lld)", who, need, (long long)a->workspace_bytes);
     if (!aligned(a->workspace, 256)) return fail(EXL3_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
@@ -719,7 +723,7 @@ size_t exl3_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top, 
     exl3::LogprobsCall c;
     c.rows = rows, c.vocab = int(vocab), c.top = top, c.x_dtype = x_dtype;
     const int sms = exl3::num_sms_cached();
-    return serve_partials(exl3::logprobs_counters(sms)) + (rows ? exl3::logprobs_workspace(c, sms) : 0);
+    return serve_partials(sms) + (rows ? exl3::logprobs_workspace(c, sms) : 0);
 }
 
 int exl3_token_logprobs(const exl3_token_logprobs_args* a, void* stream) {
@@ -742,7 +746,7 @@ int exl3_token_logprobs(const exl3_token_logprobs_args* a, void* stream) {
     c.tokens = a->tokens, c.ids_dtype = int(a->ids_dtype), c.top = int(a->top), c.logprob = a->logprob;
     c.entropy = a->entropy, c.rank = a->rank, c.top_logprobs = a->top_logprobs, c.top_ids = a->top_ids;
     const int sms = exl3::num_sms_cached();
-    const size_t partials = serve_partials(exl3::logprobs_counters(sms)), need = partials + exl3::logprobs_workspace(c, sms);
+    const size_t partials = serve_partials(sms), need = partials + exl3::logprobs_workspace(c, sms);
     if (!a->workspace || a->workspace_bytes < 0 || size_t(a->workspace_bytes) < need)
         return fail(EXL3_ERR_WORKSPACE, "%s: workspace of %zu bytes required (got %lld)", who, need, (long long)a->workspace_bytes);
     if (!aligned(a->workspace, 256)) return fail(EXL3_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
