@@ -60,8 +60,12 @@ struct AttShape {
 };
 
 // Requests of more query columns (rows x heads per kv head) than this go to
-// the prompt kernel when the call has such requests at all.
-constexpr int kAttFew = 32;
+// the prompt kernel when the call has such requests at all.  From 33 on the
+// kernel here reads the keys twice (the second time from L2), the prompt kernel
+// pads to 128 rows.  us here / there, int8, dim 128, 64 heads over 8:
+//   8 requests of 32K keys: 24 columns 111 / 186, 32 142 / 237, 40 159 / 213, 48 189 / 222, 64 225 / 225, 96 271 / 223
+//   64 requests of 1K keys: 24 88 / 112, 32 104 / 111, 40 111 / 96, 64 159 / 98
+constexpr int kAttFew = 48;
 
 // what a request asks for
 struct AttReq {
