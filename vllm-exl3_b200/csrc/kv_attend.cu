@@ -28,6 +28,16 @@
 // byte permute.  Like the prompt kernel, a column's reference follows its
 // maximum only when that has grown by more than 2^8, so that the usual tile
 // needs no exchange between lanes and no rescaling.
+//
+// Measured: 64 single tokens over up to 8192 keys (32 heads over 4, dim 128,
+// e4m3, 343 MB) 72 us, 4.8 TB/s, 73 % of the measured copy rate; 4 requests of
+// 3 tokens over up to 128K keys (64 heads over 8, int8, 24 columns) 218 us, 57 %
+// (the int8 conversions and three column tiles leave two warps per scheduler
+// at their issue latency); one token over 1021 keys 10.4 us, a chain of
+// dependent steps.  A piece of an item costs about 13K cycles beside its tiles
+// (queries in, warps joined, partials out), a third of a CTA's time at the 64.
+// Not kept, us at the 64 and the 128K: joining at a CTA's end 77 / 250, joining
+// the warps as a tree 76 / 233, separate loops for tiles with and without masks 74 / 217.
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>

@@ -18,6 +18,14 @@
 // maximum and the coding: runs of up to 8 iterations of one warp are a warp's
 // alone (no barrier), longer ones the CTA's.  Bound: HBM, 2 bytes read and 1
 // written per value.
+//
+// Measured (launches in a graph): the plan of 64 requests, a token each, 3.7 us,
+// of 512 with 23318 tokens 5.5 us: one launch and its chain of reads (lengths,
+// scan, bisection, table), the bytes are nothing.  64 tokens of 4 heads, dim
+// 128, into pages of 16: 5.4 us, the same kind of chain (slot, run, rows and
+// page, scale, codes).  8190 tokens of 8 heads, pages of 64: 13.6 us with rows
+// in L2 (3.7 TB/s), 18.5 from HBM as a lone call; a CTA's loads, reduction and
+// stores follow one another, and two or three CTAs per SM hide that in part.
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>

@@ -10,10 +10,11 @@
 // Bound: every logit is read once: HBM (bf16: about 12 logits per clock and SM
 // at the measured copy rate, near the 16 per clock of the exponential unit).
 // A CTA streams a slice of one row, each thread 4 16-byte vectors at a time
-// with the next 4 on their way (cp.async: 64 KB per SM without a register).  A thread's reference m follows its maximum
-// only when that has grown by more than 16: sums of exp(d <= 16) are as exact,
-// and the loop has no dependent rescaling.  Few rows: a row is split over CTAs
-// and joined by the one that ends last, always in the same order.
+// with the next 4 on their way (cp.async: 64 KB per SM without a register).  A
+// thread's reference m follows its maximum only when that has grown by more
+// than 16: sums of exp(d <= 16) are as exact, and the loop has no dependent
+// rescaling.  Few rows: a row is split over CTAs and joined by the one that
+// ends last, always in the same order.
 //
 // Alternatives: entries are ordered by a 64-bit key (value, then lowest index
 // first).  The `top`-th largest of 32 thread groups' maxima bounds the answer
@@ -21,6 +22,11 @@
 // all warps then read those threads' entries again (from L2) and collect what
 // passes, some `top` entries.  The buffer holds whatever one such round can
 // yield; before it could overflow (many ties) it is reduced, which raises the bound.
+//
+// Measured: 2048 rows of 131072 bf16 100 us in a graph, 117 as a lone call from
+// HBM (4.6 TB/s, 70 % of the measured copy rate; exponential unit and ALU are
+// at 66 and 57 % of their rates); 64 rows with 5 alternatives 14 us, one row
+// of 100277 f32 with 20 alternatives 12 us (pass, join, selection one after another).
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
