@@ -23,15 +23,17 @@
 // products behind the other's weights; tcgen05 runs one thread's products in order.
 //
 // Work: an item is (request, 256 rows, kv head), its steps are the 128-key
-// blocks that its rows see; all items' steps form one line that the CTAs, one
-// per SM, split evenly, whatever the lengths and the causal mask.  An item cut
+// blocks that its rows see; all items' steps, and a few for each item's start
+// and end, form one line that the CTAs, one per SM, split evenly, whatever the
+// lengths and the causal mask.  (Steps alone give a prompt's first rows, whose
+// items have one or two, to too few CTAs.)  An item cut
 // by a CTA boundary is joined from fp32 partials by the CTA that finishes it
 // last, in key order.  (A least number of steps per CTA does not pay: a prompt
 // of 256 rows of 8 heads took 49 us with four, 30 with two, 27 with one.)
 //
 // Measured: a prompt's last 4096 tokens of 16384 (32 heads over 4, dim 128, e4m3)
 // 0.98 ms, 978 TFLOP/s (59 % of the measured bf16 rate); five prompts of up to
-// 1777 tokens, window 1000 (24 heads over 8, dim 64, int8) 146 us, where half
+// 1777 tokens, window 1000 (24 heads over 8, dim 64, int8) 144 us, where half
 // of the steps have masks.  No single unit bounds it: without its exponentials
 // the first takes 1036 of then 1064 us, with an eighth of the products 1003,
 // without loads 1077.  It is the chain of a tile's scores, weights, product
@@ -59,6 +61,11 @@ constexpr int kPrRows = 256;        // query rows per CTA
 constexpr int kPrSlots = 8;         // steps whose pages and scales are kept
 constexpr float kPrSlack = 8.f;     // log2: growth of the maximum that is let pass
 constexpr uint32_t kPrTmem = 512;
+// Steps that an item's queries and results are worth on the line.  us with 0 / 3 / 6 / 10:
+//   whole prompts of 2043 to 4086 tokens (16 heads over 4, dim 128, int8) 478 / 280 / 286 / 300, one of 4086 228 / 117 / 122 / 129
+//   six of 1337 to 2673 tokens (24 heads over 8, e4m3), dim 128 603 / 382 / 398 / 418, dim 64 421 / 311 / 326 / 338
+//   up to 2000 tokens behind a prefix, 8000 in all 297 / 280 / 276 / 284
+constexpr int kPrItemCost = 3;
 
 // pages and scales of a step
 struct PrStep {
@@ -84,8 +91,10 @@ struct PrSmem {
     uint32_t tmem;
     int abort_flag, last[2];
     int64_t scan[kPrThreads / 32];
-    int found_b, found_tile;
-    int64_t found_base;
+    int found_b, found_tile, tile_index;  // of the CTA's first step: request, its tile, the tile's place among all
+    int64_t found_base;                   // that tile's first step
+    int64_t steps_from, steps_upto;       // the CTA's steps
+    int64_t line;                         // length of the line
     PrStep step[kPrSlots];
     PrItem item[kPrItems];
 };
@@ -146,7 +155,7 @@ __device__ __forceinline__ PrTile pr_tile(const KvAttendArgs& a, int b, int tile
     const int first = t.len - t.fresh + int(t.col0 / a.group), last = t.len - t.fresh + int((t.col0 + t.rows - 1) / a.group);
     t.hi = max(min(last + 1, t.len), 0);
     t.lo = min(a.window > 0 ? max(first + 1 - a.window, 0) : 0, t.hi);
-    t.k_begin = t.lo & ~(kPrKeys - 1);
+    t.k_begin = t.lo & ~15;  // pages and scales are looked up by 16 keys
     t.steps = max((t.hi - t.k_begin + kPrKeys - 1) / kPrKeys, 1);  // rows that see nothing take one step too
     return t;
 }
@@ -154,16 +163,17 @@ __device__ __forceinline__ PrTile pr_tile(const KvAttendArgs& a, int b, int tile
 // A place on the line of steps, ordered by request, tile, kv head, keys
 struct PrWalk {
     int64_t base;  // of the tile's first step
-    int b, tile, tiles;
+    int b, tile, tiles, index;
     PrTile t;
     __device__ __forceinline__ void start(const KvAttendArgs& a, const PrSmem& sm) {
-        base = sm.found_base, b = sm.found_b, tile = sm.found_tile;
+        base = sm.found_base, b = sm.found_b, tile = sm.found_tile, index = sm.tile_index;
         tiles = pr_tiles(a, b);
         t = pr_tile(a, b, tile);
     }
     __device__ __forceinline__ void seek(const KvAttendArgs& a, int64_t u) {  // forwards, to a step below the total
         while (u >= base + int64_t(a.kv_heads) * t.steps) {
             base += int64_t(a.kv_heads) * t.steps;
+            ++index;
             if (++tile >= tiles) {
                 do tiles = pr_tiles(a, ++b);
                 while (tiles == 0);
@@ -308,6 +318,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
         return v;
     };
     int32_t* sums = reinterpret_cast<int32_t*>(smem);  // [requests + 1] tiles of the requests before; the operands come later
+    int ctas;
     {
         const int per = (a.requests + kPrThreads - 1) / kPrThreads;
         int64_t mine = 0, n_tiles, total;
@@ -338,22 +349,35 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
             mine += int64_t(Hk) * pr_tile(a, b, int(t - sums[b])).steps;
         }
         const int64_t end = scan(mine, total);
-        const int ctas = int(min(int64_t(gridDim.x), total));
+        // Step s of item i (all counted from 0) is at s + (i + 1) kPrItemCost of the line
+        const int64_t line = total + int64_t(kPrItemCost) * Hk * n_tiles;
+        ctas = int(min(int64_t(gridDim.x), total));
         if (int(blockIdx.x) >= ctas) return;
-        const int64_t u0 = total * blockIdx.x / ctas;
-        if (u0 >= end - mine && u0 < end) {
-            int64_t base = end - mine, t = t0;
-            for (;; ++t) {
+        if (tid == 0) sm.line = line, sm.steps_upto = total;
+        __syncthreads();
+        const int64_t u0 = line * blockIdx.x / ctas, u1 = line * (blockIdx.x + 1) / ctas;
+        auto at_line = [&](int64_t step, int64_t t) { return step + int64_t(kPrItemCost) * Hk * t; };
+        const int64_t from = at_line(end - mine, min(t0, n_tiles)), upto = at_line(end, max(t1, t0));
+        const bool has0 = t0 < t1 && u0 >= from && u0 < upto, has1 = t0 < t1 && u1 >= from && u1 < upto;
+        if (has0 || has1) {
+            int64_t base = end - mine;
+            for (int64_t t = t0; t < t1; ++t) {
                 const int b = request(t);
-                const int64_t n = int64_t(Hk) * pr_tile(a, b, int(t - sums[b])).steps;
-                if (u0 < base + n) {
-                    sm.found_b = b, sm.found_tile = int(t - sums[b]), sm.found_base = base;
-                    break;
+                const int64_t tile_steps = pr_tile(a, b, int(t - sums[b])).steps;
+                // steps before place u of the line
+                auto steps_before = [&](int64_t u) {
+                    const int64_t o = u - at_line(base, t), item = tile_steps + kPrItemCost, head = o / item;
+                    return base + head * tile_steps + max(o - head * item - kPrItemCost, int64_t(0));
+                };
+                auto inside = [&](int64_t u) { return u >= at_line(base, t) && u < at_line(base + Hk * tile_steps, t + 1); };
+                if (has0 && inside(u0)) {
+                    sm.found_b = b, sm.found_tile = int(t - sums[b]), sm.found_base = base, sm.tile_index = int(t);
+                    sm.steps_from = steps_before(u0);
                 }
-                base += n;
+                if (has1 && inside(u1)) sm.steps_upto = steps_before(u1);
+                base += Hk * tile_steps;
             }
         }
-        if (tid == 0) sm.scan[0] = total;
     }
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -379,14 +403,15 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
         sm.abort_flag = 0;
         mbar_fence_init();
     }
+    __syncthreads();
+    const int64_t u0 = sm.steps_from, u1 = sm.steps_upto, line = sm.line;  // this CTA's steps
+    if (u0 >= u1) return;  // its part of the line has none
     if (warp == 12) tmem_alloc(&sm.tmem, kPrTmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tm = __shfl_sync(0xffffffffu, sm.tmem, 0);
-    const int64_t total = sm.scan[0];
-    const int ctas = int(min(int64_t(gridDim.x), total)), cta = blockIdx.x;
-    const int64_t u0 = total * cta / ctas, u1 = total * (cta + 1) / ctas;
+    const int cta = blockIdx.x;
     // TMEM columns: S0 0, S1 128, O0 256, O1 384
     if (warp < 8) {
         set_registers<true, kRowRegs>();
@@ -783,8 +808,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                     im.all = w.t.steps, im.steps = int(min(int64_t(w.t.steps - im.off), u1 - u));
                     im.row0 = w.t.row0, im.col0 = w.t.col0, im.rows = w.t.rows, im.fresh = w.t.fresh, im.len = w.t.len;
                     im.k_begin = w.t.k_begin;
-                    const int64_t first = u - im.off;
-                    im.c0 = int(((first + 1) * ctas - 1) / total), im.c1 = int(((first + im.all) * ctas - 1) / total);
+                    // its first step's place on the line
+                    const int64_t first = u - im.off + int64_t(kPrItemCost) * (int64_t(w.index) * Hk + im.hk + 1);
+                    im.c0 = int(((first + 1) * ctas - 1) / line), im.c1 = int(((first + im.all) * ctas - 1) / line);
                     u += im.steps;
                 }
                 if (lane == 0) {
