@@ -260,6 +260,18 @@ def test_attend_long(native, cuda, dim, x, code):
         _check_attend(cuda, p, x, window=window)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 1, 128), (12, 4, 64)])
+def test_attend_shares(native, cuda, heads, kv_heads, dim):
+    """Items of one and of many steps: the card's shares begin and end at an item's edge, inside it, or have no step at all."""
+    lens = [700, 333, 64, 450]
+    p = _problem(cuda, lens, lens, heads=heads, kv_heads=kv_heads, dim=dim, page=16, x="f16", code="e4m3")
+    for window in (0, 75):
+        _check_attend(cuda, p, "f16", window=window)
+    lens = [1 + (37 * i * i) % 600 for i in range(150)]
+    p = _problem(cuda, lens, [1] * len(lens), heads=heads, kv_heads=kv_heads, dim=dim, page=32, x="bf16", code="int8")
+    _check_attend(cuda, p, "bf16")
+
+
 def test_attend_repeats_streams_graph(native, cuda):
     """Bit-equal repeats, on other streams and from a CUDA graph."""
     import torch

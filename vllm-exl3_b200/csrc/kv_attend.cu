@@ -11,9 +11,9 @@
 //
 // Work: an item is (request, kv head, group of NC = 8 NT query columns), a
 // column being one (token, query head) that reads this kv head.  Its keys are
-// cut into units of 128 (8 warps x 16 keys); all items' units form one line
-// that the CTAs split evenly, so lengths need no balancing and the host needs
-// none of them.  An item cut by a CTA boundary is joined from fp32 partials by
+// cut into units of 128 (8 warps x 16 keys); all items' units, and a few for
+// each item's start and end, form one line that the CTAs split evenly, so
+// lengths need no balancing and the host needs none of them.  An item cut by a CTA boundary is joined from fp32 partials by
 // the CTA that finishes it last, in key order (results do not depend on timing).
 //
 // Bound: every code is read once, 2 D bytes per (key, kv head): HBM.  Each
@@ -30,14 +30,15 @@
 // needs no exchange between lanes and no rescaling.
 //
 // Measured: 64 single tokens over up to 8192 keys (32 heads over 4, dim 128,
-// e4m3, 343 MB) 72 us, 4.8 TB/s, 73 % of the measured copy rate; 4 requests of
+// e4m3, 343 MB) 70 us, 4.9 TB/s, 75 % of the measured copy rate; 4 requests of
 // 3 tokens over up to 128K keys (64 heads over 8, int8, 24 columns) 218 us, 57 %
 // (the int8 conversions and three column tiles leave two warps per scheduler
 // at their issue latency); one token over 1021 keys 10.4 us, a chain of
 // dependent steps.  A piece of an item costs about 13K cycles beside its tiles
 // (queries in, warps joined, partials out), a third of a CTA's time at the 64.
 // Not kept, us at the 64 and the 128K: joining at a CTA's end 77 / 250, joining
-// the warps as a tree 76 / 233, separate loops for tiles with and without masks 74 / 217.
+// the warps as a tree 76 / 233, separate loops for tiles with and without masks 74 / 217
+// (each against 71 / 218 then).
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -52,6 +53,12 @@ constexpr int kAttWarps = 8, kAttThreads = kAttWarps * 32, kAttUnit = 16 * kAttW
 constexpr float kAttSlack = 8.f;  // log2: growth of the maximum that is let pass
 
 constexpr int kAttMaxSms = 160;     // SMs that are used at most
+// Units that an item's start and end are worth on the line, where the CTAs have more than a unit each.  us with 0 / 3 / 5 / 10:
+//   64 single tokens over up to 8192 keys (32 heads over 4, e4m3) 71.4 / 69.5 / 70.0 / 71.6
+//   25 x 4 tokens, 20918 keys (12 heads over 4, int8) 102.6 / 99.7 / 95.9 / 98.3
+//   dim 64, int8: 126 single tokens, 2309 keys (12 heads over 1) 24.7 / 22.7 / 21.5 / 22.7, 127, 697 keys (8 over 2) 20.6 / 16.6 / 17.4 / 16.5
+//   4 x 3 tokens over 128K keys (24 columns) 216.6 / 221.5 / 218.0 / 220.0
+constexpr int kAttItemCost = 5;
 
 // Tiles of 8 query columns an item has at most: up to two with two CTAs per
 // SM; three or four need the registers of one.
@@ -125,7 +132,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
     float* fin = wl + kAttWarps * NC;                 // [2][NC] joined maximum, sum
     float* qfac = fin + 2 * NC;                       // [NC] factor of a column's scores
     float2* tile_sc = reinterpret_cast<float2*>(qfac + NC);  // [warps][S] a tile's K and V scale
-    __shared__ int64_t scan[kAttWarps];
+    __shared__ int64_t scan[2][kAttWarps];
     __shared__ int64_t found_base;
     __shared__ AttReq found;
     __shared__ int found_b, last_flag;
@@ -135,29 +142,33 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
 
     // --- this CTA's share of the line of units ---
     const int per = (a.requests + kAttThreads - 1) / kAttThreads;
-    int64_t mine = 0;
+    int64_t mine = 0, items = 0;
     AttReq own = {};
     for (int i = 0; i < per; ++i) {
         const int b = tid * per + i;
         if (b < a.requests) {
             own = att_request<NC>(a, b);
             mine += int64_t(own.groups) * Hk * own.units;
+            items += int64_t(own.groups) * Hk;
         }
     }
-    int64_t incl = mine;
+    int64_t incl = mine, items_incl = items;
     #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int64_t o = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += o;
+        const int64_t o = __shfl_up_sync(0xffffffffu, incl, d), oi = __shfl_up_sync(0xffffffffu, items_incl, d);
+        if (lane >= d) incl += o, items_incl += oi;
     }
-    if (lane == 31) scan[warp] = incl;
+    if (lane == 31) scan[0][warp] = incl, scan[1][warp] = items_incl;
     __syncthreads();
-    int64_t total = 0;
+    int64_t total = 0, n_items = 0;
     #pragma unroll
     for (int w = 0; w < kAttWarps; ++w) {
-        if (w == warp) incl += total;
-        total += scan[w];
+        if (w == warp) incl += total, items_incl += n_items;
+        total += scan[0][w], n_items += scan[1][w];
     }
+    // an item's line: `cost` places, then its units
+    const int cost = total > gridDim.x ? kAttItemCost : 0;
+    total += cost * n_items, incl += cost * items_incl, mine += cost * items;
     // rows no request owns are zeros
     if (a.cu) {
         const int64_t live = a.cu[a.requests], n = (a.q_rows - live) * a.heads;
@@ -177,7 +188,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
         int b = tid * per;
         for (;;) {
             const AttReq r = per == 1 ? own : att_request<NC>(a, b);
-            const int64_t n = int64_t(r.groups) * Hk * r.units;
+            const int64_t n = int64_t(r.groups) * Hk * (r.units + cost);
             if (u < base + n) {
                 found = r;
                 break;
@@ -192,17 +203,17 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
     AttReq rq = found;
 
     while (u < u_end) {
-        while (u >= base + int64_t(rq.groups) * Hk * rq.units) {  // next request with work
-            base += int64_t(rq.groups) * Hk * rq.units;
+        while (u >= base + int64_t(rq.groups) * Hk * (rq.units + cost)) {  // next request with work
+            base += int64_t(rq.groups) * Hk * (rq.units + cost);
             rq = att_request<NC>(a, ++b);
         }
-        const int64_t item = (u - base) / rq.units;
-        const int off = int((u - base) - item * rq.units);
-        const int n_units = int(min(int64_t(rq.units - off), u_end - u));
+        const int64_t item = (u - base) / (rq.units + cost), u_item = base + item * (rq.units + cost) + cost;  // its first unit
+        const int off = int(max(u - u_item, int64_t(0)));
+        u = min(u_item + rq.units, u_end);
+        const int n_units = int(u - u_item) - off;
+        if (n_units <= 0) break;  // the CTA's part of the line ends before the item's first unit
         const int hk = int(item / rq.groups), cg = int(item % rq.groups);
         const int ncols = min(rq.fresh * G - cg * NC, NC);
-        const int64_t u_item = u - off;
-        u += n_units;
 
         // --- the query columns: B fragments of Q^T (a warp to each 8), and each column's key range ---
         for (int t = warp; t < NT; t += kAttWarps) {

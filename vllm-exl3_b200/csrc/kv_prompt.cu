@@ -32,8 +32,8 @@
 // of 256 rows of 8 heads took 49 us with four, 30 with two, 27 with one.)
 //
 // Measured: a prompt's last 4096 tokens of 16384 (32 heads over 4, dim 128, e4m3)
-// 0.98 ms, 978 TFLOP/s (59 % of the measured bf16 rate); five prompts of up to
-// 1777 tokens, window 1000 (24 heads over 8, dim 64, int8) 144 us, where half
+// 0.964 ms, 998 TFLOP/s (60 % of the measured bf16 rate); five prompts of up to
+// 1777 tokens, window 1000 (24 heads over 8, dim 64, int8) 137 us, where half
 // of the steps have masks.  No single unit bounds it: without its exponentials
 // the first takes 1036 of then 1064 us, with an eighth of the products 1003,
 // without loads 1077.  It is the chain of a tile's scores, weights, product
