@@ -344,8 +344,9 @@ int exl3_kv_append(const exl3_kv_append_args* args, void* stream);
  * page is not in the cache are not seen, with status 7.  Results do not
  * depend on timing: repeats are equal bit for bit. */
 /* Workspace of this entry and of exl3_token_logprobs: 256-byte aligned, all
- * zero before its first use; it starts with the status word, and may serve
- * both, for calls that follow one another on a stream. */
+ * zero before its first use (zeroed on the device, not by a fill that a
+ * capture records); it starts with the status word, and may serve both, for
+ * calls that follow one another on a stream, or in one graph. */
 size_t exl3_kv_attend_workspace_size(int heads, int kv_heads, int dim, int max_new, int requests, int64_t q_rows);
 typedef struct exl3_kv_attend_args {
     const void* q;
@@ -392,6 +393,23 @@ typedef struct exl3_token_logprobs_args {
     int64_t workspace_bytes;
 } exl3_token_logprobs_args;
 int exl3_token_logprobs(const exl3_token_logprobs_args* args, void* stream);
+
+/* For hosts that hand out workspaces to calls under stream capture.  Work
+ * recorded in a graph runs later, maybe beside other work of the stream it was
+ * captured on, so a captured call wants a workspace that its graph alone uses
+ * and that was zeroed outside the capture.
+ * exl3_capture_id: 0 where `stream` is not capturing, else a number that the
+ * capture shares with no other of the process.
+ * exl3_capture_hold: `token` learns when the graph being captured on `stream`,
+ * and every executable made of it, is destroyed and has run to its end.
+ * exl3_capture_gone: 1 from then on (which frees the token), 0 before.
+ * exl3_capture_mode: sets the calling thread's capture interaction mode (0
+ * global, 1 thread-local, 2 relaxed: an allocation beside a capture needs it)
+ * and returns the previous one, -1 on error. */
+uint64_t exl3_capture_id(void* stream);
+int exl3_capture_hold(void* stream, void** token);
+int exl3_capture_gone(void* token);
+int exl3_capture_mode(int mode);
 
 /* Phase timing for benchmarks (no reference counterpart; the reference times
  * its kernels with CUDA events in tools/bench_moe_decode.py:24-55).  While

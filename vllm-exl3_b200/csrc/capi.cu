@@ -2,10 +2,12 @@
 // validation mirrors the reference's TORCH_CHECKs (csrc/bindings.cpp:117-147,
 // csrc/p2b_moe.cu:2437-2466, 2346-2428): everything is rejected before launch
 // with a message; nothing here reads device memory except exl3_device_status.
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <new>
 #include <string>
 
 #include "../../include/exl3_b200.h"
@@ -754,6 +756,66 @@ int exl3_token_logprobs(const exl3_token_logprobs_args* a, void* stream) {
     c.counters = reinterpret_cast<int32_t*>(ws + kServeCounters), c.ws = ws + partials;
     const cudaError_t e = exl3::run_logprobs(c, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? EXL3_OK : cuda_fail(e, who);
+}
+
+// --- stream capture ---
+
+uint64_t exl3_capture_id(void* stream) {
+    cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &state, &id) != cudaSuccess) {
+        cudaGetLastError();  // the legacy stream beside a capture, no device: nothing is captured here
+        return 0;
+    }
+    return state == cudaStreamCaptureStatusNone ? 0 : uint64_t(id) + 1;
+}
+
+// Runs on a thread of the driver's, which may make no CUDA call
+static void CUDART_CB mark_gone(void* token) { static_cast<std::atomic<int>*>(token)->store(1, std::memory_order_release); }
+
+int exl3_capture_hold(void* stream, void** token) {
+    const char* who = "exl3_capture_hold";
+    if (!token) return fail(EXL3_ERR_ARG, "%s: null token", who);
+    cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    cudaGraph_t graph = nullptr;
+    cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &state, &id, &graph);
+    if (e != cudaSuccess) return cuda_fail(e, who);
+    if (state != cudaStreamCaptureStatusActive) return fail(EXL3_ERR_ARG, "%s: the stream is not capturing", who);
+    auto* flag = new (std::nothrow) std::atomic<int>(0);
+    if (!flag) return fail(EXL3_ERR_ARG, "%s: out of host memory", who);
+    cudaUserObject_t object = nullptr;
+    e = cudaUserObjectCreate(&object, flag, mark_gone, 1, cudaUserObjectNoDestructorSync);
+    if (e != cudaSuccess) {
+        delete flag;
+        return cuda_fail(e, who);
+    }
+    e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) {
+        cudaUserObjectRelease(object, 1);  // the flag is left to mark_gone, which may run later
+        return cuda_fail(e, who);
+    }
+    *token = flag;
+    return EXL3_OK;
+}
+
+int exl3_capture_gone(void* token) {
+    auto* flag = static_cast<std::atomic<int>*>(token);
+    if (!flag || !flag->load(std::memory_order_acquire)) return 0;
+    delete flag;
+    return 1;
+}
+
+int exl3_capture_mode(int mode) {
+    if (mode < 0 || mode > 2) return -1;
+    cudaStreamCaptureMode m = mode == 0   ? cudaStreamCaptureModeGlobal
+                              : mode == 1 ? cudaStreamCaptureModeThreadLocal
+                                          : cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&m) != cudaSuccess) {
+        cudaGetLastError();
+        return -1;
+    }
+    return m == cudaStreamCaptureModeGlobal ? 0 : m == cudaStreamCaptureModeThreadLocal ? 1 : 2;
 }
 
 }  // extern "C"

@@ -31,8 +31,9 @@ struct Entries {
     size_t (*attend_bytes)(int, int, int, int, int, int64_t) = nullptr;
     int (*logprobs)(const exl3_token_logprobs_args*, void*) = nullptr;
     size_t (*logprobs_bytes)(int64_t, int64_t, int, int) = nullptr;
+    uint64_t (*capture_id)(void*) = nullptr;
 } entry;
-PyObject* workspace_of = nullptr;  // (device index, stream, bytes) -> (address, bytes)
+PyObject* workspace_of = nullptr;  // (device index, stream, bytes, capture) -> (address, bytes)
 PyObject* check = nullptr;         // (status, operator's name): raises
 
 // Raised by the helpers below when the short way is not open.
@@ -74,7 +75,8 @@ struct Space {
 struct PyFailed {};
 
 Space workspace(const c10::Device& dev, cudaStream_t stream, size_t need) {
-    PyObject* r = PyObject_CallFunction(workspace_of, "iLn", int(dev.index()), (long long)(intptr_t)stream, Py_ssize_t(need));
+    PyObject* r = PyObject_CallFunction(workspace_of, "iLnK", int(dev.index()), (long long)(intptr_t)stream, Py_ssize_t(need),
+                                        (unsigned long long)entry.capture_id(stream));
     if (!r) throw PyFailed();
     Space s{PyLong_AsVoidPtr(PyTuple_GET_ITEM(r, 0)), PyLong_AsLongLong(PyTuple_GET_ITEM(r, 1))};
     Py_DECREF(r);
@@ -277,18 +279,19 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
 }
 
-// setup(plan, append, attend, attend_bytes, logprobs, logprobs_bytes, workspace_of, check): addresses of the C entries
+// setup(plan, append, attend, attend_bytes, logprobs, logprobs_bytes, capture_id, workspace_of, check): addresses of the C entries
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    if (n != 8) {
-        PyErr_SetString(PyExc_TypeError, "8 arguments expected");
+    if (n != 9) {
+        PyErr_SetString(PyExc_TypeError, "9 arguments expected");
         return nullptr;
     }
-    void* p[6];
-    for (int i = 0; i < 6; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
+    void* p[7];
+    for (int i = 0; i < 7; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
     if (PyErr_Occurred()) return nullptr;
-    Py_INCREF(a[6]);
     Py_INCREF(a[7]);
-    workspace_of = a[6], check = a[7];
+    Py_INCREF(a[8]);
+    workspace_of = a[7], check = a[8];
+    entry.capture_id = reinterpret_cast<decltype(entry.capture_id)>(p[6]);
     entry.append = reinterpret_cast<decltype(entry.append)>(p[1]);
     entry.attend = reinterpret_cast<decltype(entry.attend)>(p[2]);
     entry.attend_bytes = reinterpret_cast<decltype(entry.attend_bytes)>(p[3]);

@@ -83,6 +83,10 @@ SIGNATURES = {
     "exl3_kv_attend": (I32, [P, P]),
     "exl3_token_logprobs_workspace_size": (SZ, [I64, I64, I32, I32]),
     "exl3_token_logprobs": (I32, [P, P]),
+    "exl3_capture_id": (ctypes.c_uint64, [P]),
+    "exl3_capture_hold": (I32, [P, ctypes.POINTER(P)]),
+    "exl3_capture_gone": (I32, [P]),
+    "exl3_capture_mode": (I32, [I32]),
     "exl3_profile_enable": (I32, [I32, ctypes.c_longlong]),
     "exl3_profile_read": (I32, [ctypes.POINTER(F32), I32, ctypes.POINTER(I32)]),
 }
@@ -150,7 +154,7 @@ def binding():
             mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_serving_py", loader))
             loader.exec_module(mod)
             names = ("kv_plan", "kv_append", "kv_attend", "kv_attend_workspace_size", "token_logprobs",
-                     "token_logprobs_workspace_size")
+                     "token_logprobs_workspace_size", "capture_id")
             mod.setup(*(ctypes.cast(getattr(lib, "exl3_" + n), P).value for n in names), serve_workspace, check)
             _binding = mod
         except (OSError, RuntimeError, ImportError):
@@ -246,11 +250,17 @@ def workspace(device: torch.device, nbytes: int, stream: torch.cuda.Stream | Non
 _serve_ws: dict[tuple[int, int], tuple[int, int]] = {}
 
 
-def serve_workspace(index: int, stream: int, nbytes: int = 0) -> tuple[int, int]:
+def serve_workspace(index: int, stream: int, nbytes: int = 0, capture: int | None = None) -> tuple[int, int]:
     """(address, bytes) of the workspace of the cache and log-probability
     entries for the raw ``stream`` of device ``index``.  It is kept apart from
     :func:`workspace` because those entries need its counters zero and leave
-    them zero.  Grows and is retained in the same way."""
+    them zero.  Grows and is retained in the same way.  ``capture`` is
+    ``exl3_capture_id(stream)``, asked here when not given: a call under
+    capture gets a workspace of its graph's own."""
+    if capture is None:
+        capture = load().exl3_capture_id(stream)
+    if capture:
+        return _captured_workspace(index, stream, capture, nbytes)
     have = _serve_ws.get((index, stream))
     if have is None or have[1] < nbytes:
         key = ("cuda", index, stream, "serve")
@@ -265,7 +275,63 @@ def serve_workspace(index: int, stream: int, nbytes: int = 0) -> tuple[int, int]
     return have
 
 
+# A graph's launches run on any stream, beside eager calls and other graphs, so
+# what a capture records must not share counters with them: every (capture,
+# stream) gets a workspace that belongs to its graph until the graph is gone,
+# and then to a later capture.  It is allocated outside the graph's memory and
+# zeroed on the device before the capture goes on: a fill recorded in the graph
+# would run at each replay, and not before the first.
+_captured: dict[tuple[int, int, int], tuple[int, int]] = {}     # (device, stream, capture) -> (address, bytes)
+_captured_held: list[tuple[int, tuple[int, int, int], torch.Tensor]] = []  # (token of the graph, key, buffer)
+_captured_spare: list[torch.Tensor] = []                        # of graphs that are gone
+_captured_lock = threading.Lock()
+
+
+def _captured_workspace(index: int, stream: int, capture: int, nbytes: int) -> tuple[int, int]:
+    key = (index, stream, capture)
+    have = _captured.get(key)
+    if have is not None and have[1] >= nbytes:
+        return have
+    lib = load()
+    with _captured_lock:
+        for held in list(_captured_held):
+            if lib.exl3_capture_gone(held[0]):
+                _captured_held.remove(held)
+                _captured.pop(held[1], None)
+                _captured_spare.append(held[2])
+        fits = [b for b in _captured_spare if b.device.index == index and b.numel() >= nbytes]
+        buf = min(fits, key=torch.Tensor.numel, default=None)
+        if buf is not None:
+            _captured_spare[:] = [b for b in _captured_spare if b is not buf]
+        # The work below is not the graph's: it runs, now, on a stream that is not captured
+        before = lib.exl3_capture_mode(2)
+        try:
+            with torch.cuda.device(index):
+                side = next((s for s in (torch.cuda.Stream() for _ in range(64))
+                             if s.cuda_stream != stream and not lib.exl3_capture_id(s.cuda_stream)), None)
+                if side is None:
+                    raise RuntimeError("no stream outside the capture to set up a workspace on")
+                with torch.cuda.stream(side):
+                    if buf is None:
+                        buf = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=torch.device("cuda", index))
+                    else:
+                        buf[256:].zero_()  # a status that was recorded in it stays
+                side.synchronize()
+        finally:
+            if before >= 0:
+                lib.exl3_capture_mode(before)
+        token = P()
+        rc = lib.exl3_capture_hold(stream, ctypes.byref(token))
+        if rc:
+            _captured_spare.append(buf)
+            check(rc, "serve_workspace")
+        _captured_held.append((token.value, key, buf))
+        have = _captured[key] = (buf.data_ptr(), buf.numel())
+    return have
+
+
 def device_workspaces(device: torch.device) -> list[torch.Tensor]:
     """Every workspace handed out on ``device`` (current and retained)."""
     out = [b for k, b in _ws_cache.items() if k[0] == device.type and k[1] == device.index]
-    return out + [b for b in _ws_retired if b.device == device]
+    kept = _ws_retired + [held[2] for held in _captured_held] + _captured_spare
+    return out + [b for b in kept if b.device == device]

@@ -5,8 +5,9 @@ layer ``kv_append`` (the step's keys and values into the cache) and
 ``kv_attend`` (attention over it).  The caches are codes ``[pages, kv_heads,
 page, dim]`` (``torch.float8_e4m3fn`` or ``torch.int8``; page 16, 32, 64 or
 128; dim 64 or 128) with one power-of-two scale per (page, kv head) in fp32
-``[pages, kv_heads]``: value = code * scale.  Nothing here synchronises; all
-three can be captured in a CUDA graph once each shape has run before.
+``[pages, kv_heads]``: value = code * scale.  Nothing here synchronises, and all
+three can be captured in CUDA graphs, each with a workspace of its own (the
+first captured call of a graph sets it up on the host).
 
 :class:`Exl3KvCache` keeps the tensors of one model's layers together.
 """
