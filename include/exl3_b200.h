@@ -307,8 +307,11 @@ int exl3_kv_plan(const exl3_kv_plan_args* args, void* stream);
 
 /* Writes new rows of K and V (fp16 or bf16 [tokens][kv_heads][dim], strides in
  * elements, rows at multiples of 16 bytes) to their slots as codes.  A page's
- * tokens of one call follow one another in ascending order, as exl3_kv_plan
- * gives them.  A call that writes a page's first token sets its scale from
+ * tokens of one call are one stretch of rows at consecutive slots, as
+ * exl3_kv_plan gives them.  Rows that come back to the page of the row before
+ * them (not counting skipped rows, up to a page's length of them) at another
+ * than the next slot are skipped with status 7; a page that returns behind
+ * rows of other pages has no defined content.  A call that writes a page's first token sets its scale from
  * the new tokens alone; one that joins a part-filled page keeps the larger of
  * its scale and the new tokens', rounding the older codes again when it
  * grows.  Infinities become the largest code.  int8 has no NaN: they become 0.

@@ -1,0 +1,93 @@
+"""GPU: the serving operators on device values that a plan does not give (slots
+out of order, lengths beyond the table, offsets outside the rows), and at sizes
+where a launch changes.  What is wrong is skipped with status 7; what is right
+beside it stands, and nothing is written elsewhere."""
+
+import numpy as np
+import pytest
+import serving_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _kv():
+    from exl3_b200 import kv_cache
+    return kv_cache
+
+
+def _kept(slots, page, pages):
+    """The slots that are written, -1 for the others, and whether any was refused: rows must continue the row
+    before them, or come from another page than the last kept row (up to a page's length back)."""
+    slots = [int(s) if 0 <= s < pages * page else -1 for s in slots]
+    out, refused, good = [], False, False
+    for t, s in enumerate(slots):
+        if s >= 0 and not (t and slots[t - 1] >= 0 and s == slots[t - 1] + 1 and s % page):
+            before = next((u for u in reversed(slots[max(0, t - page):t]) if u >= 0), None)
+            good = before is None or before // page != s // page
+            refused |= not good
+        out.append(s if good else -1)
+    return np.array(out), refused
+
+
+def _append(cuda, native, slots, *, page, heads, dim, code, pages, guard=4096, seed=0):
+    """Appends to caches with guard bytes on both sides; checks codes, scales, guards and the status."""
+    import torch
+    kinds = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+    rng = np.random.default_rng(seed)
+    n = pages * heads * page * dim
+    whole = [torch.full((n + 2 * guard,), 0x38, dtype=torch.uint8, device=cuda) for _ in range(2)]
+    caches = [w[guard:guard + n].view(kinds[code]).view(pages, heads, page, dim) for w in whole]
+    scales = [torch.full((pages, heads), 2.0 ** -6, device=cuda) for _ in range(2)]
+    k, v = (torch.tensor(rng.standard_normal((len(slots), heads, dim)) * np.exp2(rng.integers(-6, 3, (len(slots), heads, 1))),
+                         device=cuda).half() for _ in range(2))
+    kept, refused = _kept(slots, page, pages)
+    want = [ref.append(x.float().cpu().numpy(), kept, c.float().cpu().numpy(), s.cpu().numpy(), code, other)
+            for x, c, s, other in zip((k, v), caches, scales, (v.float().cpu().numpy(), None))]
+    _kv().kv_append(k, v, torch.tensor(np.asarray(slots), dtype=torch.int64, device=cuda), *caches, *scales)
+    torch.cuda.synchronize()
+    for (wc, ws), c, s, w in zip(want, caches, scales, whole):
+        assert np.array_equal(s.cpu().numpy(), ws)
+        assert np.array_equal(c.float().cpu().numpy(), wc)
+        assert bool((w[:guard] == 0x38).all()) and bool((w[guard + n:] == 0x38).all())
+    refused |= bool((np.asarray(slots) >= pages * page).any())
+    assert native.device_status(clear=True) == (7 if refused else 0)
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("page,dim", [(16, 128), (32, 64), (64, 128), (128, 64)])
+def test_append_stays_within_its_tile(native, cuda, page, dim, code):
+    """Slots that repeat, jump, turn back or wrap within a page, at the end of the cache too."""
+    P, pages, heads = page, 6, 2
+    end = pages * P
+    for slots in ([end - 1] * (2 * P), [end - 1, end - P], [end - 2, end - 1, end - 1, end - 1],
+                  [end - P + 3, end - P + 5, end - P + 6], list(range(end - 1, end - P - 1, -1)),
+                  list(range(end - P // 2, end)) + list(range(end - P, end - P // 2)),
+                  [0, 1, -1, 3, -1, 4], [0] + [-1] * (P - 1) + [1], [end - 1, end, end + 1, end - 1],
+                  [0, 0, P, P + 1, P + 1, 2 * P, 2 * P + 1] + list(range(3 * P, 4 * P)) * 2 + [5 * P]):
+        _append(cuda, native, slots, page=page, heads=heads, dim=dim, code=code, pages=pages)
+
+
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_append_skipped_rows_between_pages(native, cuda, page):
+    """Rows skipped before, between and behind the pages of a padded layout are no fault."""
+    P = page
+    slots = [-1] * 5 + [3, 4, 5] + [-1] * (P + 40) + [P, P + 1] + [-1] * 3 + list(range(2 * P - 1 + P, 4 * P)) + [-1] * 70
+    assert not _kept(slots, P, 8)[1]
+    _append(cuda, native, slots, page=P, heads=3, dim=64, code="int8", pages=8)
+
+
+def test_append_any_slots(native, cuda):
+    """Stretches of random kinds, in small and in page-sized windows of a launch.  A page returns only next to itself."""
+    rng = np.random.default_rng(7)
+    for page, heads, pages, tokens in ((16, 2, 400, 700), (64, 8, 200, 2000), (128, 8, 60, 2500), (32, 4, 300, 1500)):
+        order, slots = list(rng.permutation(pages)), []
+        while len(slots) < tokens and order:
+            p = int(order.pop()) * page
+            for _ in range(int(rng.integers(1, 4))):
+                a, b = sorted(rng.integers(0, page + 1, 2))
+                stretch = list(range(p + int(a), p + int(b)))
+                kind = rng.integers(0, 6)
+                slots += stretch[::-1] if kind == 0 else stretch[::2] if kind == 1 else stretch[:1] * 5 if kind == 2 else stretch
+                if kind == 3:
+                    slots += [-1] * int(rng.integers(1, page // 2))
+        _append(cuda, native, slots, page=page, heads=heads, dim=128, code="e4m3", pages=pages, seed=page)

@@ -11,9 +11,12 @@
 // memory.  New pages are read from the free list, not from the table, so the
 // table's writers and readers need no order.
 //
-// kv_append: a run is the consecutive tokens of one page.  A CTA takes the
-// runs that START in its window of tokens, for one kv head, K and V: every tile
-// has one writer, and its scale is settled without a second pass over memory.
+// kv_append: a run is consecutive tokens at consecutive slots of one page, so it
+// ends within its tile.  A CTA takes the runs that START in its window of
+// tokens, for one kv head, K and V: every tile has one writer, and its scale is
+// settled without a second pass over memory.  A run whose page the kept token
+// before it shares (slots that repeat, jump or turn back, a skipped row inside
+// a page) would be a second writer: it is skipped with a status.
 // Rows are read once, 16 bytes a lane, and stay in registers between the
 // maximum and the coding: runs of up to 8 iterations of one warp are a warp's
 // alone (no barrier), longer ones the CTA's.  Bound: HBM, 2 bytes read and 1
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv_append_kernel(cons
     constexpr int RPW = 32 / LPR;           // rows per warp and iteration; even rows are K's, odd ones V's
     constexpr int kWarps = THREADS / 32;
     constexpr int kAlone = kAppendHold * RPW / 2;  // tokens of a run that one warp holds
-    __shared__ int64_t slot[2 * kMaxPage + 1];     // 0: the token before the window
+    __shared__ int64_t slots_near[3 * kMaxPage];   // of the tokens from a page's length before the window on
     __shared__ uint32_t starts[(2 * kMaxPage) / 32];
     __shared__ int16_t begins[kMaxPage + 1];       // the window's runs: first token
     __shared__ int n_runs;
@@ -229,26 +232,35 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv_append_kernel(cons
     const int sh = a.shift, P = 1 << sh, W = a.window, span = (W + P + 31) & ~31;
     const int h = blockIdx.y;
     const int64_t w0 = int64_t(blockIdx.x) * W;
+    const int64_t* slot = slots_near + P;  // slot[i]: of token w0 + i, -1: skipped, -2: before the call
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-    for (int i = tid; i <= span; i += THREADS) {
-        const int64_t t = w0 - 1 + i;
+    for (int i = tid; i < P + span; i += THREADS) {
+        const int64_t t = w0 - P + i;
         int64_t v = t >= 0 && t < a.T ? a.slots[t] : -1;
         if (v >= (a.pages << sh)) {
-            if (h == 0 && i > 0) set_status(a.status, DEV_BAD_INDEX);
+            if (h == 0 && i >= P) set_status(a.status, DEV_BAD_INDEX);
             v = -1;
         }
-        slot[i] = v < 0 ? -1 : v;
+        slots_near[i] = t < 0 ? -2 : v < 0 ? -1 : v;
     }
     if (tid == 0) n_runs = 0;
     __syncthreads();
     for (int i = tid; i < span; i += THREADS) {
-        const int64_t v = slot[i + 1], u = slot[i];
+        const int64_t v = slot[i], u = slot[i - 1];
         // skipped tokens count as a run of their own, so that they end the one before
-        const bool start = v >= 0 ? u < 0 || (u >> sh) != (v >> sh) : u >= 0;
+        const bool start = v >= 0 ? v != u + 1 || !(v & (P - 1)) : u >= 0;
         const uint32_t m = __ballot_sync(0xffffffffu, start);
         if (lane == 0) starts[i >> 5] = m;
-        if (start && v >= 0 && i < W) begins[atomicAdd(&n_runs, 1)] = int16_t(i);  // in any order
+        if (start && v >= 0 && i < W) {
+            int64_t before = u;  // the kept token before this one, up to a page's length back
+            for (int j = i - 2; before == -1 && j >= i - P; --j) before = slot[j];
+            if (before >= 0 && (before >> sh) == (v >> sh)) {
+                if (h == 0) set_status(a.status, DEV_BAD_INDEX);
+            } else {
+                begins[atomicAdd(&n_runs, 1)] = int16_t(i);  // in any order
+            }
+        }
     }
     __syncthreads();
     const int last = int(min(int64_t(span), a.T - w0));
@@ -257,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv_append_kernel(cons
         if (i + 1 >= span) return last;
         uint32_t m = starts[w] & (0xffffffffu << ((i + 1) & 31));
         while (m == 0 && ++w < (span >> 5)) m = starts[w];
-        return min(min(m ? (w << 5) + __ffs(m) - 1 : span, last), i + P);
+        return min(m ? (w << 5) + __ffs(m) - 1 : span, last);
     };
 
     const int sub = lane / LPR, which = sub & 1, col = (lane % LPR) * 8;
@@ -303,7 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv_append_kernel(cons
     auto code = [&](auto odd, int first, int n, int row0, int step, int e) {
         constexpr bool ODD = decltype(odd)::value;
         const float inv = exp2_int(-e);
-        const int64_t s = slot[first + 1];
+        const int64_t s = slot[first];
         const int64_t base = (((s >> sh) * a.heads + h) << sh) + (s & (P - 1));
         #pragma unroll
         for (int i = 0; i < kAppendHold; ++i) {
@@ -345,7 +357,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv_append_kernel(cons
     constexpr float kMost = (E4M3 ? 448.f : 127.f) * 1099511627776.f;  // at the largest scale, 2^40
     // the scale of the run's tile, and the one it had
     auto settle = [&](int first, float m, int& old) {
-        const int64_t s = slot[first + 1];
+        const int64_t s = slot[first];
         const float* sc = scales + (s >> sh) * a.heads + h;
         int e = scale_exponent<E4M3>(m);
         old = e;
@@ -356,12 +368,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) kv_append_kernel(cons
         return e;
     };
     auto publish = [&](int first, int e) {
-        const int64_t s = slot[first + 1];
+        const int64_t s = slot[first];
         scales[(s >> sh) * a.heads + h] = exp2_int(e);
     };
     // the scale grew: the tile's older codes (rows row0, row0 + step, ... of its first tokens) move to it
     auto again = [&](int first, int row0, int step, int old, int e) {
-        const int64_t s = slot[first + 1], base = ((s >> sh) * a.heads + h) << sh;
+        const int64_t s = slot[first], base = ((s >> sh) * a.heads + h) << sh;
         const int off = int(s & (P - 1));
         const float f = exp2_int(max(old - e, -126));
         for (int r = row0; (r >> 1) < off; r += step) {

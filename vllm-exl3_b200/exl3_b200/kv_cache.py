@@ -140,6 +140,11 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
     slices of a fused projection included) into the cache at ``slots`` (int64,
     from :func:`kv_plan`; negative: skipped).
 
+    The tokens of a page in one call must be one stretch of rows at
+    consecutive slots, which is how :func:`kv_plan` gives them: rows that
+    repeat, jump or turn back within the page of the row before them are
+    skipped with status 7, and so is what follows a skipped row inside a page.
+
     A page's scale is set by the call that writes its first token and grows
     when a later token needs it, the older codes being rounded to it again.
     In e4m3 a NaN of ``v`` is kept in the token's key (attention rows that see
