@@ -344,7 +344,9 @@ int exl3_kv_append(const exl3_kv_append_args* args, void* stream);
  * of 16 bytes; out [q_rows][heads][dim] in q's type; lse (NULL, or fp32
  * [q_rows][heads]) the log of the softmax's denominator.  A row that sees no
  * key, and rows past the last request, are zeros with lse -inf.  Keys whose
- * page is not in the cache are not seen, with status 7.  Results do not
+ * page is not in the cache are not seen, with status 7.  Of a request whose
+ * rows reach past q the ones in q are computed, one that begins before q has
+ * none, with status 7.  Results do not
  * depend on timing: repeats are equal bit for bit. */
 /* Workspace of this entry and of exl3_token_logprobs: 256-byte aligned, all
  * zero before its first use (zeroed on the device, not by a fill that a

@@ -91,3 +91,65 @@ def test_append_any_slots(native, cuda):
                 if kind == 3:
                     slots += [-1] * int(rng.integers(1, page // 2))
         _append(cuda, native, slots, page=page, heads=heads, dim=128, code="e4m3", pages=pages, seed=page)
+
+
+# --- attend -----------------------------------------------------------------
+
+def _attend_problem(cuda, lens, new, *, heads=4, kv_heads=2, dim=64, page=16, seed=0):
+    import torch
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    width = max(1, max(-(-n // page) for n in lens))
+    pages = len(lens) * width
+    kc, vc = (torch.randint(-127, 128, (pages, kv_heads, page, dim), generator=g, device=cuda).to(torch.int8)
+              for _ in range(2))
+    ks, vs = (torch.full((pages, kv_heads), 2.0 ** -6, device=cuda) for _ in range(2))
+    i = lambda v: torch.tensor(np.asarray(v), dtype=torch.int32, device=cuda)  # noqa: E731
+    table = torch.randperm(pages, generator=g, device=cuda).to(torch.int32).view(len(lens), width)
+    q = torch.randn(sum(new), heads, dim, generator=g, device=cuda).half()
+    return dict(q=q, k_cache=kc, v_cache=vc, k_scale=ks, v_scale=vs, block_table=table, kv_lens=i(lens),
+                cu_tokens=i(np.concatenate([[0], np.cumsum(new)])), max_new=max(new), return_lse=True)
+
+
+def _plain(p):
+    """The 64-bit form of a problem: out, lse and their bounds (f16 outputs; derived in test_gpu_kv_cache.py)."""
+    D, n = p["q"].shape[2], max(int(p["kv_lens"].max()), 1)
+    kv = [c.double().cpu().numpy() * s.double().cpu().numpy()[:, :, None, None]
+          for c, s in ((p["k_cache"], p["k_scale"]), (p["v_cache"], p["v_scale"]))]
+    out, lse, amp, vmax, smax = ref.attend(p["q"].double().cpu().numpy(), kv, p["block_table"].cpu().numpy(),
+                                           p["kv_lens"].cpu().numpy(), p["cu_tokens"].cpu().numpy(), D ** -0.5, 0)
+    tol = 2.0 ** -11 * np.abs(out) + (2.0 ** -11 + 2.0 ** -13) * amp + n * 2.0 ** -24 * vmax + 2.0 ** -25
+    ltol = D * 2.0 ** -23 * smax + 2.0 ** -17 * (1 + np.abs(np.where(np.isinf(lse), 0, lse)))
+    return out, lse, tol, ltol
+
+
+def _near(got, want, rows=slice(None)):
+    (out, lse), (wout, wlse, tol, ltol) = got, want
+    out, lse = out.double().cpu().numpy()[rows], lse.double().cpu().numpy()[rows]
+    assert (np.abs(out - wout[rows]) <= tol[rows]).all()
+    empty = np.isneginf(wlse[rows])
+    assert np.array_equal(np.isneginf(lse), empty)
+    assert (np.abs(np.where(empty, 0, lse) - np.where(empty, 0, wlse[rows])) <= ltol[rows]).all()
+
+
+@pytest.mark.parametrize("new", [[2, 1, 3], [70, 90, 130]])
+def test_attend_row_offsets_outside_q(native, cuda, new):
+    """cu_tokens that leave q: nothing outside is read or written, rows inside stand, status 7."""
+    import torch
+    p = _attend_problem(cuda, [150, 200, 170], new)
+    want = _plain(p)
+    _near(_kv().kv_attend(**p), want)
+    n, big = sum(new), 2 ** 31 - 1
+    first, second = new[0], new[0] + new[1]
+    for cu, stands in (([-5, first, second, n], (first, n)), ([0, first, second, n + 7], (0, second)),
+                       ([0, first, second, big], (0, second)), ([-big, first, second, n], (first, n)),
+                       ([0, first, n + 3, n + 9], (0, first)), ([-2 ** 31, -4, second, -1], (0, 0)),
+                       ([big, big, big, big], (0, 0)), ([0, big, -big, big], (0, 0))):
+        bad = {**p, "cu_tokens": torch.tensor(cu, dtype=torch.int32, device=cuda)}
+        got = _kv().kv_attend(**bad)
+        torch.cuda.synchronize()
+        _near(got, want, slice(*stands))
+        assert native.device_status(clear=True) == (0 if cu == [big] * 4 else 7), cu
+    # a request that q cuts short keeps the positions of all its rows
+    cut = {**p, "q": p["q"][:-1]}
+    _near(_kv().kv_attend(**cut), [w[:-1] for w in want])
+    assert native.device_status(clear=True) == 7

@@ -86,20 +86,21 @@ constexpr int kAttFew = 48;
 
 // what a request asks for
 struct AttReq {
-    int len, fresh, lo16, groups, units;  // keys, new rows, first key's tile, column groups, units per item
+    int len, first, rows, lo16, groups, units;  // keys, first row's position, rows, first key's tile, column groups, units per item
     int64_t row0;
 };
 
 template <int NC>
 __device__ __forceinline__ AttReq att_request(const KvAttendArgs& a, int b) {
     AttReq r;
-    r.row0 = a.cu ? a.cu[b] : b;
-    r.fresh = a.cu ? max(a.cu[b + 1] - int(r.row0), 0) : 1;
+    const AttRows w = att_rows(a, b);
+    r.row0 = w.row0, r.rows = w.rows;
     r.len = int(min(int64_t(max(a.kv_lens[b], 0)), int64_t(a.width) << a.shift));
-    const int first = r.len - r.fresh;  // position of the first new row
-    const int lo = a.window > 0 ? max(first + 1 - a.window, 0) : 0;
+    r.first = r.len - w.fresh;
+    const int lo = a.window > 0 ? max(r.first + 1 - a.window, 0) : 0;
     r.lo16 = min(lo, r.len) & ~15;
-    r.groups = int64_t(r.fresh) * a.group > a.few ? 0 : (r.fresh * a.group + NC - 1) / NC;
+    const int64_t columns = int64_t(r.rows) * a.group;
+    r.groups = columns > a.few ? 0 : int((columns + NC - 1) / NC);
     r.units = max((r.len - r.lo16 + kAttUnit - 1) / kAttUnit, 1);
     return r;
 }
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
     total += cost * n_items, incl += cost * items_incl, mine += cost * items;
     // rows no request owns are zeros
     if (a.cu) {
-        const int64_t live = a.cu[a.requests], n = (a.q_rows - live) * a.heads;
+        const int64_t live = max(a.cu[a.requests], 0), n = (a.q_rows - live) * a.heads;
         for (int64_t i = int64_t(blockIdx.x) * kAttWarps + warp; i < n; i += int64_t(gridDim.x) * kAttWarps) {
             const int64_t row = live * a.heads + i;
             for (int d = lane; d < D; d += 32) a.out[row * D + d] = 0;
@@ -213,13 +214,13 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
         const int n_units = int(u - u_item) - off;
         if (n_units <= 0) break;  // the CTA's part of the line ends before the item's first unit
         const int hk = int(item / rq.groups), cg = int(item % rq.groups);
-        const int ncols = min(rq.fresh * G - cg * NC, NC);
+        const int ncols = int(min(int64_t(rq.rows) * G - int64_t(cg) * NC, int64_t(NC)));
 
         // --- the query columns: B fragments of Q^T (a warp to each 8), and each column's key range ---
         for (int t = warp; t < NT; t += kAttWarps) {
             const int n = 8 * t + g, f = cg * NC + n;
             const int64_t row = rq.row0 + f / G;
-            const bool live = n < ncols && row < a.q_rows;
+            const bool live = n < ncols;
             const uint16_t* qp = a.q + (live ? row * a.q_tok + int64_t(hk * G + f % G) * a.q_head : 0);
             float fac = a.scale_log2;
             uint2 w[KS];
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
         for (int t = 0; t < NT; ++t)
             #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int col = 8 * t + 2 * c + i, pos = rq.len - rq.fresh + (cg * NC + col) / G;
+                const int col = 8 * t + 2 * c + i, pos = rq.first + (cg * NC + col) / G;
                 cfac[t][i] = qfac[col];
                 hi[t][i] = col < ncols ? min(pos + 1, rq.len) : 0;
                 lo[t][i] = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
         auto emit = [&](int col, int d, float value, float sum, float mx) {
             const int f = cg * NC + col;
             const int64_t row = rq.row0 + f / G;
-            if (col >= ncols || row >= a.q_rows) return;
+            if (col >= ncols) return;
             const int64_t at = row * a.heads + hk * G + f % G;
             const float r = sum == 0.f ? 0.f : value / sum;  // a row that sees no key is zero
             a.out[at * D + d] = BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(r)) : __half_as_ushort(__float2half_rn(r));

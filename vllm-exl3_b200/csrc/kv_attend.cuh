@@ -27,6 +27,21 @@ struct KvAttendArgs {
     int* status;
 };
 
+// A request's rows of q: its positions count from all `fresh` that cu_tokens
+// names, `rows` of them are computed.  They are fewer where cu_tokens leaves
+// the tensor, which is recorded, so that no offset here leaves it.
+struct AttRows {
+    int64_t row0;
+    int fresh, rows;
+};
+__device__ __forceinline__ AttRows att_rows(const KvAttendArgs& a, int b) {
+    if (!a.cu) return AttRows{b, 1, 1};
+    const int64_t row0 = a.cu[b], n = max(a.cu[b + 1] - row0, int64_t(0));
+    const int rows = row0 < 0 ? 0 : int(max(min(n, a.q_rows - row0), int64_t(0)));
+    if (rows < n) set_status(a.status, DEV_BAD_INDEX);
+    return AttRows{row0, int(min(n, int64_t(INT32_MAX))), rows};
+}
+
 // two codes (bytes 0, 1 of w; int8 already offset by 128) as f16x2, exact
 template <bool E4M3>
 __device__ __forceinline__ uint32_t half2_lo(uint32_t w) {

@@ -132,11 +132,8 @@ __device__ __forceinline__ void pr_wait(uint64_t* bar, uint32_t parity, int* sta
     }
 }
 
-__device__ __forceinline__ int64_t pr_columns(const KvAttendArgs& a, int b) {
-    return int64_t(a.cu ? max(a.cu[b + 1] - a.cu[b], 0) : 1) * a.group;
-}
 __device__ __forceinline__ int pr_tiles(const KvAttendArgs& a, int b) {
-    const int64_t cols = pr_columns(a, b);
+    const int64_t cols = int64_t(att_rows(a, b).rows) * a.group;
     return cols > a.few ? int((cols + kPrRows - 1) / kPrRows) : 0;
 }
 
@@ -147,11 +144,11 @@ struct PrTile {
 };
 __device__ __forceinline__ PrTile pr_tile(const KvAttendArgs& a, int b, int tile) {
     PrTile t;
-    t.row0 = a.cu ? a.cu[b] : b;
-    t.fresh = a.cu ? a.cu[b + 1] - int(t.row0) : 1;
+    const AttRows w = att_rows(a, b);
+    t.row0 = w.row0, t.fresh = w.fresh;
     t.len = int(min(int64_t(max(a.kv_lens[b], 0)), int64_t(a.width) << a.shift));
     t.col0 = int64_t(tile) * kPrRows;
-    t.rows = int(min(int64_t(t.fresh) * a.group - t.col0, int64_t(kPrRows)));
+    t.rows = int(min(int64_t(w.rows) * a.group - t.col0, int64_t(kPrRows)));
     const int first = t.len - t.fresh + int(t.col0 / a.group), last = t.len - t.fresh + int((t.col0 + t.rows - 1) / a.group);
     t.hi = max(min(last + 1, t.len), 0);
     t.lo = min(a.window > 0 ? max(first + 1 - a.window, 0) : 0, t.hi);
@@ -438,15 +435,15 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
             }
             // --- this thread's row ---
             const int64_t fc = im.col0 + f, row = im.row0 + fc / G;
-            const bool mine = f < im.rows, live = mine && row < a.q_rows;
+            const bool mine = f < im.rows;
             const int64_t at = row * a.heads + im.hk * G + fc % G;
             float cfac = fabsf(a.scale_log2);
             {
                 const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;  // group maxima below need a factor >= 0
-                const uint4* qp = reinterpret_cast<const uint4*>(a.q + (live ? row * a.q_tok + int64_t(im.hk * G + fc % G) * a.q_head : 0));
+                const uint4* qp = reinterpret_cast<const uint4*>(a.q + (mine ? row * a.q_tok + int64_t(im.hk * G + fc % G) * a.q_head : 0));
                 uint4 x[D / 8];
                 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) x[i] = live ? __ldg(qp + i) : make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < D / 8; ++i) x[i] = mine ? __ldg(qp + i) : make_uint4(0, 0, 0, 0);
                 float mul = sign;
                 if constexpr (BF16) {
                     // to f16 by a power of two per row: largest magnitude in [2^14, 2^15), so that
@@ -590,12 +587,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                     if (inv == 0.f) x[i] = 0u;
                 }
                 uint4* dst = reinterpret_cast<uint4*>(a.out + at * D + 32 * h);
-                if (live)
+                if (mine)
                     #pragma unroll
                     for (int i = 0; i < 4; ++i) dst[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
             };
             auto emit_lse = [&](float m, float sum) {
-                if (live && a.lse) a.lse[at] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+                if (mine && a.lse) a.lse[at] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
             };
             const bool whole = steps == im.all;
             float* part = a.part + (int64_t(2 * cta + (im.off == 0 ? 1 : 0)) * 2 + t) * pr_part<D>();
