@@ -110,13 +110,13 @@ def _attend_problem(cuda, lens, new, *, heads=4, kv_heads=2, dim=64, page=16, se
                 cu_tokens=i(np.concatenate([[0], np.cumsum(new)])), max_new=max(new), return_lse=True)
 
 
-def _plain(p):
+def _plain(p, window=0):
     """The 64-bit form of a problem: out, lse and their bounds (f16 outputs; derived in test_gpu_kv_cache.py)."""
     D, n = p["q"].shape[2], max(int(p["kv_lens"].max()), 1)
     kv = [c.double().cpu().numpy() * s.double().cpu().numpy()[:, :, None, None]
           for c, s in ((p["k_cache"], p["k_scale"]), (p["v_cache"], p["v_scale"]))]
     out, lse, amp, vmax, smax = ref.attend(p["q"].double().cpu().numpy(), kv, p["block_table"].cpu().numpy(),
-                                           p["kv_lens"].cpu().numpy(), p["cu_tokens"].cpu().numpy(), D ** -0.5, 0)
+                                           p["kv_lens"].cpu().numpy(), p["cu_tokens"].cpu().numpy(), D ** -0.5, window)
     tol = 2.0 ** -11 * np.abs(out) + (2.0 ** -11 + 2.0 ** -13) * amp + n * 2.0 ** -24 * vmax + 2.0 ** -25
     ltol = D * 2.0 ** -23 * smax + 2.0 ** -17 * (1 + np.abs(np.where(np.isinf(lse), 0, lse)))
     return out, lse, tol, ltol
@@ -152,4 +152,26 @@ def test_attend_row_offsets_outside_q(native, cuda, new):
     # a request that q cuts short keeps the positions of all its rows
     cut = {**p, "q": p["q"][:-1]}
     _near(_kv().kv_attend(**cut), [w[:-1] for w in want])
+    assert native.device_status(clear=True) == 7
+
+
+@pytest.mark.parametrize("new", [[5, 1, 3, 2], [70, 64, 90, 5]])
+def test_attend_lengths_beyond_the_table(native, cuda, new):
+    """Tokens that the block table has no place for are not seen; the rows keep their positions."""
+    import torch
+    lens = [100, 90, 96, 71]
+    p = _attend_problem(cuda, lens, new)
+    p["kv_lens"] = torch.tensor([117, 90, 96, 75], dtype=torch.int32, device=cuda)
+    p["block_table"] = p["block_table"][:, :4].contiguous()  # places for 64
+    wide = torch.full((4, 8), -1, dtype=torch.int32, device=cuda)
+    wide[:, :4] = p["block_table"]
+    for window in (0, 12, 40):
+        got = _kv().kv_attend(**p, window=window)
+        _near(got, _plain({**p, "block_table": wide}, window))
+        assert native.device_status(clear=True) == 7
+    p["kv_lens"] = torch.tensor([64, 60, 64, 7], dtype=torch.int32, device=cuda)
+    _kv().kv_attend(**p)
+    assert native.device_status(clear=True) == 0
+    p["kv_lens"] = torch.full((4,), 2 ** 31 - 1, dtype=torch.int32, device=cuda)
+    assert not _kv().kv_attend(**p, window=50)[0].any()  # every row is far behind the table
     assert native.device_status(clear=True) == 7

@@ -86,7 +86,7 @@ constexpr int kAttFew = 48;
 
 // what a request asks for
 struct AttReq {
-    int len, first, rows, lo16, groups, units;  // keys, first row's position, rows, first key's tile, column groups, units per item
+    int keys, first, rows, lo16, groups, units;  // keys, first row's position, rows, first key's tile, column groups, units per item
     int64_t row0;
 };
 
@@ -95,13 +95,13 @@ __device__ __forceinline__ AttReq att_request(const KvAttendArgs& a, int b) {
     AttReq r;
     const AttRows w = att_rows(a, b);
     r.row0 = w.row0, r.rows = w.rows;
-    r.len = int(min(int64_t(max(a.kv_lens[b], 0)), int64_t(a.width) << a.shift));
-    r.first = r.len - w.fresh;
+    const int len = max(a.kv_lens[b], 0);
+    r.keys = att_keys(a, len), r.first = len - w.fresh;
     const int lo = a.window > 0 ? max(r.first + 1 - a.window, 0) : 0;
-    r.lo16 = min(lo, r.len) & ~15;
+    r.lo16 = min(lo, r.keys) & ~15;
     const int64_t columns = int64_t(r.rows) * a.group;
     r.groups = columns > a.few ? 0 : int((columns + NC - 1) / NC);
-    r.units = max((r.len - r.lo16 + kAttUnit - 1) / kAttUnit, 1);
+    r.units = max((r.keys - r.lo16 + kAttUnit - 1) / kAttUnit, 1);
     return r;
 }
 
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
             for (int i = 0; i < 2; ++i) {
                 const int col = 8 * t + 2 * c + i, pos = rq.first + (cg * NC + col) / G;
                 cfac[t][i] = qfac[col];
-                hi[t][i] = col < ncols ? min(pos + 1, rq.len) : 0;
+                hi[t][i] = col < ncols ? min(pos + 1, rq.keys) : 0;
                 lo[t][i] = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
             }
         int full_lo = 0, full_hi = 0x7fffffff;  // keys in [full_lo, full_hi) need no test
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
         }
 
         const int first = rq.lo16 + off * kAttUnit + warp * 16;
-        const int end = min(rq.len, rq.lo16 + (off + n_units) * kAttUnit);
+        const int end = min(rq.keys, rq.lo16 + (off + n_units) * kAttUnit);
         const int32_t* row_table = a.table + int64_t(b) * a.width;
         auto page_at = [&](int tok) { return tok < end ? __ldg(row_table + (tok >> a.shift)) : -1; };
 
@@ -433,10 +433,10 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
                 pf[t][0] = transpose8x8(pack_half2(p[0], p[1]));
                 pf[t][1] = transpose8x8(pack_half2(p[2], p[3]));
             }
-            if (E4M3 && tok + 16 > rq.len) {  // codes past the end may be NaN, and 0 * NaN is not 0
+            if (E4M3 && tok + 16 > rq.keys) {  // codes past the end may be NaN, and 0 * NaN is not 0
                 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (tok + 2 * c + (i & 1) + (i >> 1) * 8 >= rq.len)
+                    if (tok + 2 * c + (i & 1) + (i >> 1) * 8 >= rq.keys)
                         #pragma unroll
                         for (int w = 0; w < D / 32; ++w) vr[i][w] = 0u;
             }

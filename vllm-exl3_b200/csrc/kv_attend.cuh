@@ -42,6 +42,14 @@ __device__ __forceinline__ AttRows att_rows(const KvAttendArgs& a, int b) {
     return AttRows{row0, int(min(n, int64_t(INT32_MAX))), rows};
 }
 
+// Tokens of request b that the block table has a place for.  The others are
+// not seen; they count for the rows' positions all the same.
+__device__ __forceinline__ int att_keys(const KvAttendArgs& a, int len) {
+    const int64_t room = int64_t(a.width) << a.shift;
+    if (len > room) set_status(a.status, DEV_BAD_INDEX);
+    return int(min(int64_t(len), room));
+}
+
 // two codes (bytes 0, 1 of w; int8 already offset by 128) as f16x2, exact
 template <bool E4M3>
 __device__ __forceinline__ uint32_t half2_lo(uint32_t w) {

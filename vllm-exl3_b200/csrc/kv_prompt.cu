@@ -78,7 +78,7 @@ struct PrStep {
 struct PrItem {
     int64_t row0, col0;
     int steps, off, all;  // steps 0: no more items
-    int rows, hk, fresh, len, k_begin;
+    int rows, hk, first, keys, k_begin;
     int c0, c1;           // the CTAs that share the item
 };
 constexpr int kPrItems = 4;
@@ -140,17 +140,18 @@ __device__ __forceinline__ int pr_tiles(const KvAttendArgs& a, int b) {
 // 256 rows of a request and the keys that any of them sees
 struct PrTile {
     int64_t row0, col0;
-    int fresh, len, rows, lo, hi, k_begin, steps;
+    int first, keys, rows, lo, hi, k_begin, steps;  // first: position of the request's first row
 };
 __device__ __forceinline__ PrTile pr_tile(const KvAttendArgs& a, int b, int tile) {
     PrTile t;
     const AttRows w = att_rows(a, b);
-    t.row0 = w.row0, t.fresh = w.fresh;
-    t.len = int(min(int64_t(max(a.kv_lens[b], 0)), int64_t(a.width) << a.shift));
+    t.row0 = w.row0;
+    const int len = max(a.kv_lens[b], 0);
+    t.keys = att_keys(a, len), t.first = len - w.fresh;
     t.col0 = int64_t(tile) * kPrRows;
     t.rows = int(min(int64_t(w.rows) * a.group - t.col0, int64_t(kPrRows)));
-    const int first = t.len - t.fresh + int(t.col0 / a.group), last = t.len - t.fresh + int((t.col0 + t.rows - 1) / a.group);
-    t.hi = max(min(last + 1, t.len), 0);
+    const int first = t.first + int(t.col0 / a.group), last = t.first + int((t.col0 + t.rows - 1) / a.group);
+    t.hi = max(min(last + 1, t.keys), 0);
     t.lo = min(a.window > 0 ? max(first + 1 - a.window, 0) : 0, t.hi);
     t.k_begin = t.lo & ~15;  // pages and scales are looked up by 16 keys
     t.steps = max((t.hi - t.k_begin + kPrKeys - 1) / kPrKeys, 1);  // rows that see nothing take one step too
@@ -474,8 +475,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                 tc_fence_before();
                 mbar_arrive(&sm.q_full[t]);
             }
-            const int pos = im.len - im.fresh + int(fc / G);
-            const int hi = mine ? min(pos + 1, im.len) : 0;
+            const int pos = im.first + int(fc / G);
+            const int hi = mine ? min(pos + 1, im.keys) : 0;
             const int lo = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
             float ref = -INFINITY, l = 0.f;
             // of scores: above 0 whatever the scales, so that -inf stays -inf
@@ -803,7 +804,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                     im.hk = int((u - w.base) / w.t.steps);
                     im.off = int(u - w.base - int64_t(im.hk) * w.t.steps);
                     im.all = w.t.steps, im.steps = int(min(int64_t(w.t.steps - im.off), u1 - u));
-                    im.row0 = w.t.row0, im.col0 = w.t.col0, im.rows = w.t.rows, im.fresh = w.t.fresh, im.len = w.t.len;
+                    im.row0 = w.t.row0, im.col0 = w.t.col0, im.rows = w.t.rows, im.first = w.t.first, im.keys = w.t.keys;
                     im.k_begin = w.t.k_begin;
                     // its first step's place on the line
                     const int64_t first = u - im.off + int64_t(kPrItemCost) * (int64_t(w.index) * Hk + im.hk + 1);
