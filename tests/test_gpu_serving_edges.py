@@ -175,3 +175,34 @@ def test_attend_lengths_beyond_the_table(native, cuda, new):
     p["kv_lens"] = torch.full((4,), 2 ** 31 - 1, dtype=torch.int32, device=cuda)
     assert not _kv().kv_attend(**p, window=50)[0].any()  # every row is far behind the table
     assert native.device_status(clear=True) == 7
+
+
+# --- plan -------------------------------------------------------------------
+
+def test_plan_request_counts(native, cuda):
+    """Up to the limit, from small to large in a process of its own: a larger launch must not be what lets a smaller one through."""
+    import os
+    import subprocess
+    import sys
+
+    from conftest import PKG
+    code = """
+import numpy as np, torch
+from exl3_b200.kv_cache import kv_plan
+for B in (6000, 6125, 6126, 6130, 6143, 6144, 9000, 16384):
+    lens = torch.arange(B, dtype=torch.int32, device="cuda") % 50
+    new = torch.ones_like(lens)
+    table = torch.arange(B * 4, dtype=torch.int32, device="cuda").view(B, 4)
+    free = torch.arange(B * 4, B * 5, dtype=torch.int32, device="cuda")
+    p = kv_plan(lens, new, table, free, torch.zeros(1, dtype=torch.int32, device="cuda"), page_size=16, n_tokens=B)
+    n = np.arange(B) % 50
+    taken = n % 16 == 0
+    page = np.where(taken, B * 4 + np.cumsum(taken) - 1, np.arange(B) * 4 + n // 16)
+    assert np.array_equal(p.slots.cpu().numpy(), page * 16 + n % 16), B
+    assert np.array_equal(p.positions.cpu().numpy(), n) and int(p.cursor) == taken.sum(), B
+    assert np.array_equal(p.kv_lens.cpu().numpy(), n + 1) and np.array_equal(p.cu_tokens.cpu().numpy(), np.arange(B + 1)), B
+print("planned")
+"""
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([PKG, os.environ.get("PYTHONPATH", "")]))
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=env, timeout=300)
+    assert run.returncode == 0 and "planned" in run.stdout, run.stderr[-2000:]

@@ -166,11 +166,9 @@ cudaError_t run_kv_plan(const KvPlanCall& c, cudaStream_t s) {
     // two tokens a thread: enough CTAs for the stores, few enough that their scans stay one wave
     int grid = (work + 2 * kPlanThreads - 1) / (2 * kPlanThreads);
     grid = grid < 1 ? 1 : grid > 148 ? 148 : grid;
-    if (smem > 48 * 1024) {
-        static std::atomic<uint64_t> done{0};
-        const cudaError_t e = raise_smem(kv_plan_kernel, size_t(kKvMaxRequests + 1) * 8, done);
-        if (e != cudaSuccess) return e;
-    }
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = raise_smem(kv_plan_kernel, size_t(kKvMaxRequests + 1) * 8, done);
+    if (e != cudaSuccess) return e;
     kv_plan_kernel<<<grid, kPlanThreads, smem, s>>>(a);
     return cudaGetLastError();
 }
