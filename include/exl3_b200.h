@@ -284,8 +284,8 @@ enum { EXL3_KV_E4M3 = 0, EXL3_KV_INT8 = 1 };
  * block_table; cursor_out is the cursor after them.  Nothing that it reads is
  * changed, so a call can be repeated.  When the list or the table's width
  * runs out, the tokens concerned get slot -1 (table entries -1) and status 7
- * is recorded; so it is for negative lengths (taken as 0) and for more new
- * tokens than n_tokens.  `status` may be NULL. */
+ * is recorded; so it is for negative lengths (taken as 0), lengths whose sum
+ * passes 2^31 - 1 (cut there) and for more new tokens than n_tokens.  `status` may be NULL. */
 typedef struct exl3_kv_plan_args {
     const int32_t* lens;        /* [requests] */
     const int32_t* new_tokens;  /* [requests] */

@@ -206,3 +206,27 @@ print("planned")
     env = dict(os.environ, PYTHONPATH=os.pathsep.join([PKG, os.environ.get("PYTHONPATH", "")]))
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=env, timeout=300)
     assert run.returncode == 0 and "planned" in run.stdout, run.stderr[-2000:]
+
+
+def test_plan_sums_beyond_32_bits(native, cuda):
+    """Lengths whose sums pass 2^31: what is in order stands, nothing outside the table is read or written, status 7."""
+    import torch
+    big = 2 ** 31 - 1
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    for lens, new in (([3, 5, 0, 7], [2, big, 20, 1]), ([3, 5, 0, 7], [2, big, big, big]),
+                      ([3, big, 9, 7], [2, 5, 20, 1]), ([3, big, big - 1, 0], [2, big, 3, big]),
+                      ([3, big - 9, 100, 7], [2, big, big, 1])):
+        whole = torch.full((3, 4, 6), -5, dtype=torch.int32, device=cuda)
+        table = whole[1]
+        table.copy_(torch.arange(24, device=cuda).view(4, 6))
+        free = torch.arange(100, 140, dtype=torch.int32, device=cuda)
+        p = _kv().kv_plan(i(lens), i(new), table, free, i([0]), page_size=16, n_tokens=30)
+        torch.cuda.synchronize()
+        assert native.device_status(clear=True) == 7
+        assert p.positions[:2].tolist() == [3, 4] and p.slots[:2].tolist() == [3, 4]
+        assert p.kv_lens.tolist() == [min(a + b, big) for a, b in zip(lens, new)]
+        assert p.cu_tokens.tolist()[:2] == [0, 2] and all(0 <= c <= 30 for c in p.cu_tokens.tolist())
+        assert bool((whole[0] == -5).all()) and bool((whole[2] == -5).all())
+        slots = p.slots.tolist()
+        assert all(s == -1 or 0 <= s < 24 * 16 or 100 * 16 <= s < 140 * 16 for s in slots)
+        assert int(p.cursor) == (40 if max(new) == big else 1)

@@ -59,6 +59,8 @@ struct KvPlanArgs {
 
 __device__ __forceinline__ int pages_of(int tokens, int shift) { return int((uint32_t(tokens) + (1u << shift) - 1) >> shift); }
 
+__device__ __forceinline__ int clamp32(long long v) { return int(min(v, (long long)INT32_MAX)); }
+
 // last i in [0, n) with sums[i] <= v; sums[0] = 0 <= v
 __device__ __forceinline__ int find_segment(const int32_t* sums, int n, int v) {
     int lo = 0, hi = n;
@@ -74,10 +76,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const KvPlanArgs 
     extern __shared__ int32_t plan_smem[];
     int32_t* cu = plan_smem;            // [B + 1] token sums
     int32_t* cp = plan_smem + a.B + 1;  // [B + 1] new-page sums
-    __shared__ int2 warp_sum[kPlanThreads / 32];
-    __shared__ int2 carry;
+    __shared__ longlong2 warp_sum[kPlanThreads / 32];
+    __shared__ longlong2 carry;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) carry = make_int2(0, 0);
+    if (tid == 0) carry = make_longlong2(0, 0);
     const int base = *a.cursor;
     bool bad = base < 0;
     __syncthreads();
@@ -87,45 +89,47 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const KvPlanArgs 
         if (b < a.B) {
             len = a.lens[b], n = a.fresh[b];
             if (len < 0 || n < 0) bad = true, len = max(len, 0), n = max(n, 0);
-            need = pages_of(len + n, a.shift) - pages_of(len, a.shift);
+            if (n > INT32_MAX - len) bad = true, n = INT32_MAX - len;
+            // more than list and table hold changes nothing, and makes no longer loop below
+            need = int(min(int64_t(pages_of(len + n, a.shift) - pages_of(len, a.shift)), int64_t(a.n_free) + a.width + 1));
             if (blockIdx.x == 0) a.kv_lens[b] = len + n;
         }
-        int2 s = make_int2(n, need);
+        longlong2 s = make_longlong2(n, need);  // sums of what a caller may have got wrong: they pass 32 bits
         #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, s.x, d), y = __shfl_up_sync(0xffffffffu, s.y, d);
+            const long long x = __shfl_up_sync(0xffffffffu, s.x, d), y = __shfl_up_sync(0xffffffffu, s.y, d);
             if (lane >= d) s.x += x, s.y += y;
         }
         if (lane == 31) warp_sum[warp] = s;
         __syncthreads();
-        int2 before = carry;
+        longlong2 before = carry;
         for (int w = 0; w < warp; ++w) before.x += warp_sum[w].x, before.y += warp_sum[w].y;
-        if (b < a.B) cu[b] = before.x + s.x - n, cp[b] = before.y + s.y - need;
+        if (b < a.B) cu[b] = clamp32(before.x + s.x - n), cp[b] = clamp32(before.y + s.y - need);
         __syncthreads();
-        if (tid == kPlanThreads - 1) carry = make_int2(before.x + s.x, before.y + s.y);
+        if (tid == kPlanThreads - 1) carry = make_longlong2(before.x + s.x, before.y + s.y);
         __syncthreads();
     }
-    const int total = carry.x, pages = carry.y;
+    const int total = clamp32(carry.x), pages = clamp32(carry.y);
     if (tid == 0) cu[a.B] = total, cp[a.B] = pages;
     __syncthreads();
 
     const int i0 = blockIdx.x * kPlanThreads + tid, step = gridDim.x * kPlanThreads;
     for (int b = i0; b <= a.B; b += step) a.cu[b] = min(cu[b], a.n_tokens);
-    for (int p = i0; p < pages; p += step) {
-        const int b = find_segment(cp, a.B, p);
-        const int col = pages_of(max(a.lens[b], 0), a.shift) + p - cp[b];
+    for (int64_t p = i0; p < pages; p += step) {
+        const int b = find_segment(cp, a.B, int(p));
+        const int col = pages_of(max(a.lens[b], 0), a.shift) + int(p) - cp[b];
         const int64_t at = int64_t(base) + p;
         if (at >= a.n_free) bad = true;
         if (col < a.width) a.table[int64_t(b) * a.width + col] = at >= 0 && at < a.n_free ? a.free_pages[at] : -1;
         else bad = true;
     }
-    for (int t = i0; t < a.n_tokens; t += step) {
+    for (int64_t t = i0; t < a.n_tokens; t += step) {
         int pos = 0;
         int64_t slot = -1;
         if (t < total) {
-            const int b = find_segment(cu, a.B, t);
+            const int b = find_segment(cu, a.B, int(t));
             const int len = max(a.lens[b], 0);
-            pos = len + t - cu[b];
+            pos = len + (int(t) - cu[b]);
             const int col = pos >> a.shift, have = pages_of(len, a.shift);
             int page = -1;
             if (col < a.width) {
