@@ -26,8 +26,8 @@
 // dim may sit at any place of the contraction, so a lane's 16 bytes already
 // are its A fragment of K; for V, words of two keys are interleaved with one
 // byte permute.  Like the prompt kernel, a column's reference follows its
-// maximum only when that has grown by more than 2^8, so that the usual tile
-// needs no exchange between lanes and no rescaling.
+// maximum only when that has grown by more than 2^8 (kAttSlack), so that the usual
+// tile needs no exchange between lanes and no rescaling.
 //
 // Measured: 64 single tokens over up to 8192 keys (32 heads over 4, dim 128,
 // e4m3, 343 MB) 70 us, 4.9 TB/s, 75 % of the measured copy rate; 4 requests of
@@ -50,8 +50,6 @@
 namespace exl3 {
 
 constexpr int kAttWarps = 8, kAttThreads = kAttWarps * 32, kAttUnit = 16 * kAttWarps;
-constexpr float kAttSlack = 8.f;  // log2: growth of the maximum that is let pass
-
 constexpr int kAttMaxSms = 160;     // SMs that are used at most
 // Units that an item's start and end are worth on the line, where the CTAs have more than a unit each.  us with 0 / 3 / 5 / 10:
 //   64 single tokens over up to 8192 keys (32 heads over 4, e4m3) 71.4 / 69.5 / 70.0 / 71.6
@@ -402,14 +400,14 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
                     }
                 }
                 #pragma unroll
-                for (int i = 0; i < 2; ++i) grown |= fmaxf(s[t][i], s[t][i + 2]) > m[t][i] + kAttSlack;
+                for (int i = 0; i < 2; ++i) grown |= fmaxf(s[t][i], s[t][i + 2]) > m[t][i] + (kAttLift + kAttSlack);
             }
             if (__any_sync(0xffffffffu, grown)) {  // -inf + slack is -inf: the first key that is seen counts as growth
                 #pragma unroll
                 for (int t = 0; t < NT; ++t)
                     #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float mx = fmaxf(m[t][i], fmaxf(s[t][i], s[t][i + 2]));
+                        float mx = fmaxf(m[t][i], fmaxf(s[t][i], s[t][i + 2]) - kAttLift);
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));

@@ -6,6 +6,15 @@
 
 namespace exl3 {
 
+// A column's weights are taken against a reference that starts this far (log2)
+// below its maximum, and follows it when it has grown by kAttSlack more: the
+// largest weight is 2^7 to 2^15, so that f16 holds weights down to 2^-21 of it in
+// full and down to 2^-32 at all.  (Against the maximum itself those ends are
+// 2^-14 and 2^-25: behind one key that takes all the weight, a long tail 17 nats
+// below it came out 41 % too large, or as nothing.)  The sums l, fp32, are
+// taken against the same reference.
+constexpr float kAttLift = 7.f, kAttSlack = 8.f;
+
 struct KvAttendArgs {
     const uint16_t* q;
     int64_t q_tok, q_head, q_rows;

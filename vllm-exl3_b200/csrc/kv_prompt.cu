@@ -41,9 +41,9 @@
 // Registers decide much: a converter or an issuing warp that spills costs up to 40 %.
 //
 // O is rescaled only when a row's maximum grows by more than 2^8 over the
-// reference its weights are taken against: until then weights up to 2^8 (f16
-// holds them, the sums are fp32) cost nothing, and the final division is by a
-// sum over the same reference.
+// place that its weights' reference was set for (kAttLift, kAttSlack): until then
+// larger weights (f16 holds them, the sums are fp32) cost nothing, and the
+// final division is by a sum over the same reference.
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -59,7 +59,6 @@ constexpr int kPrThreads = 16 * 32;
 constexpr int kPrKeys = 128;        // keys per step
 constexpr int kPrRows = 256;        // query rows per CTA
 constexpr int kPrSlots = 8;         // steps whose pages and scales are kept
-constexpr float kPrSlack = 8.f;     // log2: growth of the maximum that is let pass
 constexpr uint32_t kPrTmem = 512;
 // Steps that an item's queries and results are worth on the line.  us with 0 / 3 / 6 / 10:
 //   whole prompts of 2043 to 4086 tokens (16 heads over 4, dim 128, int8) 478 / 280 / 286 / 300, one of 4086 228 / 117 / 122 / 129
@@ -524,8 +523,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv_prompt_kernel(const KvAttend
                         mx = max3(mx, fmaf(top, factor(s4.x), s4.y), -INFINITY);
                     }
                 }
-                if (__any_sync(0xffffffffu, mx > ref + kPrSlack)) {  // -inf + slack is -inf: the first key that is seen counts as growth
-                    const float nref = fmaxf(ref, mx);  // of a NaN row: any
+                if (__any_sync(0xffffffffu, mx > ref + (kAttLift + kAttSlack))) {  // -inf + slack is -inf: the first key that is seen counts as growth
+                    const float nref = fmaxf(ref, mx - kAttLift);  // of a NaN row: any
                     const float alpha = ref == nref ? 1.f : ex2(ref - nref);  // 0 where nothing has been seen
                     l *= alpha;
                     ref = nref;
