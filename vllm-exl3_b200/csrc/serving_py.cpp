@@ -62,6 +62,14 @@ int64_t whole(PyObject* o) {
     return v;
 }
 
+struct PyFailed {};
+
+bool truth(PyObject* o) {  // as Python's `if`
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw PyFailed();
+    return v != 0;
+}
+
 c10::Device current(const at::Tensor& t) {
     const c10::Device dev = t.device();
     want(dev.is_cuda() && dev.index() == c10::cuda::current_device());
@@ -72,7 +80,6 @@ struct Space {
     void* at;
     int64_t bytes;
 };
-struct PyFailed {};
 
 Space workspace(const c10::Device& dev, cudaStream_t stream, size_t need) {
     PyObject* r = PyObject_CallFunction(workspace_of, "iLnK", int(dev.index()), (long long)(intptr_t)stream, Py_ssize_t(need),
@@ -206,7 +213,7 @@ PyObject* attend_(PyObject* const* a) {
     const Space ws = workspace(m.dev, stream, entry.attend_bytes(int(heads), int(m.heads), int(m.dim), int(max_new), int(B), rows));
     const at::Tensor out = at::empty(q.sizes(), q.options());
     at::Tensor lse;
-    if (a[11] == Py_True) {
+    if (truth(a[11])) {
         lse = at::empty({rows, heads}, q.options().dtype(at::kFloat));
         c.lse = data<float>(lse);
     }
