@@ -13,6 +13,7 @@ import importlib.util
 import os
 import struct
 import threading
+import warnings
 
 import torch
 
@@ -142,9 +143,10 @@ _binding = None
 
 
 def binding():
-    """The compiled short way into the serving entries (``_serving_py.so``).
+    """The compiled short way into the serving entries (``_serving_py.*.so``).
     Its functions return None where a call needs the checks or copies of the
-    Python function, which is complete without them."""
+    Python function, which is complete without them.  Where it cannot be built
+    or loaded, whatever the reason, a warning says so once."""
     global _binding
     if _binding is None:
         lib = load()
@@ -157,7 +159,9 @@ def binding():
                      "token_logprobs_workspace_size", "capture_id")
             mod.setup(*(ctypes.cast(getattr(lib, "exl3_" + n), P).value for n in names), serve_workspace, check)
             _binding = mod
-        except (OSError, RuntimeError, ImportError):
+        except Exception as e:
+            warnings.warn(f"exl3_b200: no compiled way into the serving operators, their calls take some 10 us more on "
+                          f"the host ({type(e).__name__}: {e})", RuntimeWarning, stacklevel=2)
             _binding = _NoBinding
     return _binding
 
