@@ -86,3 +86,37 @@ def test_a_flag_that_cannot_be_asked_raises(native, cuda, way):
     table, lens = torch.zeros(2, 1, dtype=torch.int32, device=cuda), torch.tensor([3, 9], dtype=torch.int32, device=cuda)
     with pytest.raises(KeyError, match="odd"):
         kv_attend(torch.ones(2, 4, 64, device=cuda).half(), kc, kc, s, s, table, lens, return_lse=Odd())
+
+
+def test_a_backward_pass_raises(native, cuda, way):
+    """No gradient is left out in silence: results of inputs that want one raise when it is asked for."""
+    import torch
+    from exl3_b200.kv_cache import kv_attend
+    from exl3_b200.logprobs import token_logprobs
+    kc, s = torch.ones(3, 1, 16, 64, dtype=torch.int8, device=cuda), torch.ones(3, 1, device=cuda)
+    table, lens = torch.zeros(2, 1, dtype=torch.int32, device=cuda), torch.tensor([3, 9], dtype=torch.int32, device=cuda)
+    q = torch.ones(2, 4, 64, device=cuda).half()
+    x, tok = torch.randn(2, 500, device=cuda), torch.tensor([1, 2], device=cuda)
+    plain = [kv_attend(q, kc, kc, s, s, table, lens), *kv_attend(q, kc, kc, s, s, table, lens, return_lse=True)]
+    plain += [*token_logprobs(x, tok, top=3), *token_logprobs(x, tok)]
+    assert not any(t.requires_grad for t in plain)
+    q.requires_grad_()
+    x.requires_grad_()
+
+    def again():
+        got = [kv_attend(q, kc, kc, s, s, table, lens), *kv_attend(q, kc, kc, s, s, table, lens, return_lse=True)]
+        return got + [*token_logprobs(x, tok, top=3), *token_logprobs(x, tok)]
+
+    got = again()
+    assert all(torch.equal(a, b) for a, b in zip(plain, got))
+    for t in got:
+        if t.is_floating_point() and t.numel():
+            assert t.requires_grad
+            with pytest.raises(RuntimeError, match="inference"):
+                t.float().sum().backward()
+        else:
+            assert not t.requires_grad or not t.numel()
+    with torch.no_grad():
+        assert not any(t.requires_grad for t in again())
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(plain, again()))

@@ -13,6 +13,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/core/grad_mode.h>
 #include <cmath>
 #include <exception>
 
@@ -61,6 +62,9 @@ int64_t whole(PyObject* o) {
     }
     return v;
 }
+
+// autograd wants to know of it
+bool recorded(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
 struct PyFailed {};
 
@@ -191,6 +195,7 @@ PyObject* attend_(PyObject* const* a) {
     const int64_t max_new = whole(a[8]), window = whole(a[10]);
     const Cache m = cache(kc, vc, ks, vs);
     const int64_t B = lens.numel();
+    want(!recorded(q));
     want(rows_ready(q) && q.device() == m.dev && q.size(2) == m.dim && q.size(1) > 0 && q.size(1) % m.heads == 0 &&
          plain_i32(table, 2, m.dev) && plain_i32(lens, 1, m.dev) && table.size(0) == B && max_new >= 1 &&
          max_new <= INT32_MAX && window >= 0);
@@ -235,6 +240,7 @@ PyObject* logprobs_(PyObject* const* a) {
     const at::Tensor &x = tensor(a[0]), &tok = tensor(a[1]);
     const int64_t top = whole(a[2]);
     const c10::Device dev = current(x);
+    want(!recorded(x));
     exl3_token_logprobs_args c{};
     const auto kind = x.scalar_type();
     want(kind == at::kFloat || kind == at::kHalf || kind == at::kBFloat16);

@@ -202,6 +202,25 @@ def require_cuda(*tensors: torch.Tensor | None, who: str) -> None:
             raise RuntimeError(f"{who} requires CUDA tensors (the B200 path has no CPU fallback)")
 
 
+class _NoBackward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, who, result, source):
+        ctx.who = who
+        return result.view_as(result)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.who} is for inference: it has no backward pass")
+
+
+def inference_only(who: str, result: torch.Tensor, source: torch.Tensor) -> torch.Tensor:
+    """``result``; where autograd records and ``source`` wants a gradient, in a
+    form whose backward pass raises instead of leaving the gradient out."""
+    if torch.is_grad_enabled() and source.requires_grad:
+        return _NoBackward.apply(who, result, source)
+    return result
+
+
 def profile_enable(on: bool, delay_cycles: int = 0) -> None:
     check(load().exl3_profile_enable(int(bool(on)), int(delay_cycles)))
 

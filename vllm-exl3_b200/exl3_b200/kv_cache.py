@@ -198,7 +198,8 @@ def kv_attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
     already appended.  ``max_new`` is the most rows of a request.  ``heads`` is
     a multiple of the cache's kv heads.  ``window`` limits a row to the last
     ``window`` keys, its own included (0: no limit); ``scale`` defaults to
-    dim ** -0.5.  Rows that see no key are zeros (lse -inf).
+    dim ** -0.5.  Rows that see no key are zeros (lse -inf).  For inference: a
+    backward pass through the result raises.
     """
     short = _n.binding().kv_attend(q, k_cache, v_cache, k_scale, v_scale, block_table, kv_lens, cu_tokens, max_new,
                                    scale, window, return_lse)
@@ -246,7 +247,8 @@ def kv_attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
         ws, ws_bytes), stream)
     if rc:
         _n.check(rc, "kv_attend")
-    return (out, lse) if return_lse else out
+    out = _n.inference_only("kv_attend", out, q)
+    return (out, _n.inference_only("kv_attend", lse, q)) if return_lse else out
 
 
 class Exl3KvCache:

@@ -33,7 +33,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     """log softmax of ``logits`` (fp32, fp16 or bf16 [rows, vocab]) at
     ``tokens`` (int32 or int64 [rows]) in one pass over the logits, computed in
     fp32.  Equal logits rank lowest index first.  Tokens outside the vocabulary
-    (padding) get logprob -inf and rank 0.  ``top``: 0 to 32 alternatives."""
+    (padding) get logprob -inf and rank 0.  ``top``: 0 to 32 alternatives.  For
+    inference: a backward pass through the result raises."""
     short = _n.binding().token_logprobs(logits, tokens, top)
     if short is not None:
         return TokenLogprobs(*short)
@@ -58,6 +59,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
         row_stride = vocab
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
+
+    def result(t):
+        return _n.inference_only("token_logprobs", t, logits)
+
     # one buffer: logprob and entropy, the alternatives' values; rank, their ids
     buf = logits.new_empty(rows * (2 + top), dtype=torch.float32)
     whole = logits.new_empty(rows * (1 + top), dtype=torch.int32)
@@ -72,10 +77,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
             _n.check(rc, "token_logprobs")
     if top == 0:
         lp, ent = torch.unsafe_split_with_sizes(buf, (rows, rows))
-        return TokenLogprobs(lp, ent, whole, buf.new_empty((rows, 0)), whole.new_empty((rows, 0)))
+        return TokenLogprobs(result(lp), result(ent), whole, buf.new_empty((rows, 0)), whole.new_empty((rows, 0)))
     lp, ent, vals = torch.unsafe_split_with_sizes(buf, (rows, rows, rows * top))
     rank, best = torch.unsafe_split_with_sizes(whole, (rows, rows * top))
-    return TokenLogprobs(lp, ent, rank, vals.view(rows, top), best.view(rows, top))
+    return TokenLogprobs(result(lp), result(ent), rank, result(vals.view(rows, top)), best.view(rows, top))
 
 
 __all__ = ["MAX_TOP", "TokenLogprobs", "token_logprobs"]
