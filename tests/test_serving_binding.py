@@ -57,3 +57,30 @@ def test_without_it_the_operators_stand_and_say_so(monkeypatch, why):
         assert _native.binding() is _native._NoBinding
     with pytest.raises(RuntimeError, match="CUDA"):
         logprobs.token_logprobs(torch.zeros(1, 4), torch.zeros(1, dtype=torch.int64))
+
+
+def test_tensors_of_several_gpus_are_refused():
+    """Each tensor in turn on another GPU than the others: refused by name, before any address is taken."""
+    import torch
+    from exl3_b200 import kv_cache, logprobs
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+    mode = FakeTensorMode()
+
+    def on(gpu, *shape, dtype):
+        return FakeTensor(mode, torch.empty(shape, dtype=dtype, device="meta"), torch.device("cuda", gpu))
+
+    i32, i64, f16, f32, i8 = torch.int32, torch.int64, torch.float16, torch.float32, torch.int8
+    code, scale = ((3, 2, 16, 64), i8), ((3, 2), f32)
+    calls = [
+        (lambda t: kv_cache.kv_plan(*t, page_size=16, n_tokens=4),
+         [((2,), i32), ((2,), i32), ((2, 3), i32), ((9,), i32), ((1,), i32)]),
+        (lambda t: kv_cache.kv_append(*t), [((4, 2, 64), f16), ((4, 2, 64), f16), ((4,), i64), code, code, scale, scale]),
+        (lambda t: kv_cache.kv_attend(*t[:-1], cu_tokens=t[-1], max_new=2),
+         [((4, 4, 64), f16), code, code, scale, scale, ((2, 3), i32), ((2,), i32), ((3,), i32)]),
+        (lambda t: logprobs.token_logprobs(*t), [((2, 50), f32), ((2,), i64)]),
+    ]
+    for call, shapes in calls:
+        for other in range(len(shapes)):
+            tensors = [on(int(i == other), *s, dtype=d) for i, (s, d) in enumerate(shapes)]
+            with pytest.raises(ValueError, match="different GPUs"):
+                call(tensors)

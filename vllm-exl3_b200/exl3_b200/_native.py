@@ -202,6 +202,14 @@ def require_cuda(*tensors: torch.Tensor | None, who: str) -> None:
             raise RuntimeError(f"{who} requires CUDA tensors (the B200 path has no CPU fallback)")
 
 
+def require_one_device(*tensors: torch.Tensor | None, who: str) -> None:
+    """A kernel that is given another GPU's memory faults: every tensor must be on the first one's GPU."""
+    require_cuda(*tensors, who=who)
+    where = [t.device for t in tensors if t is not None]
+    if any(d != where[0] for d in where):
+        raise ValueError(f"{who}: tensors on different GPUs ({', '.join(sorted({str(d) for d in where}))})")
+
+
 class _NoBackward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, who, result, source):

@@ -68,12 +68,11 @@ def kv_plan(lens: torch.Tensor, new_tokens: torch.Tensor, block_table: torch.Ten
     if short is not None:
         return KvPlan(*short)
     B = lens.numel()
-    if not (lens.is_cuda and new_tokens.is_cuda and block_table.is_cuda and free_pages.is_cuda and cursor.is_cuda
-            and _is_i32(lens) and _is_i32(new_tokens) and _is_i32(free_pages) and _is_i32(cursor)
+    who = "kv_plan"
+    _n.require_one_device(lens, new_tokens, block_table, free_pages, cursor, who=who)
+    if not (_is_i32(lens) and _is_i32(new_tokens) and _is_i32(free_pages) and _is_i32(cursor)
             and _is_i32(block_table, 2) and new_tokens.numel() == B and block_table.size(0) == B
             and cursor.numel() == 1 and page_size in PAGES and n_tokens >= 0):
-        who = "kv_plan"
-        _n.require_cuda(lens, new_tokens, block_table, free_pages, cursor, who=who)
         named = (("lens", lens), ("new_tokens", new_tokens), ("free_pages", free_pages), ("cursor", cursor))
         _explain(who, *((not _is_i32(t), f"{n} must be a contiguous int32 tensor of one dimension") for n, t in named),
                  (not _is_i32(block_table, 2), "block_table must be a contiguous int32 tensor of two dimensions"),
@@ -102,7 +101,6 @@ def kv_plan(lens: torch.Tensor, new_tokens: torch.Tensor, block_table: torch.Ten
 
 def _bad_cache(who: str, k_cache, v_cache, k_scale, v_scale) -> None:
     """Raises what is wrong with a cache, if anything."""
-    _n.require_cuda(k_cache, v_cache, k_scale, v_scale, who=who)
     shape = k_cache.shape
     four = len(shape) == 4 and v_cache.shape == shape and k_cache.is_contiguous() and v_cache.is_contiguous()
     wrong = [(k_cache.dtype not in _CODES or v_cache.dtype != k_cache.dtype,
@@ -120,8 +118,7 @@ def _bad_cache(who: str, k_cache, v_cache, k_scale, v_scale) -> None:
 
 def _cache_ok(k_cache, v_cache, k_scale, v_scale) -> bool:
     shape = k_cache.shape
-    return (k_cache.is_cuda and v_cache.is_cuda and k_scale.is_cuda and v_scale.is_cuda and k_cache.dtype in _CODES
-            and v_cache.dtype is k_cache.dtype and len(shape) == 4 and v_cache.shape == shape
+    return (k_cache.dtype in _CODES and v_cache.dtype is k_cache.dtype and len(shape) == 4 and v_cache.shape == shape
             and k_cache.is_contiguous() and v_cache.is_contiguous() and shape[2] in PAGES and shape[3] in DIMS
             and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
             and k_scale.shape == shape[:2] and v_scale.shape == shape[:2]
@@ -154,12 +151,12 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: to
         return
     n = slots.numel()
     x = _ROWS.get(k.dtype)
-    if not (_cache_ok(k_cache, v_cache, k_scale, v_scale) and k.is_cuda and v.is_cuda and slots.is_cuda
-            and x is not None and v.dtype is k.dtype and slots.dtype is torch.int64 and slots.is_contiguous()
-            and k.dim() == 3 and k.size(0) == n and k.shape[1:] == k_cache.shape[1::2] and v.shape == k.shape):
-        who = "kv_append"
+    who = "kv_append"
+    _n.require_one_device(k_cache, v_cache, k_scale, v_scale, k, v, slots, who=who)
+    if not (_cache_ok(k_cache, v_cache, k_scale, v_scale) and x is not None and v.dtype is k.dtype
+            and slots.dtype is torch.int64 and slots.is_contiguous() and k.dim() == 3 and k.size(0) == n
+            and k.shape[1:] == k_cache.shape[1::2] and v.shape == k.shape):
         _bad_cache(who, k_cache, v_cache, k_scale, v_scale)
-        _n.require_cuda(k, v, slots, who=who)
         _, heads, _, dim = k_cache.shape
         _explain(who, (x is None or v.dtype != k.dtype, "k and v must both be fp16 or both bf16"),
                  (slots.dtype != torch.int64 or not slots.is_contiguous(), "slots must be contiguous int64"),
@@ -207,15 +204,14 @@ def kv_attend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_s
         return short
     x = _ROWS.get(q.dtype)
     B = kv_lens.numel()
-    if not (_cache_ok(k_cache, v_cache, k_scale, v_scale) and q.is_cuda and block_table.is_cuda and kv_lens.is_cuda
-            and x is not None and q.dim() == 3 and q.size(2) == k_cache.size(3) and q.size(1)
-            and not q.size(1) % k_cache.size(1) and _is_i32(block_table, 2) and _is_i32(kv_lens)
-            and block_table.size(0) == B and max_new >= 1 and window >= 0
+    who = "kv_attend"
+    _n.require_one_device(k_cache, v_cache, k_scale, v_scale, q, block_table, kv_lens, cu_tokens, who=who)
+    if not (_cache_ok(k_cache, v_cache, k_scale, v_scale) and x is not None and q.dim() == 3
+            and q.size(2) == k_cache.size(3) and q.size(1) and not q.size(1) % k_cache.size(1)
+            and _is_i32(block_table, 2) and _is_i32(kv_lens) and block_table.size(0) == B and max_new >= 1 and window >= 0
             and ((q.size(0) == B and max_new == 1) if cu_tokens is None
-                 else cu_tokens.is_cuda and _is_i32(cu_tokens) and cu_tokens.numel() == B + 1)):
-        who = "kv_attend"
+                 else _is_i32(cu_tokens) and cu_tokens.numel() == B + 1)):
         _bad_cache(who, k_cache, v_cache, k_scale, v_scale)
-        _n.require_cuda(q, block_table, kv_lens, cu_tokens, who=who)
         _, kv_heads, _, dim = k_cache.shape
         _explain(who, (x is None or q.dim() != 3 or q.size(-1) != dim, f"q must be fp16 or bf16 [rows, heads, {dim}]"),
                  (q.dim() == 3 and (q.size(1) == 0 or q.size(1) % kv_heads != 0),

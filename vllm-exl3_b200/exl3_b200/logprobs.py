@@ -39,10 +39,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     if short is not None:
         return TokenLogprobs(*short)
     x, ids = _LOGITS.get(logits.dtype), _IDS.get(tokens.dtype)
-    if not (logits.is_cuda and tokens.is_cuda and x is not None and ids is not None and logits.dim() == 2
-            and tokens.shape == logits.shape[:1] and 0 <= top <= MAX_TOP and top <= logits.size(1)):
-        who = "token_logprobs"
-        _n.require_cuda(logits, tokens, who=who)
+    who = "token_logprobs"
+    _n.require_one_device(logits, tokens, who=who)
+    if not (x is not None and ids is not None and logits.dim() == 2 and tokens.shape == logits.shape[:1]
+            and 0 <= top <= MAX_TOP and top <= logits.size(1)):
         if x is None or logits.dim() != 2:
             raise ValueError(f"{who}: logits must be fp32, fp16 or bf16 [rows, vocab]")
         if ids is None or tokens.shape != logits.shape[:1]:
