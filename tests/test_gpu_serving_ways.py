@@ -120,3 +120,18 @@ def test_a_backward_pass_raises(native, cuda, way):
         assert not any(t.requires_grad for t in again())
     with torch.inference_mode():
         assert all(torch.equal(a, b) for a, b in zip(plain, again()))
+
+
+def test_a_cache_without_heads_or_pages_is_refused(native, cuda, way):
+    import torch
+    from exl3_b200.kv_cache import kv_append, kv_attend
+    table, lens = torch.zeros(2, 1, dtype=torch.int32, device=cuda), torch.tensor([3, 9], dtype=torch.int32, device=cuda)
+    for shape, exc in (((3, 0, 16, 64), ValueError), ((0, 2, 16, 64), RuntimeError)):
+        kc, s = torch.ones(shape, dtype=torch.int8, device=cuda), torch.ones(shape[:2], device=cuda)
+        for heads in (0, 4):
+            q = torch.ones(2, heads, 64, device=cuda).half()
+            with pytest.raises(ValueError if heads == 0 else exc):
+                kv_attend(q, kc, kc, s, s, table, lens)
+        k = torch.ones(2, shape[1], 64, device=cuda).half()
+        with pytest.raises(exc):
+            kv_append(k, k, torch.tensor([0, 1], device=cuda), kc, kc, s, s)

@@ -116,7 +116,7 @@ Cache cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, cons
     const c10::Device dev = current(k);
     const bool e4m3 = k.scalar_type() == at::kFloat8_e4m3fn;
     want((e4m3 || k.scalar_type() == at::kChar) && v.scalar_type() == k.scalar_type() && k.dim() == 4 &&
-         v.sizes() == k.sizes() && k.is_contiguous() && v.is_contiguous() && v.device() == dev);
+         v.sizes() == k.sizes() && k.size(1) > 0 && k.is_contiguous() && v.is_contiguous() && v.device() == dev);
     for (const at::Tensor* s : {&ks, &vs})
         want(s->scalar_type() == at::kFloat && s->dim() == 2 && s->size(0) == k.size(0) && s->size(1) == k.size(1) &&
              s->is_contiguous() && s->device() == dev);

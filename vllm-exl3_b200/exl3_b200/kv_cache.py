@@ -105,7 +105,7 @@ def _bad_cache(who: str, k_cache, v_cache, k_scale, v_scale) -> None:
     four = len(shape) == 4 and v_cache.shape == shape and k_cache.is_contiguous() and v_cache.is_contiguous()
     wrong = [(k_cache.dtype not in _CODES or v_cache.dtype != k_cache.dtype,
               "the caches must both be float8_e4m3fn or both int8"),
-             (not four, "the caches must be contiguous [pages, kv_heads, page, dim] of one shape")]
+             (not four or shape[1] == 0, "the caches must be contiguous [pages, kv_heads, page, dim] of one shape")]
     if four:
         wrong += [(shape[2] not in PAGES or shape[3] not in DIMS,
                    f"page must be one of {PAGES} and dim one of {DIMS} (got {shape[2]}, {shape[3]})")]
@@ -119,8 +119,8 @@ def _bad_cache(who: str, k_cache, v_cache, k_scale, v_scale) -> None:
 def _cache_ok(k_cache, v_cache, k_scale, v_scale) -> bool:
     shape = k_cache.shape
     return (k_cache.dtype in _CODES and v_cache.dtype is k_cache.dtype and len(shape) == 4 and v_cache.shape == shape
-            and k_cache.is_contiguous() and v_cache.is_contiguous() and shape[2] in PAGES and shape[3] in DIMS
-            and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
+            and shape[1] > 0 and shape[2] in PAGES and shape[3] in DIMS and k_cache.is_contiguous()
+            and v_cache.is_contiguous() and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
             and k_scale.shape == shape[:2] and v_scale.shape == shape[:2]
             and k_scale.is_contiguous() and v_scale.is_contiguous())
 
