@@ -351,7 +351,8 @@ int exl3_kv_append(const exl3_kv_append_args* args, void* stream);
 /* Workspace of this entry and of exl3_token_logprobs: 256-byte aligned, all
  * zero before its first use (zeroed on the device, not by a fill that a
  * capture records); it starts with the status word, and may serve both, for
- * calls that follow one another on a stream, or in one graph. */
+ * calls that follow one another on a stream, or in one graph.  After status
+ * 4 (a wait ran out) it has to be zeroed again. */
 size_t exl3_kv_attend_workspace_size(int heads, int kv_heads, int dim, int max_new, int requests, int64_t q_rows);
 typedef struct exl3_kv_attend_args {
     const void* q;

@@ -204,3 +204,30 @@ def test_a_call_that_does_not_fit_grows_within_a_capture(native, cuda):
         torch.cuda.synchronize()
         for o, c in zip(outs, (lp, few, many, few, lp)):
             assert _same(o, c())
+
+
+def test_counters_are_renewed_after_a_wait_ran_out(native, cuda):
+    """Items given up leave their counters; clearing the status makes the workspace fit again, captured ones too.
+    The state is written by hand."""
+    import torch
+    from exl3_b200 import _native
+    calls = [c for kind in _calls(cuda) for c in kind]
+    want = [c() for c in calls]
+    graphs, outs = [], []
+    for c in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(c())
+    torch.cuda.synchronize()
+    assert native.device_status(clear=True) == 0
+    for buf in _native._serve_buffers:
+        buf[:4].view(torch.int32).fill_(4)
+        buf[256:2048].view(torch.int32).fill_(1)  # as after a piece that was counted and one that was not
+    assert native.device_status(clear=False) == 4 and native.device_status(clear=True) == 4
+    assert native.device_status(clear=True) == 0
+    for g, o, c, w in zip(graphs, outs, calls, want):
+        _clear(o)
+        g.replay()
+        assert _same(c(), w)
+        torch.cuda.synchronize()
+        assert _same(o, w)

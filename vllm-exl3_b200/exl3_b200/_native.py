@@ -279,6 +279,7 @@ def workspace(device: torch.device, nbytes: int, stream: torch.cuda.Stream | Non
 
 
 _serve_ws: dict[tuple[int, int], tuple[int, int]] = {}
+_serve_buffers: list[torch.Tensor] = []  # every serving workspace, current and retained
 
 
 def serve_workspace(index: int, stream: int, nbytes: int = 0, capture: int | None = None) -> tuple[int, int]:
@@ -302,6 +303,7 @@ def serve_workspace(index: int, stream: int, nbytes: int = 0, capture: int | Non
             _ws_retired.append(old)
         buf = torch.zeros(size, dtype=torch.uint8, device=torch.device("cuda", index))
         _ws_cache[key] = buf
+        _serve_buffers.append(buf)
         have = _serve_ws[(index, stream)] = (buf.data_ptr(), size)
     return have
 
@@ -344,7 +346,8 @@ def _captured_workspace(index: int, stream: int, capture: int, nbytes: int) -> t
                     raise RuntimeError("no stream outside the capture to set up a workspace on")
                 with torch.cuda.stream(side):
                     if buf is None:
-                        buf = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=torch.device("cuda", index))
+                        buf = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=f"cuda:{index}")
+                        _serve_buffers.append(buf)
                     else:
                         buf[256:].zero_()  # a status that was recorded in it stays
                 side.synchronize()
@@ -366,3 +369,14 @@ def device_workspaces(device: torch.device) -> list[torch.Tensor]:
     out = [b for k, b in _ws_cache.items() if k[0] == device.type and k[1] == device.index]
     kept = _ws_retired + [held[2] for held in _captured_held] + _captured_spare
     return out + [b for b in kept if b.device == device]
+
+
+DEV_WAIT_TIMEOUT = 4
+
+
+def renew_serve_workspace(workspace: torch.Tensor) -> None:
+    """Zeroes the counters of a serving workspace in which a wait ran out (on
+    the current stream, with none of its calls in flight): items that were
+    given up have left theirs behind, and the next call starts from zero."""
+    if any(b.data_ptr() == workspace.data_ptr() for b in _serve_buffers):
+        workspace[256:].zero_()

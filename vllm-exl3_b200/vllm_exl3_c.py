@@ -482,7 +482,8 @@ def ngram_dequant(packed, bits, heads, head_bias, out):
 def device_status(workspace=None, clear=True) -> int:
     """Device-side status word of a workspace (0 = clean).  Without one: the
     first nonzero word among every workspace of the current device (all
-    streams; synchronises the device first)."""
+    streams; synchronises the device first).  Clearing status 4 (a wait ran
+    out) also makes the workspace fit for the next call."""
     import ctypes
 
     lib = _n.load()
@@ -496,6 +497,8 @@ def device_status(workspace=None, clear=True) -> int:
     for ws in spaces:
         v = ctypes.c_int(0)
         _n.check(lib.exl3_device_status(ws.data_ptr(), int(bool(clear)), _n.stream_of(ws), ctypes.byref(v)))
+        if clear and v.value == _n.DEV_WAIT_TIMEOUT:
+            _n.renew_serve_workspace(ws)
         if v.value and not first:
             first = int(v.value)
     return first
