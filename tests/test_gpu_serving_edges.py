@@ -230,3 +230,35 @@ def test_plan_sums_beyond_32_bits(native, cuda):
         slots = p.slots.tolist()
         assert all(s == -1 or 0 <= s < 24 * 16 or 100 * 16 <= s < 140 * 16 for s in slots)
         assert int(p.cursor) == (40 if max(new) == big else 1)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(64, 1), (128, 1), (98, 2), (600, 1)])
+def test_attend_many_heads_per_kv_head(native, cuda, heads, kv_heads):
+    """More query columns from one token than the few-row kernel takes, up to several tiles of the prompt kernel."""
+    for lens, new in (([1, 40, 333], [1, 1, 1]), ([70, 300], [2, 3])):
+        p = _attend_problem(cuda, lens, new, heads=heads, kv_heads=kv_heads)
+        _near(_kv().kv_attend(**p), _plain(p))
+
+
+def test_attend_many_requests(native, cuda):
+    """More requests than the kernels have threads, empty ones among them, prompts between single tokens."""
+    lens = [(7 * i) % 90 for i in range(1300)]
+    new = [min(n, 1) for n in lens]
+    p = _attend_problem(cuda, lens, new)
+    _near(_kv().kv_attend(**p), _plain(p))
+    for b in (3, 600, 601, 1299):
+        new[b] = lens[b]
+    p = _attend_problem(cuda, lens, new, seed=1)
+    _near(_kv().kv_attend(**p), _plain(p))
+
+
+def test_attend_more_rows_than_tokens(native, cuda):
+    """Rows at positions before the first token see nothing; a max_new below or above the rows only selects kernels."""
+    for lens, new in (([3, 0, 20], [5, 2, 20]), ([30, 64, 1], [90, 70, 60])):
+        p = _attend_problem(cuda, lens, new)
+        want = _plain(p)
+        for most in (max(new), 1, 5000):
+            out, lse = _kv().kv_attend(**{**p, "max_new": most})
+            _near((out, lse), want)
+            empty = np.isinf(want[1])
+            assert empty.any() and not out.cpu().numpy()[empty].any()
