@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
         const int b = tid * per + i;
         if (b < a.requests) {
             own = att_request<NC>(a, b);
+            if (blockIdx.x == 0) att_check(a, b);  // of every request, the prompt kernel's too
             mine += int64_t(own.groups) * Hk * own.units;
             items += int64_t(own.groups) * Hk;
         }
@@ -205,6 +206,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
         while (u >= base + int64_t(rq.groups) * Hk * (rq.units + cost)) {  // next request with work
             base += int64_t(rq.groups) * Hk * (rq.units + cost);
             rq = att_request<NC>(a, ++b);
+            if (tid == 0) found = rq;
         }
         const int64_t item = (u - base) / (rq.units + cost), u_item = base + item * (rq.units + cost) + cost;  // its first unit
         const int off = int(max(u - u_item, int64_t(0)));
@@ -456,6 +458,7 @@ __global__ void __launch_bounds__(kAttThreads, (AttShape<D, NT>::kCtas)) kv_atte
         }
         copy_wait<0>();
         __syncthreads();  // the ring is free
+        rq = found;       // its registers were the loop's
 
         // --- join the warps ---
         #pragma unroll

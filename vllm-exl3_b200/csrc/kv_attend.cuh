@@ -38,25 +38,26 @@ struct KvAttendArgs {
 
 // A request's rows of q: its positions count from all `fresh` that cu_tokens
 // names, `rows` of them are computed.  They are fewer where cu_tokens leaves
-// the tensor, which is recorded, so that no offset here leaves it.
+// the tensor, so that no offset here leaves it.
 struct AttRows {
-    int64_t row0;
-    int fresh, rows;
+    int row0, fresh, rows;
 };
 __device__ __forceinline__ AttRows att_rows(const KvAttendArgs& a, int b) {
     if (!a.cu) return AttRows{b, 1, 1};
-    const int64_t row0 = a.cu[b], n = max(a.cu[b + 1] - row0, int64_t(0));
-    const int rows = row0 < 0 ? 0 : int(max(min(n, a.q_rows - row0), int64_t(0)));
-    if (rows < n) set_status(a.status, DEV_BAD_INDEX);
-    return AttRows{row0, int(min(n, int64_t(INT32_MAX))), rows};
+    const int row0 = a.cu[b], end = a.cu[b + 1];
+    const int n = row0 >= 0 && end > row0 ? end - row0 : 0;
+    return AttRows{row0, n, min(n, max(int(a.q_rows) - row0, 0))};
 }
 
-// Tokens of request b that the block table has a place for.  The others are
+// Tokens of a request that the block table has a place for.  The others are
 // not seen; they count for the rows' positions all the same.
-__device__ __forceinline__ int att_keys(const KvAttendArgs& a, int len) {
-    const int64_t room = int64_t(a.width) << a.shift;
-    if (len > room) set_status(a.status, DEV_BAD_INDEX);
-    return int(min(int64_t(len), room));
+__device__ __forceinline__ int att_keys(const KvAttendArgs& a, int len) { return min(len, a.width << a.shift); }
+
+// Records a request whose rows leave q or whose tokens leave the table
+__device__ __forceinline__ void att_check(const KvAttendArgs& a, int b) {
+    const AttRows w = att_rows(a, b);
+    const bool before = a.cu && a.cu[b] < 0 && a.cu[b + 1] > a.cu[b];
+    if (before || w.rows < w.fresh || a.kv_lens[b] > a.width << a.shift) set_status(a.status, DEV_BAD_INDEX);
 }
 
 // two codes (bytes 0, 1 of w; int8 already offset by 128) as f16x2, exact
