@@ -29,13 +29,15 @@
 // maximum only when that has grown by more than 2^8 (kAttSlack), so that the usual
 // tile needs no exchange between lanes and no rescaling.
 //
-// Measured: 64 single tokens over up to 8192 keys (32 heads over 4, dim 128,
-// e4m3, 343 MB) 70 us, 4.9 TB/s, 75 % of the measured copy rate; 4 requests of
-// 3 tokens over up to 128K keys (64 heads over 8, int8, 24 columns) 218 us, 57 %
-// (the int8 conversions and three column tiles leave two warps per scheduler
-// at their issue latency); one token over 1021 keys 10.4 us, a chain of
-// dependent steps.  A piece of an item costs about 13K cycles beside its tiles
-// (queries in, warps joined, partials out), a third of a CTA's time at the 64.
+// Measured (lone calls): 64 single tokens over up to 8192 keys (32 heads over 4,
+// dim 128, e4m3, 343 MB) 69 us, 4.95 TB/s, 76 % of the measured copy rate; 4
+// requests of 3 tokens over up to 128K keys (64 heads over 8, int8, 24 columns)
+// 212 us, 59 % (the int8 conversions and three column tiles leave two warps per
+// scheduler at their issue latency); one token over 1021 keys 11.2 us, 9.9 in a
+// graph, a chain of dependent steps.  A piece of an item costs about 13K cycles
+// beside its tiles (queries in, warps joined, partials out), a third of a CTA's
+// time at the 64.  The request's numbers stay in shared memory over the loop:
+// in registers they took 71, 220 and 12.3 us.
 // Not kept, us at the 64 and the 128K: joining at a CTA's end 77 / 250, joining
 // the warps as a tree 76 / 233, separate loops for tiles with and without masks 74 / 217
 // (each against 71 / 218 then).

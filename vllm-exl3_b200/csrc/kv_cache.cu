@@ -22,13 +22,14 @@
 // alone (no barrier), longer ones the CTA's.  Bound: HBM, 2 bytes read and 1
 // written per value.
 //
-// Measured (launches in a graph): the plan of 64 requests, a token each, 3.7 us,
-// of 512 with 23318 tokens 5.5 us: one launch and its chain of reads (lengths,
+// Measured (launches in a graph): the plan of 64 requests, a token each, 3.6 us,
+// of 512 with 23318 tokens 5.3 us: one launch and its chain of reads (lengths,
 // scan, bisection, table), the bytes are nothing.  64 tokens of 4 heads, dim
-// 128, into pages of 16: 5.4 us, the same kind of chain (slot, run, rows and
-// page, scale, codes).  8190 tokens of 8 heads, pages of 64: 13.6 us with rows
-// in L2 (3.7 TB/s), 18.5 from HBM as a lone call; a CTA's loads, reduction and
-// stores follow one another, and two or three CTAs per SM hide that in part.
+// 128, into pages of 16: 5.5 us, the same kind of chain (slot, run, rows and
+// page, scale, codes).  8190 tokens of 8 heads, pages of 64: 13.5 us with rows
+// in L2 (3.7 TB/s), 18.5 from HBM as a lone call (2.7 TB/s, 2.4 times its 7.7 us
+// at the measured copy rate); a CTA's loads, reduction and stores follow one
+// another, and two or three CTAs per SM hide that in part.
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -199,12 +200,6 @@ template <bool BF16>
 __device__ __forceinline__ float2 pair_to_float(uint32_t v) {
     if constexpr (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
     else return __half22float2(*reinterpret_cast<const __half2*>(&v));
-}
-
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
 }
 
 // the larger magnitude of two pairs, NaN if either is

@@ -31,13 +31,16 @@
 // last, in key order.  (A least number of steps per CTA does not pay: a prompt
 // of 256 rows of 8 heads took 49 us with four, 30 with two, 27 with one.)
 //
-// Measured: a prompt's last 4096 tokens of 16384 (32 heads over 4, dim 128, e4m3)
-// 0.964 ms, 998 TFLOP/s (60 % of the measured bf16 rate); five prompts of up to
-// 1777 tokens, window 1000 (24 heads over 8, dim 64, int8) 137 us, where half
-// of the steps have masks.  No single unit bounds it: without its exponentials
-// the first takes 1036 of then 1064 us, with an eighth of the products 1003,
+// Measured (lone calls): a prompt's last 4096 tokens of 16384 (32 heads over 4,
+// dim 128, e4m3) 1.03 ms, 935 TFLOP/s (56 % of the measured bf16 rate); in a graph,
+// inputs partly in L2, 0.99.  No single unit bounds it: without its
+// exponentials it takes 1036 of then 1064 us, with an eighth of the products 1003,
 // without loads 1077.  It is the chain of a tile's scores, weights, product
 // and next scores, with three warps per scheduler at 0.4 instructions a clock.
+// Five prompts of up to 1777 tokens, window 1000 (24 heads over 8, dim 64, int8)
+// 145 us, 138 in a graph: 4.7 items of 9 steps a CTA, and at each item's start
+// and end (queries in, first scores, last output out) the units wait; a third of the
+// CTAs' steps and a quarter of the warps' have masks.
 // Registers decide much: a converter or an issuing warp that spills costs up to 40 %.
 //
 // O is rescaled only when a row's maximum grows by more than 2^8 over the

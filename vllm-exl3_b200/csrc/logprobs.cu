@@ -20,8 +20,9 @@
 // token's log p has the digits of a plain fp32 softmax (an entry 10 above the best of
 // 131071 others: log p to 1e-7, with a lag of 16 and without this to 1.1e-6).
 // Cost: 64 rows with 5 alternatives 15.0 -> 15.6 us, 2048 rows 124.6 -> 125.7;
-// a lag of 8 would take 125.0.  Few rows: a row is split over CTAs and joined by the one that
-// ends last, always in the same order.
+// a lag of 8 would take 125.0.
+// Few rows: a row is split over CTAs and joined by the one that ends last,
+// always in the same order.
 //
 // Alternatives: entries are ordered by a 64-bit key (value, then lowest index
 // first).  The `top`-th largest of 32 thread groups' maxima bounds the answer
@@ -30,10 +31,11 @@
 // passes, some `top` entries.  The buffer holds whatever one such round can
 // yield; before it could overflow (many ties) it is reduced, which raises the bound.
 //
-// Measured: 2048 rows of 131072 bf16 100 us in a graph, 117 as a lone call from
-// HBM (4.6 TB/s, 70 % of the measured copy rate; exponential unit and ALU are
-// at 66 and 57 % of their rates); 64 rows with 5 alternatives 14 us, one row
-// of 100277 f32 with 20 alternatives 12 us (pass, join, selection one after another).
+// Measured: 2048 rows of 131072 bf16 104 us in a graph, 119 to 126 as a lone call
+// from HBM, by the card (4.3 to 4.5 TB/s, 66 to 69 % of the measured copy rate;
+// exponential unit and ALU are at 68 and 58 % of their rates); 64 rows with 5
+// alternatives 15.4 us, 14.2 in a graph, one row of 100277 f32 with 20
+// alternatives 12.5 us (pass, join, selection one after another).
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -76,12 +78,6 @@ struct LpStats {
     float m, s, w;  // m = -inf: nothing but -inf so far
     int above;
 };
-
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 
 __device__ __forceinline__ void lp_join(LpStats& a, const LpStats& b) {
     const float m = fmaxf(a.m, b.m);
